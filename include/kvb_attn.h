@@ -65,7 +65,8 @@ enum {
   KVB_STATUS_EPILOGUE_WAIT = 8,/* epilogue waited too long for the output     */
   KVB_STATUS_BAD_BLOCK = 16,    /* a block-table entry was outside the pool    */
   KVB_STATUS_BAD_LENGTH = 32,   /* a chunk's token count did not fit its blocks */
-  KVB_STATUS_PEER_WAIT = 64     /* a cross-GPU barrier waited too long for a peer */
+  KVB_STATUS_PEER_WAIT = 64,    /* a cross-GPU barrier waited too long for a peer */
+  KVB_STATUS_POOL_EMPTY = 128   /* a request's new blocks did not fit the free list */
 };
 
 /*
@@ -463,6 +464,191 @@ typedef struct KvbCacheBlendParams {
 } KvbCacheBlendParams;
 
 int kvb_cacheblend_fwd(const KvbCacheBlendParams* params, void* stream);
+
+/* ---- One decode step of a batch of requests over the block pool ----
+ *
+ * Four entry points, in the order of a step: block tables and slots of the
+ * step's new tokens, the new tokens' K/V into the pool, attention of each
+ * request's new token over its blocks, and the logits' processing.  None of
+ * them reads the device's data on the host, so a step can be captured in a
+ * CUDA graph.  The reference runs each of these on the host, per sequence and
+ * token (cpu_paged/paged_attn_cpu.py:33-163), and has no logits processing.
+ */
+
+/*
+ * Block tables and slot map of one step, on the device.  Row b holds
+ * seq_lens[b] tokens and gets new_lens[b] more (0: an idle row).  With have =
+ * ceil(seq_lens[b] / 16) and want = ceil((seq_lens[b] + new_lens[b]) / 16), the
+ * row's new blocks are popped from the end of the free list (free_blocks[0 ..
+ * *num_free)), rows in order, as BlockAllocator.allocate pops them
+ * (cpu_paged/block_allocator.py:85-96), and written to its table entries
+ * [have, want).  New token t of row b is packed at cu_new[b] + t: slots there =
+ * block * 16 + offset in the pool, positions = seq_lens[b] + t; entries from
+ * cu_new[batch] to max_new_tokens get slot -1 and position 0.
+ *
+ * A row that does not fit is left as it was: its length does not grow, its
+ * tokens' slots are -1, and its positions 0.  A row does not fit
+ *   - when seq_lens[b] < 0, or new_lens[b] < 0 or > max_new_tokens (such a row
+ *     takes no place in the packed arrays), or seq_lens[b] + new_lens[b] >
+ *     16 * max_blocks_per_seq, or its tokens end past max_new_tokens
+ *     (KVB_STATUS_BAD_LENGTH);
+ *   - when it needs new blocks and the blocks needed by the rows up to and
+ *     including it (whatever keeps them out, other than the reasons above)
+ *     exceed *num_free (KVB_STATUS_POOL_EMPTY).
+ * A table or free-list entry outside [0, num_blocks) gives its tokens slot -1
+ * and sets KVB_STATUS_BAD_BLOCK.  *num_free is read as clamped to [0, free_capacity].
+ *
+ * seq_lens_out and num_free_out may be seq_lens and num_free themselves (the
+ * step in place).  batch in [1, KVB_MAX_STEP_ROWS], block_size 16.
+ */
+#define KVB_MAX_STEP_ROWS 8192
+
+typedef struct KvbExtendTablesParams {
+  int32_t batch;
+  int32_t max_blocks_per_seq;
+  int32_t block_size;
+  int32_t num_blocks;
+  int32_t max_new_tokens;        /* length of slots and positions, >= 0 */
+  int32_t free_capacity;         /* length of free_blocks */
+  int64_t block_table_stride;    /* elements from one row's table to the next, >= max_blocks_per_seq */
+  int32_t* block_tables;         /* device [batch][block_table_stride] */
+  const int32_t* seq_lens;       /* device [batch] */
+  const int32_t* new_lens;       /* device [batch] */
+  const int32_t* free_blocks;    /* device [free_capacity] */
+  const int32_t* num_free;       /* device [1] */
+  int32_t* slots;                /* device [max_new_tokens], written */
+  int64_t* positions;            /* device [max_new_tokens], written */
+  int32_t* cu_new;               /* device [batch + 1], written */
+  int32_t* seq_lens_out;         /* device [batch], written */
+  int32_t* num_free_out;         /* device [1], written */
+  int32_t* status;
+} KvbExtendTablesParams;
+
+int kvb_extend_block_tables(const KvbExtendTablesParams* params, void* stream);
+
+/*
+ * The new tokens' K/V into a 16-bit pool (KVB_POOL_COMPUTE): token t's vectors
+ * of every KV head go to block slots[t] / 16, offset slots[t] % 16 (the device
+ * form of append_kv_to_blocks, cpu_paged/paged_attn_cpu.py:111-163).  Slot -1
+ * skips the token; a slot outside the pool skips it and sets
+ * KVB_STATUS_BAD_BLOCK.  The slots of one call must be distinct.  Nothing else
+ * of the pool is touched.  Element (t, h, d) of k_new sits at t *
+ * k_token_stride + h * k_head_stride + d; strides are multiples of 8 elements,
+ * pointers 16-byte aligned; the pool does not overlap the sources.
+ */
+typedef struct KvbAppendPagedParams {
+  int32_t head_dim;              /* a multiple of 8, up to 256 */
+  int32_t num_kv_heads;
+  int32_t num_tokens;
+  int32_t num_blocks;
+  const void* k_new;
+  const void* v_new;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  void* kv_pool;                 /* 16-bit [num_blocks][2][num_kv_heads][16][head_dim] */
+  const int32_t* slots;          /* device [num_tokens] */
+  int32_t* status;
+} KvbAppendPagedParams;
+
+int kvb_append_paged_kv(const KvbAppendPagedParams* params, void* stream);
+
+/*
+ * Attention of one new token per request over the request's blocks, read in
+ * place: query row b attends to the first seq_lens[b] tokens of its block table
+ * (which include the new token's own K/V once appended).  GQA, any group size.
+ * A row with seq_lens[b] <= 0 gets O = 0 and LSE = -inf; a length above 16 *
+ * max_blocks_per_seq is cut to that and sets KVB_STATUS_BAD_LENGTH.  Pool
+ * formats as KvbPagedPrefillParams; int8 pools are read with their float16
+ * scales (k_scale16 [num_blocks][num_kv_heads][16], v_scale16
+ * [num_blocks][num_kv_heads][head_dim]), the products taken in float32 without
+ * rounding the dequantised values.  Blocks outside [0, num_blocks) read as
+ * zeros and set KVB_STATUS_BAD_BLOCK.  Table entries past a row's last block
+ * and pool slots past its last token are never used, whatever they hold.
+ *
+ * The rows' blocks are divided evenly over the GPU's warps, whatever the
+ * lengths (device data); requests that end up on several CTAs are joined by a
+ * second launch.  workspace: kvb_paged_decode_workspace_bytes(params) bytes
+ * (-1: invalid params), 16-byte aligned, no initialisation needed; calls that
+ * may overlap on the GPU must not share one.  max_seq_len (0: unknown) is a hint
+ * that only chooses the launch shape; any value gives right results.
+ */
+typedef struct KvbPagedDecodeParams {
+  int32_t dtype;
+  int32_t head_dim;              /* 64, 96 or 128 */
+  int32_t batch;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t block_size;            /* 16 */
+  int32_t pool_format;           /* KVB_POOL_* */
+  float softmax_scale;
+  const void* q;                 /* element (b, h, d) at b * q_batch_stride + h * q_head_stride + d */
+  void* o;
+  float* lse;                    /* optional, (b, h) at b * lse_batch_stride + h */
+  int64_t q_batch_stride, q_head_stride;
+  int64_t o_batch_stride, o_head_stride;
+  int64_t lse_batch_stride;
+  const void* kv_pool;           /* [num_blocks][2][num_kv_heads][16][head_dim] */
+  const void* k_scale16;
+  const void* v_scale16;
+  int32_t num_blocks;
+  int32_t max_blocks_per_seq;
+  int64_t block_table_stride;
+  const int32_t* block_tables;
+  const int32_t* seq_lens;
+  int32_t max_seq_len;
+  int32_t reserved0;
+  int32_t* status;
+  void* workspace;
+  int64_t workspace_bytes;
+} KvbPagedDecodeParams;
+
+int64_t kvb_paged_decode_workspace_bytes(const KvbPagedDecodeParams* params);
+int kvb_paged_decode_fwd(const KvbPagedDecodeParams* params, void* stream);
+
+/*
+ * Logits of a step, processed in one pass.  With x the row's logits in float32,
+ * seen = the tokens in token_ids[b][0 .. total_lens[b]), count = how often a token
+ * occurs in token_ids[b][prompt_lens[b] .. total_lens[b]):
+ *   x = x > 0 ? x / r : x * r           for seen tokens     (repetition_penalty)
+ *   x = x - frequency * count           (frequency_penalty)
+ *   x = x - presence   where count > 0  (presence_penalty)
+ *   x = x + bias       for each entry of the row's bias list, in its order
+ *   x = x / max(temperature, 1e-5)
+ *   x = -inf           where the token's bit of allowed_mask is clear
+ * Each step is left out where its arrays are NULL.  Token ids outside [0, vocab)
+ * in the history or the bias list are ignored; total_lens is clamped to [0,
+ * history_len], prompt_lens to [0, total].  A row whose mask leaves nothing is all -inf.
+ * Output: float32, or the logits' dtype rounded once at the end; o may be the
+ * logits themselves (same dtype and stride).  No counterpart in the reference,
+ * which samples from softmax(logits / max(temperature, 1e-5)).
+ */
+enum { KVB_DTYPE_FP32 = 2 }; /* logits only */
+
+typedef struct KvbLogitsParams {
+  int32_t dtype;                 /* of logits: KVB_DTYPE_BF16, _FP16 or _FP32 */
+  int32_t out_dtype;             /* KVB_DTYPE_FP32 or dtype */
+  int32_t batch;                 /* <= 65535 */
+  int32_t vocab;
+  int32_t history_len;           /* columns of token_ids */
+  int32_t num_bias;              /* columns of bias_ids */
+  const void* logits;
+  void* out;
+  int64_t logits_stride, out_stride;
+  const int32_t* token_ids;      /* device [batch] rows, history_stride apart, or NULL */
+  int64_t history_stride;
+  const int32_t* prompt_lens;    /* device [batch] or NULL (0) */
+  const int32_t* total_lens;     /* device [batch] */
+  const float* repetition_penalty;  /* device [batch] or NULL, as the next three */
+  const float* frequency_penalty;
+  const float* presence_penalty;
+  const float* temperature;
+  const int32_t* bias_ids;       /* device [batch][num_bias]; negative entries are padding */
+  const float* bias_values;      /* device [batch][num_bias] */
+  const uint32_t* allowed_mask;  /* device [batch][mask_stride]: bit v % 32 of word v / 32 */
+  int64_t mask_stride;           /* words, >= ceil(vocab / 32) */
+} KvbLogitsParams;
+
+int kvb_process_logits(const KvbLogitsParams* params, void* stream);
 
 /* Human-readable reason for the last non-zero return on this host thread. */
 const char* kvb_last_error(void);

@@ -23,6 +23,9 @@ KVB_ERR_CUDA = -1
 KVB_NOALLOC_SCRATCH_BYTES = 32 << 20
 KVB_POOL_INT8_KIVI, KVB_POOL_COMPUTE = 0, 1
 KVB_STATUS_BAD_BLOCK, KVB_STATUS_BAD_LENGTH, KVB_STATUS_PEER_WAIT = 16, 32, 64
+KVB_STATUS_POOL_EMPTY = 128
+KVB_DTYPE_FP32 = 2          # logits only
+KVB_MAX_STEP_ROWS = 8192
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
@@ -129,6 +132,61 @@ class KvbQuantizeStoreBatch(ctypes.Structure):
     ]
 
 
+class KvbExtendTablesParams(ctypes.Structure):
+    """Mirror of ``KvbExtendTablesParams``."""
+
+    _fields_ = [
+        ("batch", _i32), ("max_blocks_per_seq", _i32), ("block_size", _i32), ("num_blocks", _i32),
+        ("max_new_tokens", _i32), ("free_capacity", _i32), ("block_table_stride", _i64),
+        ("block_tables", _vp), ("seq_lens", _vp), ("new_lens", _vp), ("free_blocks", _vp),
+        ("num_free", _vp), ("slots", _vp), ("positions", _vp), ("cu_new", _vp),
+        ("seq_lens_out", _vp), ("num_free_out", _vp), ("status", _vp),
+    ]
+
+
+class KvbAppendPagedParams(ctypes.Structure):
+    """Mirror of ``KvbAppendPagedParams``."""
+
+    _fields_ = [
+        ("head_dim", _i32), ("num_kv_heads", _i32), ("num_tokens", _i32), ("num_blocks", _i32),
+        ("k_new", _vp), ("v_new", _vp),
+        ("k_token_stride", _i64), ("k_head_stride", _i64),
+        ("v_token_stride", _i64), ("v_head_stride", _i64),
+        ("kv_pool", _vp), ("slots", _vp), ("status", _vp),
+    ]
+
+
+class KvbPagedDecodeParams(ctypes.Structure):
+    """Mirror of ``KvbPagedDecodeParams``."""
+
+    _fields_ = [
+        ("dtype", _i32), ("head_dim", _i32), ("batch", _i32), ("num_q_heads", _i32),
+        ("num_kv_heads", _i32), ("block_size", _i32), ("pool_format", _i32),
+        ("softmax_scale", _f32),
+        ("q", _vp), ("o", _vp), ("lse", _vp),
+        ("q_batch_stride", _i64), ("q_head_stride", _i64),
+        ("o_batch_stride", _i64), ("o_head_stride", _i64), ("lse_batch_stride", _i64),
+        ("kv_pool", _vp), ("k_scale16", _vp), ("v_scale16", _vp),
+        ("num_blocks", _i32), ("max_blocks_per_seq", _i32), ("block_table_stride", _i64),
+        ("block_tables", _vp), ("seq_lens", _vp), ("max_seq_len", _i32), ("reserved0", _i32),
+        ("status", _vp), ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
+class KvbLogitsParams(ctypes.Structure):
+    """Mirror of ``KvbLogitsParams``."""
+
+    _fields_ = [
+        ("dtype", _i32), ("out_dtype", _i32), ("batch", _i32), ("vocab", _i32),
+        ("history_len", _i32), ("num_bias", _i32), ("logits", _vp), ("out", _vp),
+        ("logits_stride", _i64), ("out_stride", _i64),
+        ("token_ids", _vp), ("history_stride", _i64), ("prompt_lens", _vp), ("total_lens", _vp),
+        ("repetition_penalty", _vp), ("frequency_penalty", _vp), ("presence_penalty", _vp),
+        ("temperature", _vp), ("bias_ids", _vp), ("bias_values", _vp),
+        ("allowed_mask", _vp), ("mask_stride", _i64),
+    ]
+
+
 def pointer_array(ptrs):
     """A ctypes ``void*[n]`` of device addresses (keep it alive across the call)."""
     arr = (ctypes.c_void_p * len(ptrs))(*[int(p) if p else None for p in ptrs])
@@ -189,6 +247,16 @@ def load() -> ctypes.CDLL:
         lib.kvb_quantize_store_batch.restype = ctypes.c_int
         lib.kvb_cacheblend_fwd.argtypes = [ctypes.POINTER(KvbCacheBlendParams), _vp]
         lib.kvb_cacheblend_fwd.restype = ctypes.c_int
+        lib.kvb_extend_block_tables.argtypes = [ctypes.POINTER(KvbExtendTablesParams), _vp]
+        lib.kvb_extend_block_tables.restype = ctypes.c_int
+        lib.kvb_append_paged_kv.argtypes = [ctypes.POINTER(KvbAppendPagedParams), _vp]
+        lib.kvb_append_paged_kv.restype = ctypes.c_int
+        lib.kvb_paged_decode_fwd.argtypes = [ctypes.POINTER(KvbPagedDecodeParams), _vp]
+        lib.kvb_paged_decode_fwd.restype = ctypes.c_int
+        lib.kvb_paged_decode_workspace_bytes.argtypes = [ctypes.POINTER(KvbPagedDecodeParams)]
+        lib.kvb_paged_decode_workspace_bytes.restype = ctypes.c_int64
+        lib.kvb_process_logits.argtypes = [ctypes.POINTER(KvbLogitsParams), _vp]
+        lib.kvb_process_logits.restype = ctypes.c_int
         lib.kvb_last_error.argtypes = []
         lib.kvb_last_error.restype = ctypes.c_char_p
         lib.kvb_abi_version.argtypes = []
