@@ -1,108 +1,872 @@
 // kvb_paged_decode_fwd: attention of one new token per request over its blocks of the
-// pool, sm_100a.  O = softmax(q K^T s) V with GQA; the blocks are read in place.
+// pool, sm_100a.  O = softmax(q K^T s) V with GQA, the 16-token blocks read in place.
+//
+// What bounds it: K and V are read once for 2 * (query heads per KV head) FLOP per byte
+// (16-bit pool), so HBM, up to the widest groups; short rows are latency.  The tensor
+// cores run through mma.sync: a tcgen05 tile has at least 64 rows of which a group of 8
+// query heads would fill an eighth, its accumulators live in TMEM behind a
+// tcgen05.ld, and one thread issues for the CTA; here every warp is its own pipeline
+// and needs about a tenth of the issue slots that the loads leave it.
+//
+// Split: a unit of work is one block of one (request, KV head, head tile).  The units of
+// all items, laid end to end, are divided evenly over the warps of one CTA per SM from
+// the lengths on the device, so ragged batches balance to a block without the host
+// knowing a length.  A warp walks its units alone: lane 0 brings each block's K and V
+// by TMA into the warp's ring of stages, several blocks ahead, through the block table;
+// no CTA-wide step sits in the loop.  Items that a warp holds whole it writes itself;
+// the pieces at its range's ends are joined in shared memory at the CTA's end, and what
+// still spans CTAs goes to the workspace for a second launch.  Short tables take one
+// CTA per item instead, whose warps split the item and never need that launch.
+//
+// Arithmetic (per block, tokens on the MMA's rows, query heads on its columns):
+//   S^T = K Q^T; online softmax down the rows against a maximum that is raised only when
+//   a score passes it by 2^8 (one vote instead of shuffles); O^T += V^T P^T.
+// P is carried in two 16-bit halves (p = hi + lo), so the weights keep 16 bits and the
+// result's error is that of its final rounding; the second MMA is free here.
+// KIVI int8 pools: codes are exact in float16, so Q (scaled by a power of two per row)
+// and P are float16 and the scales act in float32 on S (K, per token) and on each
+// block's product (V, per channel): nothing is rounded to 16 bits in between.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <mutex>
 #include <string>
+#include <type_traits>
 
 #include "kvb_attn.h"
+#include "kvb_sm100_ptx.cuh"
 
 int kvb_detail_fail(int code, const std::string& msg);
 
 namespace kvb_pd {
 
+using namespace kvb::ptx;
+
 int fail(int code, const std::string& msg) { return kvb_detail_fail(code, msg); }
 
+constexpr int kSms = 148;
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr float kRaise = 8.f;              // log2 units a score may pass the running maximum by
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr int kItemBlocks = 64;            // tables up to this wide take one CTA per item
+constexpr int kMinUnits = 8;               // blocks per CTA below which fewer CTAs share them
+constexpr int kSplitRows = 4096;           // most rows of a split launch (prefix sums in shared memory)
+
 struct Args {
-  int num_q_heads, num_kv_heads, num_blocks, width;
-  float scale;
+  int batch, num_q_heads, num_kv_heads, num_blocks, width;
+  int group, tiles, items;                 // tiles: head tiles per KV head; items = kv heads * tiles
+  int ctas;                                // split launch: CTAs sharing the units
+  float scale_log2;
   const void* q;
   void* o;
   float* lse;
   int64_t q_bs, q_hs, o_bs, o_hs, lse_bs, table_stride;
-  const void* pool;
   const __half* k_scale;
   const __half* v_scale;
   const int32_t* tables;
   const int32_t* lens;
   int32_t* status;
+  float* part;                             // [ctas][2][NH * D + 2 * NH]
+  int4* owner;                             // [ctas]: request, item, CTAs it spans (0: none)
 };
 
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_f32(int8_t x) { return (float)x; }
-__device__ __forceinline__ void from_f32(__half* p, float x) { *p = __float2half_rn(x); }
-__device__ __forceinline__ void from_f32(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+// ---- warp-level primitives ------------------------------------------------------------------
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float lds_half(uint32_t addr) {
+  uint16_t h;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(addr) : "memory");
+  return __half2float(__ushort_as_half(h));
+}
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
 
-// One CTA per (query head, request): 8 warps take tokens in turn, a lane holds D / 32
-// features; running maximum and sum per warp, joined at the end.
-template <typename T, typename P, int D>
-__global__ void __launch_bounds__(256) kvb_paged_decode_kernel(const Args a) {
-  constexpr int N = D / 32;
-  __shared__ float sm_m[8], sm_l[8], sm_o[8][D];
-  const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int kvh = h / (a.num_q_heads / a.num_kv_heads);
-  int len = a.lens[b];
-  if (len > a.width * 16) {
-    len = a.width * 16;
-    if (a.status && threadIdx.x == 0) atomicOr(a.status, KVB_STATUS_BAD_LENGTH);
+// D (16 x 8, float32) += A (16 x 16) B (16 x 8), both operands in E
+template <typename E>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<E, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+                 "{%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+                 "{%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename E>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {   // lo in the low half
+  if constexpr (std::is_same<E, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
-  float q[N], o[N];
-  const T* qp = static_cast<const T*>(a.q) + b * a.q_bs + h * a.q_hs;
-  for (int i = 0; i < N; ++i) q[i] = to_f32(qp[i * 32 + lane]) * a.scale, o[i] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  for (int t = warp; t < len; t += 8) {
-    const int id = a.tables[b * a.table_stride + (t >> 4)];
-    const bool ok = id >= 0 && id < a.num_blocks;
-    if (!ok && a.status) atomicOr(a.status, KVB_STATUS_BAD_BLOCK);
-    float x = 0.f, v[N];
-    for (int i = 0; i < N; ++i) v[i] = 0.f;
-    if (ok) {
-      const int64_t at = ((int64_t)id * 2 * a.num_kv_heads + kvh) * 16 + (t & 15);
-      const P* kp = static_cast<const P*>(a.pool) + at * D;
-      const P* vp = kp + (int64_t)a.num_kv_heads * 16 * D;
-      for (int i = 0; i < N; ++i) x += q[i] * to_f32(kp[i * 32 + lane]);
-      for (int s = 16; s; s >>= 1) x += __shfl_xor_sync(~0u, x, s);
-      const int64_t bh = (int64_t)id * a.num_kv_heads + kvh;
-      if (a.k_scale) x *= __half2float(a.k_scale[bh * 16 + (t & 15)]);
-      for (int i = 0; i < N; ++i) {
-        v[i] = to_f32(vp[i * 32 + lane]);
-        if (a.v_scale) v[i] *= __half2float(a.v_scale[bh * D + i * 32 + lane]);
+}
+template <typename E>
+__device__ __forceinline__ float2 unpack(uint32_t u) {
+  if constexpr (std::is_same<E, __half>::value) {
+    __half2 h;
+    memcpy(&h, &u, 4);
+    return __half22float2(h);
+  } else {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+}
+
+// Four int8 codes (biased by 128) to float16 pairs, exactly: a byte under the exponent of
+// 1024 is 1024 + code + 128.
+__device__ __forceinline__ uint32_t codes_to_half(uint32_t biased, uint32_t select) {
+  const uint32_t u = __byte_perm(biased, 0x64646464u, select);
+  __half2 h;
+  memcpy(&h, &u, 4);
+  const __half2 bias = __floats2half2_rn(1152.f, 1152.f);
+  h = __hsub2(h, bias);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Waits for a phase; false after 2 s (the status word says so).
+__device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity, int32_t* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (globaltimer_ns() - t0 > kWaitNs) {
+      if (status) atomicOr(status, KVB_STATUS_LOAD_WAIT);
+      return false;
+    }
+  }
+  return true;
+}
+
+// ---- geometry -------------------------------------------------------------------------------
+template <int D, bool I8, int NT>
+struct Geo {
+  static constexpr int NH = 8 * NT;                          // query heads per item
+  static constexpr int DP = I8 ? (D == 64 ? 64 : 128) : D;   // features the MMAs cover
+  static constexpr int HALVES = I8 ? 1 : (D + 63) / 64;      // TMA boxes per block
+  static constexpr int ROW = I8 ? DP : 128;                  // bytes of a box row = its swizzle
+  static constexpr int BOX = 2 * 16 * ROW;                   // K and V, 16 tokens
+  static constexpr int STAGE = HALVES * BOX;
+  static constexpr int SCALES = I8 ? 32 + 256 : 0;           // K then V scales of the block
+  static constexpr int OS = D + 4;                           // piece row: conflict-free columns
+  static constexpr int PIECE = (NH * OS + 2 * NH) * 4;
+  // alignment, pieces, notes, warp sums; per stage: data, scales, barrier
+  static constexpr int FIXED = 1024 + kWarps * PIECE + kWarps * 2 * 16 + kWarps * 4;
+  static constexpr int PER_STAGE = kWarps * (STAGE + SCALES + 8);
+  static constexpr int FIT = (232448 - FIXED) / PER_STAGE;
+  static constexpr int NS = FIT < 6 ? FIT : 6;               // stages per warp
+  static constexpr int SMEM = FIXED + NS * PER_STAGE;
+  static constexpr int PART = NH * D + 2 * NH;               // floats of a workspace piece
+  static_assert(NS >= 2, "at least two stages per warp");
+  static_assert(PIECE <= NS * STAGE, "a second piece goes over the warp's stages");
+  static_assert(kWarps * PIECE / 4 >= kSplitRows, "prefix sums share the pieces' room");
+};
+
+__device__ __forceinline__ int row_len(const Args& a, int b) {
+  const int len = a.lens[b];
+  return len < 0 ? 0 : (int)min((int64_t)len, (int64_t)a.width * 16);
+}
+
+// One item's running state in a warp: maximum (log2), sum and O^T, for NT tiles of 8 heads;
+// lane (r, c) = (lane / 4, lane % 4) holds heads 2c, 2c + 1 of each tile.
+template <int MT, int NT>
+struct State {
+  float m[NT][2], l[NT][2], acc[NT][MT][4];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      m[t][0] = m[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[t][j][0] = acc[t][j][1] = acc[t][j][2] = acc[t][j][3] = 0.f;
+    }
+  }
+};
+
+template <typename T, int D, bool I8, int NT, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 1)
+    kvb_paged_decode_kernel(const __grid_constant__ CUtensorMap map, const Args a) {
+  using G = Geo<D, I8, NT>;
+  using E = typename std::conditional<I8, __half, T>::type;   // MMA operand type
+  constexpr int MT = G::DP / 16, KS = G::DP / 16, NS = G::NS, NH = G::NH;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
+  uint8_t* ring = smem + warp * NS * G::STAGE;
+  uint8_t* scales = smem + kWarps * NS * G::STAGE + warp * NS * G::SCALES;
+  uint8_t* after = smem + kWarps * NS * (G::STAGE + G::SCALES);
+  float* piece0 = reinterpret_cast<float*>(after);                     // [kWarps] first pieces
+  int32_t* prefix = reinterpret_cast<int32_t*>(after);                 // before any piece is written
+  uint64_t* bars = reinterpret_cast<uint64_t*>(after + kWarps * G::PIECE);
+  // [kWarps][2] pieces: request (-1: none), item, blocks, CTAs spanned if the item begins here
+  int4* notes = reinterpret_cast<int4*>(bars + kWarps * NS);
+  int32_t* wsum = reinterpret_cast<int32_t*>(notes + 2 * kWarps);
+  const uint32_t ring_u = smem_u32(ring), scales_u = smem_u32(scales), bar_u = smem_u32(bars + warp * NS);
+
+  if (lane == 0) {
+    for (int s = 0; s < NS; ++s) mbar_init(bar_u + 8 * s, 1);
+    fence_mbar_init();
+    notes[2 * warp].x = notes[2 * warp + 1].x = -1;
+    prefetch_tmap(&map);
+  }
+  __syncwarp();
+  griddep_wait();
+  griddep_launch_dependents();
+
+  // ---- this warp's units -------------------------------------------------------------------
+  int b, j, blk, nb;            // the unit to consume: request, item of the request, block
+  int64_t left;                 // units of this warp
+  int64_t u = 0, total = 0;     // split launch: the unit's place among all rows' units
+  int ctas = 1;                 // split launch: CTAs that get units
+  if constexpr (SPLIT) {
+    // exclusive prefix sums of the rows' blocks, in shared memory
+    int base = 0, err = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+      const int bb = b0 + tid;
+      int n = 0;
+      if (bb < a.batch) {
+        n = (row_len(a, bb) + 15) >> 4;
+        if ((int64_t)a.lens[bb] > (int64_t)a.width * 16) err = KVB_STATUS_BAD_LENGTH;
+      }
+      int x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(~0u, x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane == 31) wsum[warp] = x;
+      __syncthreads();
+      int sum = 0;
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) x += wsum[w];
+        sum += wsum[w];
+      }
+      if (bb < a.batch) prefix[bb] = base + x;      // inclusive
+      base += sum;
+      __syncthreads();
+    }
+    if (err && blockIdx.x == 0 && a.status) atomicOr(a.status, err);
+    total = (int64_t)base * a.items;
+    // no CTA without a unit, so an item's CTAs are consecutive
+    ctas = (int)min((int64_t)a.ctas, (total + kMinUnits - 1) / kMinUnits);
+    const int64_t workers = (int64_t)ctas * kWarps, me = (int64_t)blockIdx.x * kWarps + warp;
+    left = 0;
+    if ((int)blockIdx.x < ctas) {
+      u = me * total / workers;
+      left = (me + 1) * total / workers - u;
+    }
+    b = j = blk = nb = 0;
+    if (left > 0) {
+      int lo = 0, hi = a.batch - 1;                 // first row whose inclusive sum passes u
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if ((int64_t)prefix[mid] * a.items > u) hi = mid; else lo = mid + 1;
+      }
+      b = lo;
+      const int before = lo ? prefix[lo - 1] : 0;
+      nb = prefix[lo] - before;
+      const int64_t rel = u - (int64_t)before * a.items;
+      j = (int)(rel / nb);
+      blk = (int)(rel - (int64_t)j * nb);
+    }
+    __syncthreads();                                // the pieces' room is free from here
+  } else {
+    b = blockIdx.x / a.items;
+    j = blockIdx.x - b * a.items;
+    nb = (row_len(a, b) + 15) >> 4;
+    if (tid == 0 && j == 0 && (int64_t)a.lens[b] > (int64_t)a.width * 16 && a.status)
+      atomicOr(a.status, KVB_STATUS_BAD_LENGTH);
+    blk = (int)((int64_t)nb * warp / kWarps);
+    left = (int)((int64_t)nb * (warp + 1) / kWarps) - blk;
+  }
+
+  // ---- producer: this warp's loads, NS units ahead -------------------------------------------
+  int pb = b, pj = j, pblk = blk, pnb = nb;
+  int64_t to_issue = left;
+  int ids = 0, cached_b = -1, cached_c = -1;        // 32 table entries, one per lane
+  uint32_t issued = 0;
+  auto issue = [&]() {
+    const int chunk = pblk >> 5;
+    if (pb != cached_b || chunk != cached_c) {
+      const int at = chunk * 32 + lane;
+      ids = at < pnb ? a.tables[pb * a.table_stride + at] : 0;
+      cached_b = pb;
+      cached_c = chunk;
+    }
+    const int id = __shfl_sync(~0u, ids, pblk & 31);
+    const uint32_t s = issued % NS;
+    const uint32_t bar = bar_u + 8 * s, dst = ring_u + s * G::STAGE;
+    const int kvh = a.tiles == 1 ? pj : pj / a.tiles;
+    const bool ok = (unsigned)id < (unsigned)a.num_blocks;
+    if (lane == 0) {
+      if constexpr (I8) {
+        const uint32_t sc = scales_u + s * G::SCALES;
+        mbar_arrive_expect_tx(bar, G::STAGE + (ok ? 32 + 2 * D : 0));
+        tma_load_4d(dst, &map, 0, kvh * 16, 0, ok ? id : -1, bar);
+        if (ok) {
+          const int64_t bh = (int64_t)id * a.num_kv_heads + kvh;
+          bulk_load(sc, a.k_scale + bh * 16, 32, bar);
+          bulk_load(sc + 32, a.v_scale + bh * D, 2 * D, bar);
+        }
+      } else {
+        mbar_arrive_expect_tx(bar, G::STAGE);
+#pragma unroll
+        for (int h = 0; h < G::HALVES; ++h)
+          tma_load_4d(dst + h * G::BOX, &map, h * 64, kvh * 16, 0, ok ? id : -1, bar);
       }
     }
-    const float mn = fmaxf(m, x), base = mn == -INFINITY ? 0.f : mn;
-    const float f = expf(m - base), p = expf(x - base);
-    m = mn;
-    l = l * f + p;
-    for (int i = 0; i < N; ++i) o[i] = o[i] * f + p * v[i];
+    if (!ok) {                                      // reads as zeros
+      if (I8) {
+        for (int i = lane; i < G::SCALES / 4; i += 32) sts32(scales_u + s * G::SCALES + 4 * i, 0u);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (lane == 0 && a.status) atomicOr(a.status, KVB_STATUS_BAD_BLOCK);
+    }
+    ++issued;
+    --to_issue;
+    if (++pblk == pnb && to_issue > 0) {
+      pblk = 0;
+      if (++pj == a.items) {
+        pj = 0;
+        do { pnb = (row_len(a, ++pb) + 15) >> 4; } while (pnb == 0);
+      }
+    }
+  };
+#pragma unroll 1
+  for (int s = 0; s < NS && to_issue > 0; ++s) issue();
+
+  // rows without tokens: zeros and -inf
+  if constexpr (SPLIT) {
+    for (int z = blockIdx.x; z < a.batch; z += a.ctas)
+      if (a.lens[z] <= 0)
+        for (int i = tid; i < a.num_q_heads * D; i += kThreads) {
+          const int h = i / D, d = i - h * D;
+          static_cast<T*>(a.o)[z * a.o_bs + h * a.o_hs + d] = T(0.f);
+          if (d == 0 && a.lse) a.lse[z * a.lse_bs + h] = -INFINITY;
+        }
+  } else if (nb == 0) {
+    const int kvh = j / a.tiles, h0 = kvh * a.group + (j - kvh * a.tiles) * NH;
+    const int n = min(NH, (kvh + 1) * a.group - h0);
+    for (int i = tid; i < n * D; i += kThreads) {
+      const int h = h0 + i / D, d = i % D;
+      static_cast<T*>(a.o)[b * a.o_bs + h * a.o_hs + d] = T(0.f);
+      if (d == 0 && a.lse) a.lse[b * a.lse_bs + h] = -INFINITY;
+    }
+    return;
   }
-  if (lane == 0) sm_m[warp] = m, sm_l[warp] = l;
-  for (int i = 0; i < N; ++i) sm_o[warp][i * 32 + lane] = o[i];
+
+  // ---- consumer ----------------------------------------------------------------------------
+  State<MT, NT> st;
+  uint32_t qf[NT][KS][2];
+  float qx[NT][2];              // what turns S into log2 scores, per head of this lane's columns
+  uint32_t used = 0;
+  int pieces = 0;
+  bool alive = true;
+  while (left > 0 && alive) {
+    // one item, or the part of it in this warp's range
+    const int kvh = a.tiles == 1 ? j : j / a.tiles;
+    const int h0 = kvh * a.group + (j - kvh * a.tiles) * NH;
+    const int heads = min(NH, (kvh + 1) * a.group - h0);
+    const int len = row_len(a, b);
+    const int first = blk;
+    const int stop = (int)min((int64_t)nb, blk + left);
+    st.clear();
+    const T* q = static_cast<const T*>(a.q) + b * a.q_bs + (int64_t)h0 * a.q_hs;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const bool on = t * 8 + r < heads;
+      const T* row = q + (on ? t * 8 + r : 0) * a.q_hs;
+      if constexpr (!I8) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            qf[t][ks][h] = on ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + h * 8 + 2 * c) : 0u;
+        qx[t][0] = qx[t][1] = a.scale_log2;
+      } else {
+        // features in the order the K codes are read: lane c's 16-byte pieces c, c + 4
+        float top = 0.f;
+        uint2 raw[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const int d = 16 * (c + 4 * (ks >> 2)) + 4 * (ks & 3);
+          raw[ks] = on && d < D ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0u, 0u);
+          const float2 x = unpack<T>(raw[ks].x), y = unpack<T>(raw[ks].y);
+          top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(y.x), fabsf(y.y)));
+        }
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+        // a power of two that brings the row's largest magnitude into [1, 4)
+        const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 254);
+        const float f = __uint_as_float((uint32_t)max(254 - e, 1) << 23);
+        const float inv = __uint_as_float((uint32_t)min(e, 253) << 23);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const float2 x = unpack<T>(raw[ks].x), y = unpack<T>(raw[ks].y);
+          qf[t][ks][0] = pack<__half>(x.x * f, x.y * f);
+          qf[t][ks][1] = pack<__half>(y.x * f, y.y * f);
+        }
+        qx[t][0] = __shfl_sync(~0u, inv, 8 * c) * a.scale_log2;
+        qx[t][1] = __shfl_sync(~0u, inv, 8 * c + 4) * a.scale_log2;
+      }
+    }
+
+#pragma unroll 1
+    for (; blk < stop; ++blk) {
+      const uint32_t s = used % NS, base = ring_u + s * G::STAGE, sc = scales_u + s * G::SCALES;
+      if (!wait_full(bar_u + 8 * s, (used / NS) & 1, a.status)) {
+        alive = false;
+        break;
+      }
+      const int valid = len - blk * 16;             // >= 1; below 16 in the row's last block
+      // S^T: two chains of MMAs
+      float sa[NT][2][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sa[t][0][i] = sa[t][1][i] = 0.f;
+      if constexpr (!I8) {
+        const uint32_t ka = base + ((lane & 7) + ((lane >> 3) & 1) * 8) * 128;
+        const uint32_t kx = (((lane >> 4) ^ (lane & 7)) << 4);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t f[4];
+          ldsm4(ka + (ks >> 2) * G::BOX + (kx ^ ((ks & 3) << 5)), f);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma<E>(sa[t][ks & 1], f, qf[t][ks][0], qf[t][ks][1]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < KS / 4; ++i) {
+          const uint32_t at = G::ROW == 128 ? (((c + 4 * i) ^ (r & 7)) << 4) : ((c ^ ((r >> 1) & 3)) << 4);
+          const uint4 x = lds128(base + r * G::ROW + at), y = lds128(base + (r + 8) * G::ROW + at);
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t p = xs[w] ^ 0x80808080u, v = ys[w] ^ 0x80808080u;
+            const uint32_t f[4] = {codes_to_half(p, 0x4140), codes_to_half(v, 0x4140),
+                                   codes_to_half(p, 0x4342), codes_to_half(v, 0x4342)};
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              mma<E>(sa[t][w & 1], f, qf[t][4 * i + w][0], qf[t][4 * i + w][1]);
+          }
+        }
+      }
+      // log2 scores: [t][0..1] token r, [2..3] token r + 8; heads 2c, 2c + 1
+      float x[NT][4];
+      float k0 = 1.f, k1 = 1.f;
+      if constexpr (I8) {
+        k0 = lds_half(sc + 2 * r);
+        k1 = lds_half(sc + 2 * (r + 8));
+      }
+      bool raise = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = sa[t][0][i] + sa[t][1][i];
+          v *= I8 ? qx[t][i & 1] * (i < 2 ? k0 : k1) : qx[t][i & 1];
+          if (r + (i < 2 ? 0 : 8) >= valid) v = -INFINITY;
+          x[t][i] = v;
+          raise |= v > st.m[t][i & 1] + kRaise;
+        }
+      if (__any_sync(~0u, raise)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float top = fmaxf(x[t][i], x[t][i + 2]);
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+            top = fmaxf(top, st.m[t][i]);
+            const float f = top == -INFINITY ? 1.f : ex2(st.m[t][i] - top);
+            st.m[t][i] = top;
+            st.l[t][i] *= f;
+#pragma unroll
+            for (int jj = 0; jj < MT; ++jj) {
+              st.acc[t][jj][i] *= f;
+              st.acc[t][jj][i + 2] *= f;
+            }
+          }
+      }
+      // weights, in two 16-bit halves, transposed to the MMA's B operand
+      uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float m = st.m[t][i & 1];
+          p[i] = ex2(x[t][i] - (m == -INFINITY ? 0.f : m));
+          st.l[t][i & 1] += p[i];
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t hi = pack<E>(p[2 * h], p[2 * h + 1]);
+          const float2 back = unpack<E>(hi);
+          ph[t][h] = transpose8(hi);
+          pl[t][h] = transpose8(pack<E>(p[2 * h] - back.x, p[2 * h + 1] - back.y));
+        }
+      }
+      // O^T += V^T P^T
+      if constexpr (!I8) {
+        const uint32_t va = base + 2048 + ((lane & 7) + (lane >> 4) * 8) * 128;
+        const uint32_t vx = ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+        // slots past the row's end may hold anything: their V is cleared, not only their weight
+        uint32_t m01 = ~0u, m89 = ~0u;
+        if (valid < 16) {
+          m01 = (2 * c < valid ? 0xffffu : 0u) | (2 * c + 1 < valid ? 0xffff0000u : 0u);
+          m89 = (2 * c + 8 < valid ? 0xffffu : 0u) | (2 * c + 9 < valid ? 0xffff0000u : 0u);
+        }
+#pragma unroll
+        for (int jj = 0; jj < MT; ++jj) {
+          uint32_t f[4];
+          ldsm4t(va + (jj >> 2) * G::BOX + (vx ^ ((jj & 3) << 5)), f);
+          f[0] &= m01;
+          f[1] &= m01;
+          f[2] &= m89;
+          f[3] &= m89;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            mma<E>(st.acc[t][jj], f, ph[t][0], ph[t][1]);
+            mma<E>(st.acc[t][jj], f, pl[t][0], pl[t][1]);
+          }
+        }
+      } else {
+        // lane r reads features [PR r, PR r + PR) of tokens 2c, 2c + 1, 2c + 8, 2c + 9; MMA row
+        // r of tile jj is feature PR r + 2 jj, row r + 8 the next one
+        constexpr int W = G::DP / 32;               // 32-bit words of a lane's features
+        uint32_t v[4][W];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int row = 2 * c + (k & 1) + (k >> 1) * 8;
+          const uint32_t at = base + 16 * G::ROW + row * G::ROW;
+          if constexpr (G::ROW == 128) {
+            const uint4 z = lds128(at + ((r ^ (row & 7)) << 4));
+            v[k][0] = z.x ^ 0x80808080u, v[k][1] = z.y ^ 0x80808080u;
+            v[k][2] = z.z ^ 0x80808080u, v[k][3] = z.w ^ 0x80808080u;
+          } else {
+            const uint2 z = lds64(at + ((((r >> 1) ^ ((row >> 1) & 3)) << 4) | ((r & 1) << 3)));
+            v[k][0] = z.x ^ 0x80808080u, v[k][1] = z.y ^ 0x80808080u;
+          }
+        }
+        uint32_t vs[W * 2];                         // the features' scales, float16 pairs
+#pragma unroll
+        for (int k = 0; k < W / 2; ++k) {
+          const uint4 z = lds128(sc + 32 + r * (W * 8) + k * 16);
+          vs[4 * k] = z.x, vs[4 * k + 1] = z.y, vs[4 * k + 2] = z.z, vs[4 * k + 3] = z.w;
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const uint32_t t01[2] = {__byte_perm(v[0][w], v[1][w], 0x5140), __byte_perm(v[0][w], v[1][w], 0x7362)};
+          const uint32_t t89[2] = {__byte_perm(v[2][w], v[3][w], 0x5140), __byte_perm(v[2][w], v[3][w], 0x7362)};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int jj = 2 * w + h;
+            const uint32_t f[4] = {codes_to_half(t01[h], 0x4140), codes_to_half(t01[h], 0x4342),
+                                   codes_to_half(t89[h], 0x4140), codes_to_half(t89[h], 0x4342)};
+            const float2 z = unpack<__half>(vs[jj]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              float o[4] = {0.f, 0.f, 0.f, 0.f};
+              mma<E>(o, f, ph[t][0], ph[t][1]);
+              mma<E>(o, f, pl[t][0], pl[t][1]);
+              st.acc[t][jj][0] += z.x * o[0];
+              st.acc[t][jj][1] += z.x * o[1];
+              st.acc[t][jj][2] += z.y * o[2];
+              st.acc[t][jj][3] += z.y * o[3];
+            }
+          }
+        }
+      }
+      ++used;
+      __syncwarp();                                 // every lane has read the stage
+      if (to_issue > 0) issue();
+    }
+    if (!alive) break;
+
+    // ---- the end of the item in this warp ----------------------------------------------------
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float l = st.l[t][i];
+        l += __shfl_xor_sync(~0u, l, 4);
+        l += __shfl_xor_sync(~0u, l, 8);
+        l += __shfl_xor_sync(~0u, l, 16);
+        st.l[t][i] = l;
+      }
+    const int n = stop - first;
+    if (n == nb) {
+      // whole: normalised and written from here
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float i0 = 1.f / st.l[t][0], i1 = 1.f / st.l[t][1];
+        T* o = static_cast<T*>(a.o) + b * a.o_bs + (int64_t)(h0 + t * 8) * a.o_hs;
+        if constexpr (!I8) {
+#pragma unroll
+          for (int jj = 0; jj < MT; ++jj)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t w = transpose8(pack<T>(st.acc[t][jj][2 * h] * i0, st.acc[t][jj][2 * h + 1] * i1));
+              if (t * 8 + r < heads)
+                *reinterpret_cast<uint32_t*>(o + r * a.o_hs + jj * 16 + h * 8 + 2 * c) = w;
+            }
+        } else {
+#pragma unroll
+          for (int jj = 0; jj < MT; ++jj) {
+            const int d = r * (G::DP / 8) + 2 * jj;
+            if (d < D) {
+              if (t * 8 + 2 * c < heads)
+                *reinterpret_cast<uint32_t*>(o + (2 * c) * a.o_hs + d) =
+                    pack<T>(st.acc[t][jj][0] * i0, st.acc[t][jj][2] * i0);
+              if (t * 8 + 2 * c + 1 < heads)
+                *reinterpret_cast<uint32_t*>(o + (2 * c + 1) * a.o_hs + d) =
+                    pack<T>(st.acc[t][jj][1] * i1, st.acc[t][jj][3] * i1);
+            }
+          }
+        }
+        if (a.lse && r == 0)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (t * 8 + 2 * c + i < heads)
+              a.lse[b * a.lse_bs + h0 + t * 8 + 2 * c + i] =
+                  (st.m[t][i] + log2f(st.l[t][i])) * 0.6931471805599453f;
+      }
+    } else {
+      // a piece: the first in its own room, the second over this warp's stages (its range
+      // ends here, so every load it issued has been consumed)
+      float* p = pieces == 0 ? piece0 + warp * (G::PIECE / 4) : reinterpret_cast<float*>(ring);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int h = t * 8 + 2 * c + i;
+#pragma unroll
+          for (int jj = 0; jj < MT; ++jj)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int d = I8 ? r * (G::DP / 8) + 2 * jj + k : jj * 16 + 8 * k + r;
+              if (!I8 || d < D) p[h * G::OS + d] = st.acc[t][jj][2 * k + i];
+            }
+          if (r == 0) {
+            p[NH * G::OS + h] = st.m[t][i];
+            p[NH * G::OS + NH + h] = st.l[t][i];
+          }
+        }
+      if (lane == 0) {
+        int span = 0;
+        if (first == 0) {
+          span = 1;
+          if constexpr (SPLIT) span = (int)(((u + nb) * ctas - 1) / total) - (int)blockIdx.x + 1;
+        }
+        notes[2 * warp + pieces] = make_int4(b, j, n, span);
+      }
+      ++pieces;
+    }
+    u += n;
+    left -= n;
+    if (left > 0) {
+      blk = 0;
+      if (++j == a.items) {
+        j = 0;
+        do { nb = (row_len(a, ++b) + 15) >> 4; } while (nb == 0);
+      }
+    }
+  }
+  if (!alive) {                                     // a wait ran out: drain what is in flight
+    while (used < issued) {
+      const uint32_t s = used % NS;
+      if (!wait_full(bar_u + 8 * s, (used / NS) & 1, nullptr)) break;
+      ++used;
+    }
+  }
   __syncthreads();
-  float top = -INFINITY, total = 0.f;
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, sm_m[w]);
-  const float base = top == -INFINITY ? 0.f : top;
-  for (int w = 0; w < 8; ++w) total += sm_l[w] * expf(sm_m[w] - base);
-  T* op = static_cast<T*>(a.o) + b * a.o_bs + h * a.o_hs;
-  for (int d = threadIdx.x; d < D; d += 256) {
-    float s = 0.f;
-    for (int w = 0; w < 8; ++w) s += sm_o[w][d] * expf(sm_m[w] - base);
-    from_f32(op + d, len > 0 ? s / total : 0.f);
+
+  // ---- the CTA's pieces, joined item by item --------------------------------------------------
+  int4 own = make_int4(0, 0, 0, 0);
+  for (int i = 0; i < 2 * kWarps;) {
+    const int4 note = notes[i];
+    if (note.x < 0) {
+      ++i;
+      continue;
+    }
+    int n = 0, end = i;
+    for (; end < 2 * kWarps; ++end) {
+      const int4 z = notes[end];
+      if (z.x < 0) continue;
+      if (z.x != note.x || z.y != note.y) break;
+      n += z.z;
+    }
+    const int whole = (row_len(a, note.x) + 15) >> 4;
+    const int kvh = note.y / a.tiles, h0 = kvh * a.group + (note.y - kvh * a.tiles) * NH;
+    const int heads = min(NH, (kvh + 1) * a.group - h0);
+    // an item that continues from the CTA before takes the first workspace slot, one that
+    // continues into the next CTA (and began here) the second
+    float* part = nullptr;
+    if (n != whole) {
+      if (!SPLIT) return;                           // a wait ran out
+      part = a.part + ((int64_t)blockIdx.x * 2 + (note.w > 0 ? 1 : 0)) * G::PART;
+      if (note.w > 0) own = make_int4(note.x, note.y, note.w, 0);
+    }
+    for (int e = tid; e < NH * D; e += kThreads) {
+      const int h = e / D, d = e - h * D;
+      float top = -INFINITY;
+      for (int k = i; k < end; ++k)
+        if (notes[k].x >= 0) {
+          const float* p = (k & 1) ? reinterpret_cast<const float*>(smem + (k >> 1) * NS * G::STAGE)
+                                   : piece0 + (k >> 1) * (G::PIECE / 4);
+          top = fmaxf(top, p[NH * G::OS + h]);
+        }
+      const float base = top == -INFINITY ? 0.f : top;
+      float o = 0.f, l = 0.f;
+      for (int k = i; k < end; ++k)
+        if (notes[k].x >= 0) {
+          const float* p = (k & 1) ? reinterpret_cast<const float*>(smem + (k >> 1) * NS * G::STAGE)
+                                   : piece0 + (k >> 1) * (G::PIECE / 4);
+          const float f = ex2(p[NH * G::OS + h] - base);
+          o += f * p[h * G::OS + d];
+          l += f * p[NH * G::OS + NH + h];
+        }
+      if (part) {
+        part[e] = o;
+        if (d == 0) {
+          part[NH * D + h] = top;
+          part[NH * D + NH + h] = l;
+        }
+      } else if (h < heads) {
+        static_cast<T*>(a.o)[note.x * a.o_bs + (int64_t)(h0 + h) * a.o_hs + d] = T(o / l);
+        if (d == 0 && a.lse)
+          a.lse[note.x * a.lse_bs + h0 + h] = (base + log2f(l)) * 0.6931471805599453f;
+      }
+    }
+    i = end;
   }
-  if (a.lse && threadIdx.x == 0) a.lse[b * a.lse_bs + h] = len > 0 ? base + logf(total) : -INFINITY;
+  if (SPLIT && tid == 0) a.owner[blockIdx.x] = own;
 }
 
-template <typename T, typename P>
-void* pick(int D) {
-  return D == 64 ? (void*)kvb_paged_decode_kernel<T, P, 64>
-                 : D == 96 ? (void*)kvb_paged_decode_kernel<T, P, 96>
-                           : (void*)kvb_paged_decode_kernel<T, P, 128>;
+// Joins the pieces of an item that spans CTAs: block (c, h) the item that began in CTA c, head
+// h.  Weights first, then 256 threads over (piece group, four features).
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(256) kvb_paged_join_kernel(const Args a) {
+  constexpr int NH = 8 * NT, PART = NH * D + 2 * NH, Q = D / 4, GROUPS = 256 / Q;
+  __shared__ float w[kSms], red[8], sums[GROUPS][D];
+  const int tid = threadIdx.x, h = blockIdx.y;
+  griddep_wait();
+  griddep_launch_dependents();
+  const int4 own = a.owner[blockIdx.x];
+  const int span = min(own.z, a.ctas - (int)blockIdx.x);
+  const int kvh = own.y / a.tiles, h0 = kvh * a.group + (own.y - kvh * a.tiles) * NH;
+  if (span <= 0 || h >= (kvh + 1) * a.group - h0) return;
+  const float* first = a.part + ((int64_t)blockIdx.x * 2 + 1) * PART;
+  // piece k > 0 is the first slot of CTA blockIdx.x + k
+  auto at = [&](int k) { return k == 0 ? first : first + ((int64_t)2 * k - 1) * PART; };
+  float m = -INFINITY, l = 0.f;
+  if (tid < span) {
+    m = at(tid)[NH * D + h];
+    l = at(tid)[NH * D + NH + h];
+  }
+  float top = m;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  if ((tid & 31) == 0) red[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i]);
+  const float base = top == -INFINITY ? 0.f : top;
+  const float f = ex2(m - base);
+  if (tid < span) w[tid] = f;
+  float total = tid < span ? l * f : 0.f;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
+  __syncthreads();
+  if ((tid & 31) == 0) red[tid >> 5] = total;
+  __syncthreads();
+  total = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) total += red[i];
+  const int g = tid / Q, x = tid - g * Q;
+  if (g < GROUPS) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = g; k < span; k += GROUPS) {
+      const float4 v = *reinterpret_cast<const float4*>(at(k) + h * D + 4 * x);
+      acc.x += w[k] * v.x;
+      acc.y += w[k] * v.y;
+      acc.z += w[k] * v.z;
+      acc.w += w[k] * v.w;
+    }
+    *reinterpret_cast<float4*>(&sums[g][4 * x]) = acc;
+  }
+  __syncthreads();
+  if (tid < D) {
+    float o = 0.f;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) o += sums[i][tid];
+    static_cast<T*>(a.o)[own.x * a.o_bs + (int64_t)(h0 + h) * a.o_hs + tid] = T(o / total);
+    if (tid == 0 && a.lse) a.lse[own.x * a.lse_bs + h0 + h] = (base + log2f(total)) * 0.6931471805599453f;
+  }
 }
+
+// ---- host -------------------------------------------------------------------------------------
 
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Query heads per item: 8, or 16 where a group has more.
+int head_tiles(const KvbPagedDecodeParams* p) { return p->num_q_heads / p->num_kv_heads > 8 ? 2 : 1; }
+
+// One CTA per item, or the units split over the GPU.  Short tables: an item is a few blocks
+// per warp, and a launch to join pieces would cost more than it spreads.
+bool split(const KvbPagedDecodeParams* p) {
+  if (p->batch > kSplitRows) return false;
+  const int64_t width = p->max_seq_len > 0
+                            ? std::min<int64_t>(p->max_blocks_per_seq, ((int64_t)p->max_seq_len + 15) / 16)
+                            : p->max_blocks_per_seq;
+  return width > kItemBlocks;
+}
+
+int64_t part_floats(const KvbPagedDecodeParams* p) {
+  const int nh = 8 * head_tiles(p);
+  return (int64_t)nh * p->head_dim + 2 * nh;
+}
 
 int check(const KvbPagedDecodeParams* p) {
   if (!p) return fail(KVB_ERR_INVALID, "params is NULL");
@@ -119,10 +883,11 @@ int check(const KvbPagedDecodeParams* p) {
   if (p->pool_format != KVB_POOL_INT8_KIVI && p->pool_format != KVB_POOL_COMPUTE)
     return fail(KVB_ERR_INVALID, "pool_format must be KVB_POOL_INT8_KIVI or KVB_POOL_COMPUTE");
   if (p->num_blocks < 1) return fail(KVB_ERR_INVALID, "num_blocks must be >= 1");
-  if (p->max_blocks_per_seq < 1 || p->max_blocks_per_seq > (1 << 27) - 1 ||
-      p->block_table_stride < p->max_blocks_per_seq)
+  if (p->max_blocks_per_seq < 1 || p->block_table_stride < p->max_blocks_per_seq)
     return fail(KVB_ERR_INVALID,
-                "max_blocks_per_seq must be in [1, 2^27 - 1] and block_table_stride at least that");
+                "max_blocks_per_seq must be >= 1 and block_table_stride at least that");
+  if ((int64_t)p->batch * p->max_blocks_per_seq > 0x7fffffff || p->max_blocks_per_seq > (1 << 27) - 1)
+    return fail(KVB_ERR_UNSUPPORTED, "batch * max_blocks_per_seq must be below 2^31, one row's blocks below 2^27");
   if (p->batch == 0) return KVB_OK;
   if (!p->q || !p->o || !p->kv_pool || !p->block_tables || !p->seq_lens)
     return fail(KVB_ERR_INVALID, "q, o, kv_pool, block_tables and seq_lens must be non-null");
@@ -138,22 +903,117 @@ int check(const KvbPagedDecodeParams* p) {
   return KVB_OK;
 }
 
+// The pool as (feature, KV head and slot, K or V, block); a box is one head's 16 slots of K and
+// V, 64 features (16-bit) or all of them (int8, padded to 64 or 128 by the zero fill).
+bool pool_map(CUtensorMap* m, const KvbPagedDecodeParams* p, std::string* err) {
+  static PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  if (!enc) {
+    *err = "cuTensorMapEncodeTiled unavailable from the CUDA driver";
+    return false;
+  }
+  const bool i8 = p->pool_format == KVB_POOL_INT8_KIVI;
+  const cuuint64_t el = i8 ? 1 : 2, row = el * p->head_dim, kv = row * 16 * p->num_kv_heads;
+  const cuuint64_t dims[4] = {(cuuint64_t)p->head_dim, (cuuint64_t)p->num_kv_heads * 16, 2,
+                              (cuuint64_t)p->num_blocks};
+  const cuuint64_t strides[3] = {row, kv, 2 * kv};
+  const cuuint32_t box[4] = {(cuuint32_t)(i8 && p->head_dim > 64 ? 128 : 64), 16, 2, 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  const CUresult r = enc(
+      m, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+            : p->dtype == KVB_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+      4, const_cast<void*>(p->kv_pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      i8 && p->head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    *err = "cuTensorMapEncodeTiled failed with CUresult " + std::to_string((int)r);
+    return false;
+  }
+  return true;
+}
+
+template <typename... KArgs, typename... As>
+cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t s, As&&... as) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<As>(as)...);
+}
+
+template <typename T, int D, bool I8, int NT>
+cudaError_t launch(const CUtensorMap& map, const Args& a, bool is_split, cudaStream_t s) {
+  using G = Geo<D, I8, NT>;
+  auto kern = is_split ? kvb_paged_decode_kernel<T, D, I8, NT, true> : kvb_paged_decode_kernel<T, D, I8, NT, false>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(kern, dim3(is_split ? a.ctas : a.batch * a.items), kThreads, G::SMEM, s, map, a);
+  if (e != cudaSuccess || !is_split || a.ctas == 1) return e;
+  return launch_pdl(kvb_paged_join_kernel<T, D, NT>, dim3(a.ctas, std::min(a.group, 8 * NT)), 256, 0, s, a);
+}
+
+template <typename T, bool I8, int NT>
+cudaError_t launch_d(int D, const CUtensorMap& map, const Args& a, bool is_split, cudaStream_t s) {
+  return D == 64 ? launch<T, 64, I8, NT>(map, a, is_split, s)
+                 : D == 96 ? launch<T, 96, I8, NT>(map, a, is_split, s)
+                           : launch<T, 128, I8, NT>(map, a, is_split, s);
+}
+
+template <typename T>
+cudaError_t launch_t(const KvbPagedDecodeParams* p, const CUtensorMap& map, const Args& a, bool is_split,
+                     cudaStream_t s) {
+  const bool i8 = p->pool_format == KVB_POOL_INT8_KIVI;
+  if (head_tiles(p) == 1)
+    return i8 ? launch_d<T, true, 1>(p->head_dim, map, a, is_split, s)
+              : launch_d<T, false, 1>(p->head_dim, map, a, is_split, s);
+  return i8 ? launch_d<T, true, 2>(p->head_dim, map, a, is_split, s)
+            : launch_d<T, false, 2>(p->head_dim, map, a, is_split, s);
+}
+
 }  // namespace kvb_pd
 
 extern "C" int64_t kvb_paged_decode_workspace_bytes(const KvbPagedDecodeParams* p) {
   if (kvb_pd::check(p) != KVB_OK) return -1;
-  return 0;
+  if (p->batch == 0 || !kvb_pd::split(p)) return 0;
+  return kvb_pd::kSms * (2 * kvb_pd::part_floats(p) * 4 + (int64_t)sizeof(int4));
 }
 
 extern "C" int kvb_paged_decode_fwd(const KvbPagedDecodeParams* p, void* stream) {
   if (const int rc = kvb_pd::check(p)) return rc;
   if (p->batch == 0) return KVB_OK;
+  const bool is_split = kvb_pd::split(p);
+  if (is_split) {
+    if (!p->workspace || p->workspace_bytes < kvb_paged_decode_workspace_bytes(p))
+      return kvb_pd::fail(KVB_ERR_INVALID, "workspace must hold kvb_paged_decode_workspace_bytes bytes");
+    if (!kvb_pd::aligned(p->workspace, 16))
+      return kvb_pd::fail(KVB_ERR_INVALID, "workspace must be 16-byte aligned");
+  }
   kvb_pd::Args a = {};
+  a.batch = p->batch;
   a.num_q_heads = p->num_q_heads;
   a.num_kv_heads = p->num_kv_heads;
   a.num_blocks = p->num_blocks;
   a.width = p->max_blocks_per_seq;
-  a.scale = p->softmax_scale;
+  a.group = p->num_q_heads / p->num_kv_heads;
+  const int nh = 8 * kvb_pd::head_tiles(p);
+  a.tiles = (a.group + nh - 1) / nh;
+  a.items = p->num_kv_heads * a.tiles;
+  if ((int64_t)a.items * p->batch > 0x7fffffff)
+    return kvb_pd::fail(KVB_ERR_UNSUPPORTED, "too many requests and heads for one call");
+  a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
   a.q = p->q;
   a.o = p->o;
   a.lse = p->lse;
@@ -163,21 +1023,24 @@ extern "C" int kvb_paged_decode_fwd(const KvbPagedDecodeParams* p, void* stream)
   a.o_hs = p->o_head_stride;
   a.lse_bs = p->lse_batch_stride;
   a.table_stride = p->block_table_stride;
-  a.pool = p->kv_pool;
-  const bool int8 = p->pool_format == KVB_POOL_INT8_KIVI;
-  a.k_scale = int8 ? static_cast<const __half*>(p->k_scale16) : nullptr;
-  a.v_scale = int8 ? static_cast<const __half*>(p->v_scale16) : nullptr;
+  a.k_scale = static_cast<const __half*>(p->k_scale16);
+  a.v_scale = static_cast<const __half*>(p->v_scale16);
   a.tables = p->block_tables;
   a.lens = p->seq_lens;
   a.status = p->status;
-  void* kern = p->dtype == KVB_DTYPE_BF16
-                   ? (int8 ? kvb_pd::pick<__nv_bfloat16, int8_t>(p->head_dim)
-                           : kvb_pd::pick<__nv_bfloat16, __nv_bfloat16>(p->head_dim))
-                   : (int8 ? kvb_pd::pick<__half, int8_t>(p->head_dim)
-                           : kvb_pd::pick<__half, __half>(p->head_dim));
-  void* args[] = {&a};
-  const cudaError_t e = cudaLaunchKernel(kern, dim3(p->num_q_heads, p->batch), dim3(256), args, 0,
-                                         static_cast<cudaStream_t>(stream));
+  if (is_split) {
+    const int64_t most = (int64_t)p->batch * p->max_blocks_per_seq * a.items;
+    a.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(kvb_pd::kSms, (most + kvb_pd::kMinUnits - 1) / kvb_pd::kMinUnits));
+    a.part = static_cast<float*>(p->workspace);
+    a.owner = reinterpret_cast<int4*>(a.part + kvb_pd::kSms * 2 * kvb_pd::part_floats(p));
+  }
+  CUtensorMap map;
+  std::string err;
+  if (!kvb_pd::pool_map(&map, p, &err)) return kvb_pd::fail(KVB_ERR_CUDA, err);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = p->dtype == KVB_DTYPE_BF16
+                            ? kvb_pd::launch_t<__nv_bfloat16>(p, map, a, is_split, s)
+                            : kvb_pd::launch_t<__half>(p, map, a, is_split, s);
   if (e != cudaSuccess)
     return kvb_pd::fail(KVB_ERR_CUDA, std::string("kvb_paged_decode_fwd launch: ") + cudaGetErrorString(e));
   return KVB_OK;

@@ -356,7 +356,8 @@ def test_paged_decode_non_finite_values_stay_in_their_rows():
 
 def test_paged_decode_layouts_and_streams():
     """HF's transposed query, a misaligned one, a caller's output view, sliced tables, no
-    LSE, another stream; the same bits every time."""
+    LSE, another stream; the same bits every time.  (A hint that changes the launch's shape
+    changes the order of the sums: ``test_paged_decode_shapes_of_the_launch_agree``.)"""
     from kvboost_b200.paged_decode import paged_decode_attention
     g = torch.Generator().manual_seed(6)
     ln = [1700, 3, 0, 513]
@@ -374,7 +375,7 @@ def test_paged_decode_layouts_and_streams():
     room = torch.full((4, 1, 20, 128), 5.0, dtype=torch.bfloat16, device=DEV)
     out = room[:, :, 2:18].transpose(1, 2)
     for qq, kw in ((hf, {}), (odd[..., 1:], dict(return_lse=False)), (q.cuda(), dict(out=out)),
-                   (q.cuda(), dict(max_seq_len=1700)), (q.cuda(), dict(max_seq_len=5))):
+                   (q.cuda(), dict(max_seq_len=1700))):
         o, l2 = paged_decode_attention(qq, P, view, lens, **kw)
         assert torch.equal(o, want), kw
         assert (l2 is None) if "return_lse" in kw else torch.equal(l2, lse)
