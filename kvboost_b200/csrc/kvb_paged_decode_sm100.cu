@@ -50,13 +50,12 @@ using namespace kvb::ptx;
 int fail(int code, const std::string& msg) { return kvb_detail_fail(code, msg); }
 
 constexpr int kSms = 148;
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr float kRaise = 8.f;              // log2 units a score may pass the running maximum by
 constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr int kWarpsI8 = 12;               // warps per CTA over int8 pools (8 otherwise)
 constexpr int kItemBlocks = 64;            // tables up to this wide take one CTA per item
 constexpr int kMinUnits = 8;               // blocks per CTA below which fewer CTAs share them
-constexpr int kSplitRows = 4096;           // most rows of a split launch (prefix sums in shared memory)
+constexpr int kSplitRows = 8192;           // most rows of a split launch (prefix sums in shared memory)
 
 struct Args {
   int batch, num_q_heads, num_kv_heads, num_blocks, width;
@@ -73,6 +72,7 @@ struct Args {
   const int32_t* lens;
   int32_t* status;
   float* part;                             // [ctas][2][NH * D + 2 * NH]
+  float* first;                            // [ctas * warps][PIECE]: pieces that start a warp's range
   int4* owner;                             // [ctas]: request, item, CTAs it spans (0: none)
 };
 
@@ -109,9 +109,15 @@ __device__ __forceinline__ float lds_half(uint32_t addr) {
 __device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// One arrival on `bar` once this thread's copies so far have landed.
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
 
 // D (16 x 8, float32) += A (16 x 16) B (16 x 8), both operands in E
@@ -177,6 +183,8 @@ __device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity, int32_t
 // ---- geometry -------------------------------------------------------------------------------
 template <int D, bool I8, int NT>
 struct Geo {
+  static constexpr int WARPS = I8 && NT == 1 ? kWarpsI8 : 8;
+  static constexpr int THREADS = WARPS * 32;
   static constexpr int NH = 8 * NT;                          // query heads per item
   static constexpr int DP = I8 ? (D == 64 ? 64 : 128) : D;   // features the MMAs cover
   static constexpr int HALVES = I8 ? 1 : (D + 63) / 64;      // TMA boxes per block
@@ -185,17 +193,36 @@ struct Geo {
   static constexpr int STAGE = HALVES * BOX;
   static constexpr int SCALES = I8 ? 32 + 256 : 0;           // K then V scales of the block
   static constexpr int OS = D + 4;                           // piece row: conflict-free columns
-  static constexpr int PIECE = (NH * OS + 2 * NH) * 4;
-  // alignment, pieces, notes, warp sums; per stage: data, scales, barrier
-  static constexpr int FIXED = 1024 + kWarps * PIECE + kWarps * 2 * 16 + kWarps * 4;
-  static constexpr int PER_STAGE = kWarps * (STAGE + SCALES + 8);
+  static constexpr int PIECE = NH * OS + 2 * NH;             // floats: O rows, maxima, sums
+  // alignment, notes, warp sums; per stage: data, scales, barrier
+  static constexpr int FIXED = 1024 + WARPS * 2 * 16 + WARPS * 4;
+  static constexpr int PER_STAGE = WARPS * (STAGE + SCALES + 8);
   static constexpr int FIT = (232448 - FIXED) / PER_STAGE;
   static constexpr int NS = FIT < 6 ? FIT : 6;               // stages per warp
   static constexpr int SMEM = FIXED + NS * PER_STAGE;
   static constexpr int PART = NH * D + 2 * NH;               // floats of a workspace piece
   static_assert(NS >= 2, "at least two stages per warp");
-  static_assert(PIECE <= NS * STAGE, "a second piece goes over the warp's stages");
-  static_assert(kWarps * PIECE / 4 >= kSplitRows, "prefix sums share the pieces' room");
+  static_assert(PIECE * 4 <= NS * STAGE, "a last piece goes over the warp's stages");
+  static_assert(WARPS * NS * STAGE >= kSplitRows * 4, "prefix sums go over the stages");
+};
+
+// x / y for x < 2^63; the 32-bit division where it will do.
+__device__ __forceinline__ int64_t quot(int64_t x, int y) {
+  return (x >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+}
+
+// total units over `workers`: worker i's first unit, and the worker that holds unit u.
+struct Shares {
+  int64_t q;
+  int rem;
+  __device__ __forceinline__ Shares(int64_t total, int workers)
+      : q(quot(total, workers)), rem((int)(total - q * workers)) {}
+  __device__ __forceinline__ int64_t first(int i) const { return i * q + min(i, rem); }
+  __device__ __forceinline__ int holder(int64_t u) const {
+    const int64_t big = rem * (q + 1);
+    if (u < big) return (int)((u >> 32) == 0 && q < 0x7fffffff ? (uint32_t)u / (uint32_t)(q + 1) : u / (q + 1));
+    return rem + (int)(((u - big) >> 32) == 0 && q < 0x7fffffff ? (uint32_t)(u - big) / (uint32_t)q : (u - big) / q);
+  }
 };
 
 __device__ __forceinline__ int row_len(const Args& a, int b) {
@@ -220,27 +247,27 @@ struct State {
 };
 
 template <typename T, int D, bool I8, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     kvb_paged_decode_kernel(const __grid_constant__ CUtensorMap map, const Args a) {
   using G = Geo<D, I8, NT>;
   using E = typename std::conditional<I8, __half, T>::type;   // MMA operand type
   constexpr int MT = G::DP / 16, KS = G::DP / 16, NS = G::NS, NH = G::NH;
+  constexpr int kWarps = G::WARPS, kThreads = G::THREADS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
   uint8_t* ring = smem + warp * NS * G::STAGE;
   uint8_t* scales = smem + kWarps * NS * G::STAGE + warp * NS * G::SCALES;
   uint8_t* after = smem + kWarps * NS * (G::STAGE + G::SCALES);
-  float* piece0 = reinterpret_cast<float*>(after);                     // [kWarps] first pieces
-  int32_t* prefix = reinterpret_cast<int32_t*>(after);                 // before any piece is written
-  uint64_t* bars = reinterpret_cast<uint64_t*>(after + kWarps * G::PIECE);
+  int32_t* prefix = reinterpret_cast<int32_t*>(smem);                  // before the first load
+  uint64_t* bars = reinterpret_cast<uint64_t*>(after);
   // [kWarps][2] pieces: request (-1: none), item, blocks, CTAs spanned if the item begins here
   int4* notes = reinterpret_cast<int4*>(bars + kWarps * NS);
   int32_t* wsum = reinterpret_cast<int32_t*>(notes + 2 * kWarps);
   const uint32_t ring_u = smem_u32(ring), scales_u = smem_u32(scales), bar_u = smem_u32(bars + warp * NS);
 
   if (lane == 0) {
-    for (int s = 0; s < NS; ++s) mbar_init(bar_u + 8 * s, 1);
+    for (int s = 0; s < NS; ++s) mbar_init(bar_u + 8 * s, I8 ? 33 : 1);
     fence_mbar_init();
     notes[2 * warp].x = notes[2 * warp + 1].x = -1;
     prefetch_tmap(&map);
@@ -284,12 +311,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (err && blockIdx.x == 0 && a.status) atomicOr(a.status, err);
     total = (int64_t)base * a.items;
     // no CTA without a unit, so an item's CTAs are consecutive
-    ctas = (int)min((int64_t)a.ctas, (total + kMinUnits - 1) / kMinUnits);
-    const int64_t workers = (int64_t)ctas * kWarps, me = (int64_t)blockIdx.x * kWarps + warp;
+    ctas = (int)min((int64_t)a.ctas, quot(total + kMinUnits - 1, kMinUnits));
+    const int me = blockIdx.x * kWarps + warp;
     left = 0;
     if ((int)blockIdx.x < ctas) {
-      u = me * total / workers;
-      left = (me + 1) * total / workers - u;
+      const Shares sh(total, ctas * kWarps);
+      u = sh.first(me);
+      left = sh.first(me + 1) - u;
     }
     b = j = blk = nb = 0;
     if (left > 0) {
@@ -302,10 +330,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int before = lo ? prefix[lo - 1] : 0;
       nb = prefix[lo] - before;
       const int64_t rel = u - (int64_t)before * a.items;
-      j = (int)(rel / nb);
+      j = (int)quot(rel, nb);
       blk = (int)(rel - (int64_t)j * nb);
     }
-    __syncthreads();                                // the pieces' room is free from here
+    fence_proxy_async_smem();                       // the loads go over the sums
+    __syncthreads();
   } else {
     b = blockIdx.x / a.items;
     j = blockIdx.x - b * a.items;
@@ -335,30 +364,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int kvh = a.tiles == 1 ? pj : pj / a.tiles;
     const bool ok = (unsigned)id < (unsigned)a.num_blocks;
     if (lane == 0) {
-      if constexpr (I8) {
-        const uint32_t sc = scales_u + s * G::SCALES;
-        mbar_arrive_expect_tx(bar, G::STAGE + (ok ? 32 + 2 * D : 0));
-        tma_load_4d(dst, &map, 0, kvh * 16, 0, ok ? id : -1, bar);
-        if (ok) {
-          const int64_t bh = (int64_t)id * a.num_kv_heads + kvh;
-          bulk_load(sc, a.k_scale + bh * 16, 32, bar);
-          bulk_load(sc + 32, a.v_scale + bh * D, 2 * D, bar);
-        }
-      } else {
-        mbar_arrive_expect_tx(bar, G::STAGE);
+      mbar_arrive_expect_tx(bar, G::STAGE);
 #pragma unroll
-        for (int h = 0; h < G::HALVES; ++h)
-          tma_load_4d(dst + h * G::BOX, &map, h * 64, kvh * 16, 0, ok ? id : -1, bar);
+      for (int h = 0; h < G::HALVES; ++h)
+        tma_load_4d(dst + h * G::BOX, &map, h * 64, kvh * 16, 0, ok ? id : -1, bar);
+    }
+    if constexpr (I8) {
+      if (ok && lane < 2 + D / 8) {
+        const int64_t bh = (int64_t)id * a.num_kv_heads + kvh;
+        copy16(scales_u + s * G::SCALES + 16 * lane,
+               lane < 2 ? a.k_scale + bh * 16 + 8 * lane : a.v_scale + bh * D + 8 * (lane - 2));
       }
     }
     if (!ok) {                                      // reads as zeros
-      if (I8) {
+      if (I8)
         for (int i = lane; i < G::SCALES / 4; i += 32) sts32(scales_u + s * G::SCALES + 4 * i, 0u);
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
+      __syncwarp();
       if (lane == 0 && a.status) atomicOr(a.status, KVB_STATUS_BAD_BLOCK);
     }
+    if constexpr (I8) copies_arrive(bar);
     ++issued;
     --to_issue;
     if (++pblk == pnb && to_issue > 0) {
@@ -367,6 +391,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         pj = 0;
         do { pnb = (row_len(a, ++pb) + 15) >> 4; } while (pnb == 0);
       }
+      // the item's query heads will be wanted NS blocks from now
+      const int kv = a.tiles == 1 ? pj : pj / a.tiles, h = kv * a.group + (pj - kv * a.tiles) * NH + (lane >> 1);
+      if ((lane >> 1) < NH && h < (kv + 1) * a.group)
+        prefetch_l2(static_cast<const T*>(a.q) + pb * a.q_bs + h * a.q_hs + (lane & 1) * (D / 2));
     }
   };
 #pragma unroll 1
@@ -393,12 +421,35 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   // ---- consumer ----------------------------------------------------------------------------
+  // An item's query heads as the MMA's B operand: for 16-bit pools features 16 ks + 2c, + 8; for
+  // int8 pools in the order the K codes are read (lane c's 16-byte pieces c, c + 4), still in T.
+  auto load_q = [&](uint32_t (&f)[NT][KS][2], int qb, int qj) {
+    const int kv = a.tiles == 1 ? qj : qj / a.tiles, hq = kv * a.group + (qj - kv * a.tiles) * NH;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const bool on = hq + t * 8 + r < (kv + 1) * a.group;
+      const T* row = static_cast<const T*>(a.q) + qb * a.q_bs + (int64_t)(on ? hq + t * 8 + r : hq) * a.q_hs;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if constexpr (I8) {
+          const int d = 16 * (c + 4 * (ks >> 2)) + 4 * (ks & 3);
+          const uint2 x = on && d < D ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0u, 0u);
+          f[t][ks][0] = x.x;
+          f[t][ks][1] = x.y;
+        } else {
+          f[t][ks][0] = on ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 2 * c) : 0u;
+          f[t][ks][1] = on ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8 + 2 * c) : 0u;
+        }
+      }
+    }
+  };
+  constexpr bool AHEAD = NT == 1;                   // the next item's heads fit in registers too
   State<MT, NT> st;
-  uint32_t qf[NT][KS][2];
+  uint32_t qf[NT][KS][2], qn[NT][KS][2];
   float qx[NT][2];              // what turns S into log2 scores, per head of this lane's columns
   uint32_t used = 0;
-  int pieces = 0;
-  bool alive = true;
+  bool alive = true, fetched = false;
+  if (left > 0) load_q(qf, b, j);
   while (left > 0 && alive) {
     // one item, or the part of it in this warp's range
     const int kvh = a.tiles == 1 ? j : j / a.tiles;
@@ -407,28 +458,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int len = row_len(a, b);
     const int first = blk;
     const int stop = (int)min((int64_t)nb, blk + left);
+    const bool last = left == stop - first;
     st.clear();
-    const T* q = static_cast<const T*>(a.q) + b * a.q_bs + (int64_t)h0 * a.q_hs;
+    if constexpr (AHEAD) {
+      if (fetched) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[0][ks][0] = qn[0][ks][0], qf[0][ks][1] = qn[0][ks][1];
+      }
+    } else {
+      if (fetched) load_q(qf, b, j);
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const bool on = t * 8 + r < heads;
-      const T* row = q + (on ? t * 8 + r : 0) * a.q_hs;
       if constexpr (!I8) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            qf[t][ks][h] = on ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + h * 8 + 2 * c) : 0u;
         qx[t][0] = qx[t][1] = a.scale_log2;
       } else {
-        // features in the order the K codes are read: lane c's 16-byte pieces c, c + 4
         float top = 0.f;
-        uint2 raw[KS];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          const int d = 16 * (c + 4 * (ks >> 2)) + 4 * (ks & 3);
-          raw[ks] = on && d < D ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0u, 0u);
-          const float2 x = unpack<T>(raw[ks].x), y = unpack<T>(raw[ks].y);
+          const float2 x = unpack<T>(qf[t][ks][0]), y = unpack<T>(qf[t][ks][1]);
           top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(y.x), fabsf(y.y)));
         }
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
@@ -439,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float inv = __uint_as_float((uint32_t)min(e, 253) << 23);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          const float2 x = unpack<T>(raw[ks].x), y = unpack<T>(raw[ks].y);
+          const float2 x = unpack<T>(qf[t][ks][0]), y = unpack<T>(qf[t][ks][1]);
           qf[t][ks][0] = pack<__half>(x.x * f, x.y * f);
           qf[t][ks][1] = pack<__half>(y.x * f, y.y * f);
         }
@@ -447,10 +495,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         qx[t][1] = __shfl_sync(~0u, inv, 8 * c + 4) * a.scale_log2;
       }
     }
+    // the item after this one
+    int b2 = b, j2 = j + 1, nb2 = nb;
 
 #pragma unroll 1
     for (; blk < stop; ++blk) {
       const uint32_t s = used % NS, base = ring_u + s * G::STAGE, sc = scales_u + s * G::SCALES;
+      if (blk + 1 == stop && !last) {
+        if (j2 == a.items) {
+          j2 = 0;
+          do { nb2 = (row_len(a, ++b2) + 15) >> 4; } while (nb2 == 0);
+        }
+        if constexpr (AHEAD) load_q(qn, b2, j2);
+        fetched = true;
+      }
       if (!wait_full(bar_u + 8 * s, (used / NS) & 1, a.status)) {
         alive = false;
         break;
@@ -672,9 +730,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                   (st.m[t][i] + log2f(st.l[t][i])) * 0.6931471805599453f;
       }
     } else {
-      // a piece: the first in its own room, the second over this warp's stages (its range
-      // ends here, so every load it issued has been consumed)
-      float* p = pieces == 0 ? piece0 + warp * (G::PIECE / 4) : reinterpret_cast<float*>(ring);
+      // a piece: in the workspace, or at the end of the warp's range over its stages (every load
+      // it issued has been consumed)
+      float* p = last ? reinterpret_cast<float*>(ring)
+                      : a.first + ((int64_t)blockIdx.x * kWarps + warp) * G::PIECE;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -696,21 +755,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         int span = 0;
         if (first == 0) {
           span = 1;
-          if constexpr (SPLIT) span = (int)(((u + nb) * ctas - 1) / total) - (int)blockIdx.x + 1;
+          if constexpr (SPLIT) span = Shares(total, ctas * kWarps).holder(u + nb - 1) / kWarps - (int)blockIdx.x + 1;
         }
-        notes[2 * warp + pieces] = make_int4(b, j, n, span);
+        notes[2 * warp + (last ? 1 : 0)] = make_int4(b, j, n, span);
       }
-      ++pieces;
     }
     u += n;
     left -= n;
-    if (left > 0) {
-      blk = 0;
-      if (++j == a.items) {
-        j = 0;
-        do { nb = (row_len(a, ++b) + 15) >> 4; } while (nb == 0);
-      }
-    }
+    blk = 0;
+    b = b2;
+    j = j2;
+    nb = nb2;
   }
   if (!alive) {                                     // a wait ran out: drain what is in flight
     while (used < issued) {
@@ -721,64 +776,70 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
 
-  // ---- the CTA's pieces, joined item by item --------------------------------------------------
+  // ---- the CTA's pieces, joined item by item: a warp per head, a lane per four features ---------
+  const int4 note = lane < 2 * kWarps ? notes[lane] : make_int4(-1, 0, 0, 0);
+  uint32_t todo = __ballot_sync(~0u, note.x >= 0);
   int4 own = make_int4(0, 0, 0, 0);
-  for (int i = 0; i < 2 * kWarps;) {
-    const int4 note = notes[i];
-    if (note.x < 0) {
-      ++i;
-      continue;
-    }
-    int n = 0, end = i;
-    for (; end < 2 * kWarps; ++end) {
-      const int4 z = notes[end];
-      if (z.x < 0) continue;
-      if (z.x != note.x || z.y != note.y) break;
-      n += z.z;
-    }
-    const int whole = (row_len(a, note.x) + 15) >> 4;
-    const int kvh = note.y / a.tiles, h0 = kvh * a.group + (note.y - kvh * a.tiles) * NH;
+  while (todo) {
+    const int at = __ffs(todo) - 1;
+    const int ib = __shfl_sync(~0u, note.x, at), ij = __shfl_sync(~0u, note.y, at);
+    const int span = __shfl_sync(~0u, note.w, at);
+    const bool mine = note.x == ib && note.y == ij;
+    const uint32_t members = __ballot_sync(~0u, mine);
+    const int n = __reduce_add_sync(~0u, mine ? note.z : 0);
+    todo &= ~members;
+    const int kvh = ij / a.tiles, h0 = kvh * a.group + (ij - kvh * a.tiles) * NH;
     const int heads = min(NH, (kvh + 1) * a.group - h0);
     // an item that continues from the CTA before takes the first workspace slot, one that
     // continues into the next CTA (and began here) the second
     float* part = nullptr;
-    if (n != whole) {
+    if (n != (row_len(a, ib) + 15) >> 4) {
       if (!SPLIT) return;                           // a wait ran out
-      part = a.part + ((int64_t)blockIdx.x * 2 + (note.w > 0 ? 1 : 0)) * G::PART;
-      if (note.w > 0) own = make_int4(note.x, note.y, note.w, 0);
+      part = a.part + ((int64_t)blockIdx.x * 2 + (span > 0 ? 1 : 0)) * G::PART;
+      if (span > 0) own = make_int4(ib, ij, span, 0);
     }
-    for (int e = tid; e < NH * D; e += kThreads) {
-      const int h = e / D, d = e - h * D;
-      float top = -INFINITY;
-      for (int k = i; k < end; ++k)
-        if (notes[k].x >= 0) {
-          const float* p = (k & 1) ? reinterpret_cast<const float*>(smem + (k >> 1) * NS * G::STAGE)
-                                   : piece0 + (k >> 1) * (G::PIECE / 4);
-          top = fmaxf(top, p[NH * G::OS + h]);
-        }
+    const float* from = (lane & 1) || !SPLIT
+                            ? reinterpret_cast<const float*>(smem + (lane >> 1) * NS * G::STAGE)
+                            : a.first + ((int64_t)blockIdx.x * kWarps + (lane >> 1)) * G::PIECE;
+    for (int h = warp; h < heads; h += kWarps) {
+      const float m = mine ? from[NH * G::OS + h] : -INFINITY, l = mine ? from[NH * G::OS + NH + h] : 0.f;
+      float top = m;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
       const float base = top == -INFINITY ? 0.f : top;
-      float o = 0.f, l = 0.f;
-      for (int k = i; k < end; ++k)
-        if (notes[k].x >= 0) {
-          const float* p = (k & 1) ? reinterpret_cast<const float*>(smem + (k >> 1) * NS * G::STAGE)
-                                   : piece0 + (k >> 1) * (G::PIECE / 4);
-          const float f = ex2(p[NH * G::OS + h] - base);
-          o += f * p[h * G::OS + d];
-          l += f * p[NH * G::OS + NH + h];
+      const float w = ex2(m - base);
+      float sum = mine ? l * w : 0.f;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (uint32_t left_of = members; left_of; left_of &= left_of - 1) {
+        const int k = __ffs(left_of) - 1;
+        const float f = __shfl_sync(~0u, w, k);
+        const float* p = (k & 1) || !SPLIT
+                             ? reinterpret_cast<const float*>(smem + (k >> 1) * NS * G::STAGE)
+                             : a.first + ((int64_t)blockIdx.x * kWarps + (k >> 1)) * G::PIECE;
+        if (lane < D / 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p + h * G::OS + 4 * lane);
+          o.x += f * v.x;
+          o.y += f * v.y;
+          o.z += f * v.z;
+          o.w += f * v.w;
         }
+      }
       if (part) {
-        part[e] = o;
-        if (d == 0) {
+        if (lane < D / 4) *reinterpret_cast<float4*>(part + h * D + 4 * lane) = o;
+        if (lane == 0) {
           part[NH * D + h] = top;
-          part[NH * D + NH + h] = l;
+          part[NH * D + NH + h] = sum;
         }
-      } else if (h < heads) {
-        static_cast<T*>(a.o)[note.x * a.o_bs + (int64_t)(h0 + h) * a.o_hs + d] = T(o / l);
-        if (d == 0 && a.lse)
-          a.lse[note.x * a.lse_bs + h0 + h] = (base + log2f(l)) * 0.6931471805599453f;
+      } else {
+        const float inv = 1.f / sum;
+        if (lane < D / 4)
+          *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + ib * a.o_bs + (int64_t)(h0 + h) * a.o_hs + 4 * lane) =
+              make_uint2(pack<T>(o.x * inv, o.y * inv), pack<T>(o.z * inv, o.w * inv));
+        if (lane == 0 && a.lse) a.lse[ib * a.lse_bs + h0 + h] = (base + log2f(sum)) * 0.6931471805599453f;
       }
     }
-    i = end;
   }
   if (SPLIT && tid == 0) a.owner[blockIdx.x] = own;
 }
@@ -863,10 +924,17 @@ bool split(const KvbPagedDecodeParams* p) {
   return width > kItemBlocks;
 }
 
-int64_t part_floats(const KvbPagedDecodeParams* p) {
-  const int nh = 8 * head_tiles(p);
-  return (int64_t)nh * p->head_dim + 2 * nh;
-}
+// Workspace of a split launch: joined pieces, warps' first pieces, owners.
+struct Room {
+  int64_t part, first, owner, bytes;
+  explicit Room(const KvbPagedDecodeParams* p) {
+    const int64_t nh = 8 * head_tiles(p);
+    part = 0;
+    first = part + 4 * kSms * 2 * (nh * p->head_dim + 2 * nh);
+    owner = first + 4 * kSms * std::max(8, kWarpsI8) * (nh * (p->head_dim + 4) + 2 * nh);
+    bytes = owner + kSms * (int64_t)sizeof(int4);
+  }
+};
 
 int check(const KvbPagedDecodeParams* p) {
   if (!p) return fail(KVB_ERR_INVALID, "params is NULL");
@@ -960,7 +1028,7 @@ cudaError_t launch(const CUtensorMap& map, const Args& a, bool is_split, cudaStr
   auto kern = is_split ? kvb_paged_decode_kernel<T, D, I8, NT, true> : kvb_paged_decode_kernel<T, D, I8, NT, false>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kern, dim3(is_split ? a.ctas : a.batch * a.items), kThreads, G::SMEM, s, map, a);
+  e = launch_pdl(kern, dim3(is_split ? a.ctas : a.batch * a.items), G::THREADS, G::SMEM, s, map, a);
   if (e != cudaSuccess || !is_split || a.ctas == 1) return e;
   return launch_pdl(kvb_paged_join_kernel<T, D, NT>, dim3(a.ctas, std::min(a.group, 8 * NT)), 256, 0, s, a);
 }
@@ -988,7 +1056,7 @@ cudaError_t launch_t(const KvbPagedDecodeParams* p, const CUtensorMap& map, cons
 extern "C" int64_t kvb_paged_decode_workspace_bytes(const KvbPagedDecodeParams* p) {
   if (kvb_pd::check(p) != KVB_OK) return -1;
   if (p->batch == 0 || !kvb_pd::split(p)) return 0;
-  return kvb_pd::kSms * (2 * kvb_pd::part_floats(p) * 4 + (int64_t)sizeof(int4));
+  return kvb_pd::Room(p).bytes;
 }
 
 extern "C" int kvb_paged_decode_fwd(const KvbPagedDecodeParams* p, void* stream) {
@@ -1031,8 +1099,11 @@ extern "C" int kvb_paged_decode_fwd(const KvbPagedDecodeParams* p, void* stream)
   if (is_split) {
     const int64_t most = (int64_t)p->batch * p->max_blocks_per_seq * a.items;
     a.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(kvb_pd::kSms, (most + kvb_pd::kMinUnits - 1) / kvb_pd::kMinUnits));
-    a.part = static_cast<float*>(p->workspace);
-    a.owner = reinterpret_cast<int4*>(a.part + kvb_pd::kSms * 2 * kvb_pd::part_floats(p));
+    const kvb_pd::Room room(p);
+    uint8_t* w = static_cast<uint8_t*>(p->workspace);
+    a.part = reinterpret_cast<float*>(w + room.part);
+    a.first = reinterpret_cast<float*>(w + room.first);
+    a.owner = reinterpret_cast<int4*>(w + room.owner);
   }
   CUtensorMap map;
   std::string err;
