@@ -33,6 +33,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <mutex>
 #include <string>
@@ -53,6 +54,7 @@ constexpr int kSms = 148;
 constexpr float kRaise = 8.f;              // log2 units a score may pass the running maximum by
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kWarpsI8 = 12;               // warps per CTA over int8 pools (8 otherwise)
+constexpr int kItemCost = 1;               // an item's start and end, in blocks
 constexpr int kItemBlocks = 64;            // tables up to this wide take one CTA per item
 constexpr int kMinUnits = 8;               // blocks per CTA below which fewer CTAs share them
 constexpr int kSplitRows = 8192;           // most rows of a split launch (prefix sums in shared memory)
@@ -135,6 +137,15 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// D = A B + C in float16
+__device__ __forceinline__ void mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                         const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
 template <typename E>
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {   // lo in the low half
   if constexpr (std::is_same<E, __half>::value) {
@@ -156,15 +167,12 @@ __device__ __forceinline__ float2 unpack(uint32_t u) {
   }
 }
 
-// Four int8 codes (biased by 128) to float16 pairs, exactly: a byte under the exponent of
-// 1024 is 1024 + code + 128.
+// Two of four int8 codes, biased by 128 to 0 .. 255, as float16: under a zero byte a code is
+// (code + 128) * 2^-24, exactly (a subnormal, which the tensor core multiplies as any other);
+// the bias leaves through the accumulator's start.
+constexpr float kCode = 1.f / 16777216.f;  // 2^-24
 __device__ __forceinline__ uint32_t codes_to_half(uint32_t biased, uint32_t select) {
-  const uint32_t u = __byte_perm(biased, 0x64646464u, select);
-  __half2 h;
-  memcpy(&h, &u, 4);
-  const __half2 bias = __floats2half2_rn(1152.f, 1152.f);
-  h = __hsub2(h, bias);
-  return *reinterpret_cast<const uint32_t*>(&h);
+  return __byte_perm(biased, 0u, select);
 }
 
 // Waits for a phase; false after 2 s (the status word says so).
@@ -251,6 +259,8 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     kvb_paged_decode_kernel(const __grid_constant__ CUtensorMap map, const Args a) {
   using G = Geo<D, I8, NT>;
   using E = typename std::conditional<I8, __half, T>::type;   // MMA operand type
+  // int8 pools under bfloat16: float16 weights (2^-11) are well below the output's own 2^-8
+  constexpr bool LOW = !(I8 && std::is_same<T, __nv_bfloat16>::value);
   constexpr int MT = G::DP / 16, KS = G::DP / 16, NS = G::NS, NH = G::NH;
   constexpr int kWarps = G::WARPS, kThreads = G::THREADS;
   extern __shared__ uint8_t smem_raw[];
@@ -261,7 +271,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   uint8_t* after = smem + kWarps * NS * (G::STAGE + G::SCALES);
   int32_t* prefix = reinterpret_cast<int32_t*>(smem);                  // before the first load
   uint64_t* bars = reinterpret_cast<uint64_t*>(after);
-  // [kWarps][2] pieces: request (-1: none), item, blocks, CTAs spanned if the item begins here
+  // [kWarps][2] pieces: request (-1: none), item, CTAs the item spans if it begins here (or 0)
   int4* notes = reinterpret_cast<int4*>(bars + kWarps * NS);
   int32_t* wsum = reinterpret_cast<int32_t*>(notes + 2 * kWarps);
   const uint32_t ring_u = smem_u32(ring), scales_u = smem_u32(scales), bar_u = smem_u32(bars + warp * NS);
@@ -282,59 +292,90 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   int64_t u = 0, total = 0;     // split launch: the unit's place among all rows' units
   int ctas = 1;                 // split launch: CTAs that get units
   if constexpr (SPLIT) {
-    // exclusive prefix sums of the rows' blocks, in shared memory
-    int base = 0, err = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
-      const int bb = b0 + tid;
-      int n = 0;
-      if (bb < a.batch) {
-        n = (row_len(a, bb) + 15) >> 4;
-        if ((int64_t)a.lens[bb] > (int64_t)a.width * 16) err = KVB_STATUS_BAD_LENGTH;
-      }
-      int x = n;
+    // A row weighs its blocks and kItemCost for each of its items; the weights laid end to end
+    // are shared out, so u and left count places, of which an item's first nb are its blocks.
+    b = j = blk = nb = 0;
+    left = 0;
+    const int me = blockIdx.x * kWarps + warp;
+    int before = 0, weight = 0, err = 0;
+    auto row = [&](int i) {
+      const int n = (row_len(a, i) + 15) >> 4;
+      if ((int64_t)a.lens[i] > (int64_t)a.width * 16) err = KVB_STATUS_BAD_LENGTH;
+      return n ? n + kItemCost : 0;
+    };
+    auto scan = [&](int x) {
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(~0u, x, o);
         if (lane >= o) x += y;
       }
-      if (lane == 31) wsum[warp] = x;
-      __syncthreads();
-      int sum = 0;
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) x += wsum[w];
-        sum += wsum[w];
+      return x;
+    };
+    auto share = [&](int rows_weight) {
+      total = (int64_t)rows_weight * a.items;
+      // no CTA without a block, so an item's CTAs are consecutive
+      ctas = (int)min((int64_t)a.ctas, quot(total + kMinUnits - 1, kMinUnits));
+      if ((int)blockIdx.x < ctas) {
+        const Shares sh(total, ctas * kWarps);
+        u = sh.first(me);
+        left = sh.first(me + 1) - u;
       }
-      if (bb < a.batch) prefix[bb] = base + x;      // inclusive
-      base += sum;
+    };
+    if (a.batch <= 32) {                            // every warp for itself
+      const int w = lane < a.batch ? row(lane) : 0, sum = scan(w);
+      share(__shfl_sync(~0u, sum, 31));
+      const uint32_t past = __ballot_sync(~0u, (int64_t)sum * a.items > u);
+      b = past ? __ffs(past) - 1 : 0;
+      weight = __shfl_sync(~0u, w, b);
+      before = __shfl_sync(~0u, sum, b) - weight;
+    } else {
+      int base = 0;
+      for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+        const int i = b0 + tid;
+        int x = scan(i < a.batch ? row(i) : 0);
+        if (lane == 31) wsum[warp] = x;
+        __syncthreads();
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < warp) x += wsum[w];
+          sum += wsum[w];
+        }
+        if (i < a.batch) prefix[i] = base + x;      // inclusive
+        base += sum;
+        __syncthreads();
+      }
+      share(base);
+      if (left > 0) {
+        int lo = 0, hi = a.batch - 1;               // first row whose inclusive sum passes u
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if ((int64_t)prefix[mid] * a.items > u) hi = mid; else lo = mid + 1;
+        }
+        b = lo;
+        before = lo ? prefix[lo - 1] : 0;
+        weight = prefix[lo] - before;
+      }
+      fence_proxy_async_smem();                     // the loads go over the sums
       __syncthreads();
     }
     if (err && blockIdx.x == 0 && a.status) atomicOr(a.status, err);
-    total = (int64_t)base * a.items;
-    // no CTA without a unit, so an item's CTAs are consecutive
-    ctas = (int)min((int64_t)a.ctas, quot(total + kMinUnits - 1, kMinUnits));
-    const int me = blockIdx.x * kWarps + warp;
-    left = 0;
-    if ((int)blockIdx.x < ctas) {
-      const Shares sh(total, ctas * kWarps);
-      u = sh.first(me);
-      left = sh.first(me + 1) - u;
-    }
-    b = j = blk = nb = 0;
     if (left > 0) {
-      int lo = 0, hi = a.batch - 1;                 // first row whose inclusive sum passes u
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if ((int64_t)prefix[mid] * a.items > u) hi = mid; else lo = mid + 1;
-      }
-      b = lo;
-      const int before = lo ? prefix[lo - 1] : 0;
-      nb = prefix[lo] - before;
       const int64_t rel = u - (int64_t)before * a.items;
-      j = (int)quot(rel, nb);
-      blk = (int)(rel - (int64_t)j * nb);
+      j = (int)quot(rel, weight);
+      blk = (int)(rel - (int64_t)j * weight);
+      nb = weight - kItemCost;
+      if (blk >= nb) {                              // between two items: on to the next
+        const int skip = weight - blk;
+        blk = 0;
+        u += skip;
+        left -= skip;
+        if (left > 0 && ++j == a.items) {
+          j = 0;
+          do { nb = (row_len(a, ++b) + 15) >> 4; } while (nb == 0);
+        }
+      }
     }
-    fence_proxy_async_smem();                       // the loads go over the sums
-    __syncthreads();
   } else {
     b = blockIdx.x / a.items;
     j = blockIdx.x - b * a.items;
@@ -384,8 +425,8 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     }
     if constexpr (I8) copies_arrive(bar);
     ++issued;
-    --to_issue;
-    if (++pblk == pnb && to_issue > 0) {
+    to_issue -= ++pblk == pnb ? 1 + (SPLIT ? kItemCost : 0) : 1;
+    if (pblk == pnb && to_issue > 0) {
       pblk = 0;
       if (++pj == a.items) {
         pj = 0;
@@ -443,10 +484,11 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
       }
     }
   };
-  constexpr bool AHEAD = NT == 1;                   // the next item's heads fit in registers too
+  constexpr bool AHEAD = NT == 1 && !I8;                   // the next item's heads fit in registers too
   State<MT, NT> st;
   uint32_t qf[NT][KS][2], qn[NT][KS][2];
   float qx[NT][2];              // what turns S into log2 scores, per head of this lane's columns
+  float qb[NT][2];              // int8: -128 * 2^-24 * sum q, the codes' bias in S
   uint32_t used = 0;
   bool alive = true, fetched = false;
   if (left > 0) load_q(qf, b, j);
@@ -458,7 +500,8 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     const int len = row_len(a, b);
     const int first = blk;
     const int stop = (int)min((int64_t)nb, blk + left);
-    const bool last = left == stop - first;
+    const int past = stop == nb && SPLIT ? kItemCost : 0;
+    const bool last = left <= stop - first + past;
     st.clear();
     if constexpr (AHEAD) {
       if (fetched) {
@@ -485,14 +528,22 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
         const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 254);
         const float f = __uint_as_float((uint32_t)max(254 - e, 1) << 23);
         const float inv = __uint_as_float((uint32_t)min(e, 253) << 23);
+        float sum = 0.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           const float2 x = unpack<T>(qf[t][ks][0]), y = unpack<T>(qf[t][ks][1]);
           qf[t][ks][0] = pack<__half>(x.x * f, x.y * f);
           qf[t][ks][1] = pack<__half>(y.x * f, y.y * f);
+          const float2 xr = unpack<__half>(qf[t][ks][0]), yr = unpack<__half>(qf[t][ks][1]);
+          sum += (xr.x + xr.y) + (yr.x + yr.y);
         }
-        qx[t][0] = __shfl_sync(~0u, inv, 8 * c) * a.scale_log2;
-        qx[t][1] = __shfl_sync(~0u, inv, 8 * c + 4) * a.scale_log2;
+        sum += __shfl_xor_sync(~0u, sum, 1);
+        sum += __shfl_xor_sync(~0u, sum, 2);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          qx[t][i] = __shfl_sync(~0u, inv, 8 * c + 4 * i) * a.scale_log2 * (1.f / kCode);
+          qb[t][i] = __shfl_sync(~0u, sum, 8 * c + 4 * i) * (-128.f * kCode);
+        }
       }
     }
     // the item after this one
@@ -519,7 +570,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sa[t][0][i] = sa[t][1][i] = 0.f;
+        for (int i = 0; i < 4; ++i) sa[t][0][i] = I8 ? qb[t][i & 1] : 0.f, sa[t][1][i] = 0.f;
       if constexpr (!I8) {
         const uint32_t ka = base + ((lane & 7) + ((lane >> 3) & 1) * 8) * 128;
         const uint32_t kx = (((lane >> 4) ^ (lane & 7)) << 4);
@@ -601,7 +652,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
           const uint32_t hi = pack<E>(p[2 * h], p[2 * h + 1]);
           const float2 back = unpack<E>(hi);
           ph[t][h] = transpose8(hi);
-          pl[t][h] = transpose8(pack<E>(p[2 * h] - back.x, p[2 * h + 1] - back.y));
+          if (LOW) pl[t][h] = transpose8(pack<E>(p[2 * h] - back.x, p[2 * h + 1] - back.y));
         }
       }
       // O^T += V^T P^T
@@ -652,6 +703,15 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
           const uint4 z = lds128(sc + 32 + r * (W * 8) + k * 16);
           vs[4 * k] = z.x, vs[4 * k + 1] = z.y, vs[4 * k + 2] = z.z, vs[4 * k + 3] = z.w;
         }
+        // -128 * 2^-24 * the block's weights: what the codes' bias adds to every feature
+        float bias[NT][4];
+        const uint32_t minus[4] = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};   // -2^-17
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          bias[t][0] = bias[t][1] = bias[t][2] = bias[t][3] = 0.f;
+          mma<E>(bias[t], minus, ph[t][0], ph[t][1]);
+          if (LOW) mma<E>(bias[t], minus, pl[t][0], pl[t][1]);
+        }
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           const uint32_t t01[2] = {__byte_perm(v[0][w], v[1][w], 0x5140), __byte_perm(v[0][w], v[1][w], 0x7362)};
@@ -664,9 +724,9 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
             const float2 z = unpack<__half>(vs[jj]);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-              float o[4] = {0.f, 0.f, 0.f, 0.f};
-              mma<E>(o, f, ph[t][0], ph[t][1]);
-              mma<E>(o, f, pl[t][0], pl[t][1]);
+              float o[4];
+              mma_from(o, f, ph[t][0], ph[t][1], bias[t]);
+              if (LOW) mma<E>(o, f, pl[t][0], pl[t][1]);
               st.acc[t][jj][0] += z.x * o[0];
               st.acc[t][jj][1] += z.x * o[1];
               st.acc[t][jj][2] += z.y * o[2];
@@ -697,7 +757,8 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
       // whole: normalised and written from here
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const float i0 = 1.f / st.l[t][0], i1 = 1.f / st.l[t][1];
+        const float unit = I8 ? 1.f / kCode : 1.f;
+        const float i0 = unit / st.l[t][0], i1 = unit / st.l[t][1];
         T* o = static_cast<T*>(a.o) + b * a.o_bs + (int64_t)(h0 + t * 8) * a.o_hs;
         if constexpr (!I8) {
 #pragma unroll
@@ -744,7 +805,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const int d = I8 ? r * (G::DP / 8) + 2 * jj + k : jj * 16 + 8 * k + r;
-              if (!I8 || d < D) p[h * G::OS + d] = st.acc[t][jj][2 * k + i];
+              if (!I8 || d < D) p[h * G::OS + d] = st.acc[t][jj][2 * k + i] * (I8 ? 1.f / kCode : 1.f);
             }
           if (r == 0) {
             p[NH * G::OS + h] = st.m[t][i];
@@ -757,11 +818,11 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
           span = 1;
           if constexpr (SPLIT) span = Shares(total, ctas * kWarps).holder(u + nb - 1) / kWarps - (int)blockIdx.x + 1;
         }
-        notes[2 * warp + (last ? 1 : 0)] = make_int4(b, j, n, span);
+        notes[2 * warp + (last ? 1 : 0)] = make_int4(b, j, span, 0);
       }
     }
-    u += n;
-    left -= n;
+    u += n + past;
+    left -= n + past;
     blk = 0;
     b = b2;
     j = j2;
@@ -783,18 +844,16 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   while (todo) {
     const int at = __ffs(todo) - 1;
     const int ib = __shfl_sync(~0u, note.x, at), ij = __shfl_sync(~0u, note.y, at);
-    const int span = __shfl_sync(~0u, note.w, at);
+    const int span = __shfl_sync(~0u, note.z, at);
     const bool mine = note.x == ib && note.y == ij;
     const uint32_t members = __ballot_sync(~0u, mine);
-    const int n = __reduce_add_sync(~0u, mine ? note.z : 0);
     todo &= ~members;
     const int kvh = ij / a.tiles, h0 = kvh * a.group + (ij - kvh * a.tiles) * NH;
     const int heads = min(NH, (kvh + 1) * a.group - h0);
     // an item that continues from the CTA before takes the first workspace slot, one that
     // continues into the next CTA (and began here) the second
     float* part = nullptr;
-    if (n != (row_len(a, ib) + 15) >> 4) {
-      if (!SPLIT) return;                           // a wait ran out
+    if (SPLIT && span != 1) {                       // 1: all of it is here
       part = a.part + ((int64_t)blockIdx.x * 2 + (span > 0 ? 1 : 0)) * G::PART;
       if (span > 0) own = make_int4(ib, ij, span, 0);
     }
@@ -853,17 +912,26 @@ __global__ void __launch_bounds__(256) kvb_paged_join_kernel(const Args a) {
   const int tid = threadIdx.x, h = blockIdx.y;
   griddep_wait();
   griddep_launch_dependents();
-  const int4 own = a.owner[blockIdx.x];
-  const int span = min(own.z, a.ctas - (int)blockIdx.x);
-  const int kvh = own.y / a.tiles, h0 = kvh * a.group + (own.y - kvh * a.tiles) * NH;
-  if (span <= 0 || h >= (kvh + 1) * a.group - h0) return;
+  // What an item of this CTA would read is loaded before the note that says whether there is
+  // one: piece k > 0 is the first slot of CTA blockIdx.x + k.
+  const int most = a.ctas - (int)blockIdx.x;
   const float* first = a.part + ((int64_t)blockIdx.x * 2 + 1) * PART;
-  // piece k > 0 is the first slot of CTA blockIdx.x + k
   auto at = [&](int k) { return k == 0 ? first : first + ((int64_t)2 * k - 1) * PART; };
+  const int g = tid / Q, x = tid - g * Q;
   float m = -INFINITY, l = 0.f;
-  if (tid < span) {
+  float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int4 own = a.owner[blockIdx.x];
+  if (tid < most) {
     m = at(tid)[NH * D + h];
     l = at(tid)[NH * D + NH + h];
+  }
+  if (g < min(GROUPS, most)) v0 = *reinterpret_cast<const float4*>(at(g) + h * D + 4 * x);
+  const int span = min(own.z, most);
+  const int kvh = own.y / a.tiles, h0 = kvh * a.group + (own.y - kvh * a.tiles) * NH;
+  if (span <= 0 || h >= (kvh + 1) * a.group - h0) return;
+  if (tid >= span) {
+    m = -INFINITY;
+    l = 0.f;
   }
   float top = m;
 #pragma unroll
@@ -884,11 +952,11 @@ __global__ void __launch_bounds__(256) kvb_paged_join_kernel(const Args a) {
   total = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) total += red[i];
-  const int g = tid / Q, x = tid - g * Q;
   if (g < GROUPS) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (g < span) acc = make_float4(w[g] * v0.x, w[g] * v0.y, w[g] * v0.z, w[g] * v0.w);
 #pragma unroll 4
-    for (int k = g; k < span; k += GROUPS) {
+    for (int k = g + GROUPS; k < span; k += GROUPS) {
       const float4 v = *reinterpret_cast<const float4*>(at(k) + h * D + 4 * x);
       acc.x += w[k] * v.x;
       acc.y += w[k] * v.y;
@@ -954,7 +1022,7 @@ int check(const KvbPagedDecodeParams* p) {
   if (p->max_blocks_per_seq < 1 || p->block_table_stride < p->max_blocks_per_seq)
     return fail(KVB_ERR_INVALID,
                 "max_blocks_per_seq must be >= 1 and block_table_stride at least that");
-  if ((int64_t)p->batch * p->max_blocks_per_seq > 0x7fffffff || p->max_blocks_per_seq > (1 << 27) - 1)
+  if ((int64_t)p->batch * (p->max_blocks_per_seq + kItemCost) > 0x7fffffff || p->max_blocks_per_seq > (1 << 27) - 1)
     return fail(KVB_ERR_UNSUPPORTED, "batch * max_blocks_per_seq must be below 2^31, one row's blocks below 2^27");
   if (p->batch == 0) return KVB_OK;
   if (!p->q || !p->o || !p->kv_pool || !p->block_tables || !p->seq_lens)
@@ -1026,8 +1094,17 @@ template <typename T, int D, bool I8, int NT>
 cudaError_t launch(const CUtensorMap& map, const Args& a, bool is_split, cudaStream_t s) {
   using G = Geo<D, I8, NT>;
   auto kern = is_split ? kvb_paged_decode_kernel<T, D, I8, NT, true> : kvb_paged_decode_kernel<T, D, I8, NT, false>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
+  // the shared-memory limit is set once per device and instantiation
+  static std::atomic<uint64_t> ready[2];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev > 63 || !(ready[is_split].load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
+    if (e != cudaSuccess) return e;
+    ready[is_split].fetch_or(bit, std::memory_order_release);
+  }
   e = launch_pdl(kern, dim3(is_split ? a.ctas : a.batch * a.items), G::THREADS, G::SMEM, s, map, a);
   if (e != cudaSuccess || !is_split || a.ctas == 1) return e;
   return launch_pdl(kvb_paged_join_kernel<T, D, NT>, dim3(a.ctas, std::min(a.group, 8 * NT)), 256, 0, s, a);

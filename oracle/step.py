@@ -78,15 +78,15 @@ def gather(pool, table, n, k_scale=None, v_scale=None):
 
 
 def decode_attention(q, pool, tables, lens, scale, k_scale=None, v_scale=None):
-    """q [B, Hq, D].  Returns o, lse and, for error bounds, ``a`` = sum_t w_t |v_t| (as o),
-    ``x`` = max_t scale * sum_d |q_d k_td| (as lse), ``vmax`` and ``kq`` = max_t scale *
-    max_d|q| * sum_d |k_td| (as lse)."""
+    """q [B, Hq, D].  Returns o, lse and, for error bounds, ``a`` = sum_t w_t |v_t| (as o) and, as
+    lse, ``x`` = max_t scale * sum_d |q_d k_td|, ``vmax`` = max|v|, ``kq`` = max_t scale * max_d|q| *
+    sum_d |k_td| and ``kb`` = scale * sum_d|q| * max|k|."""
     B, Hq, D = q.shape
     H = pool.shape[2]
     g = Hq // H
     o, a = np.zeros((B, Hq, D)), np.zeros((B, Hq, D))
     lse = np.full((B, Hq), -np.inf)
-    x, vmax, kq = np.zeros((B, Hq)), np.zeros((B, Hq)), np.zeros((B, Hq))
+    x, vmax, kq, kb = (np.zeros((B, Hq)) for _ in range(4))
     cap = tables.shape[1] * BLOCK
     for b in range(B):
         n = min(int(lens[b]), cap)
@@ -104,7 +104,8 @@ def decode_attention(q, pool, tables, lens, scale, k_scale=None, v_scale=None):
             x[b, h] = scale * (np.abs(k) @ np.abs(qq)).max()
             vmax[b, h] = np.abs(v).max()
             kq[b, h] = scale * np.abs(qq).max() * np.abs(k).sum(-1).max()
-    return o, lse, a, x, vmax, kq
+            kb[b, h] = scale * np.abs(qq).sum() * np.abs(k).max()
+    return o, lse, a, x, vmax, kq, kb
 
 
 def logits(x, token_ids=None, prompt_lens=None, total_lens=None, repetition=None, frequency=None,

@@ -2,14 +2,18 @@
 64-bit restatement (``oracle/step.py``), and all of them together as a step.
 
 Tolerances.  u = 2^-24 is float32's half step.  Attention: a score is a dot of D products
-in float32, off by at most (D + 4) u times scale * sum|q k| (``x``), plus, over int8 pools,
-the query's rounding to float16 multiples of 2^-25 of its row maximum (``kq`` * 2^-25, twice
-for the power-of-two normalisation); the exponential and the scale's product add 2^-21 of
-relative error, so a weight is off by e = x (D + 6) u + kq 2^-24 + 2^-20 relative.  The sums of n
-weights add n u, the weights themselves are carried in two 16-bit halves (2^-16 of relative
-error in bfloat16; in float16 2^-21 and at worst 2^-24 absolute, of a largest weight >= 1).
-So |o - o64| <= half a step of the output's type times |o| + (2 e + 2 n u + 2^-16) a +
-n 2^-23 max|v| with a = sum w|v|, and |lse - lse64| <= e + 2 n u + 2^-20 + 2 u |lse|.
+in float32, off by at most (D + 6) u times scale * sum|q k| (``x``).  The exponential and the
+scale's product add 2^-21 of relative error, so a weight is off by e = (D + 6) u x + 2^-20
+relative.  The sums of n weights add n u; the weights themselves are carried in two 16-bit
+halves (2^-16 of relative error in bfloat16; in float16 2^-21 and at worst 2^-24 absolute, of a
+largest weight >= 1).  So |o - o64| <= half a step of the output's type times |o| + (2 e + 2 n u +
+2^-16) a + n 2^-23 max|v| with a = sum w|v|, and |lse - lse64| <= e + 2 n u + 2^-20 + 2 u |lse|.
+
+Over int8 pools a code c is multiplied as c + 128 <= 255 and the bias taken out of the sum, so
+a score's terms are at most 255 scales = 2.1 max|k| times |q| (``kb``) instead of |q k|: e has
+(D + 6) u (x + 2.1 kb); the query is rounded to multiples of 2^-25 of its row maximum (``kq`` *
+2^-24 with the normalisation).  The same bias in V adds 18 roundings of 2.1 max|v|: 48 u max|v|.
+Under bfloat16 the weights are single float16 numbers: 2^-11 a instead of 2^-16 a.
 """
 
 import math
@@ -225,14 +229,17 @@ def _np(t):
 def _check_attention(o, lse, q, pool, tables, lens, scale, ks=None, vs=None):
     dtype, int8 = q.dtype, ks is not None
     D = q.shape[-1]
-    want, wl, a, x, vmax, kq = ostep.decode_attention(
+    want, wl, a, x, vmax, kq, kb = ostep.decode_attention(
         _np(q[:, :, 0]), _np(pool), tables.numpy(), lens, scale, _np(ks), _np(vs))
     n = np.minimum(np.maximum(np.asarray(lens), 0), tables.shape[1] * 16)[:, None]
-    e = x * (D + 6) * U + (kq * 2.0 ** -24 if int8 else 0.0) + 2.0 ** -20
+    e = x * (D + 6) * U + 2.0 ** -20
+    if int8:
+        e = e + kb * 2.1 * (D + 6) * U + kq * 2.0 ** -24
+    weights = 2.0 ** -11 if int8 and dtype == torch.bfloat16 else 2.0 ** -16
     half = torch.finfo(dtype).eps / 2
     small = torch.finfo(dtype).tiny
-    bound = half * np.abs(want) + ((2 * e + 2 * n * U + 2.0 ** -16)[..., None]) * a + \
-        (n * 2.0 ** -23 * vmax)[..., None] + small
+    bound = half * np.abs(want) + ((2 * e + 2 * n * U + weights)[..., None]) * a + \
+        ((n * 2.0 ** -23 + (48 * U if int8 else 0.0)) * vmax)[..., None] + small
     got = o[:, :, 0].double().cpu().numpy()
     assert np.isfinite(got).all()
     bad = np.abs(got - want) > bound
