@@ -321,13 +321,31 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
         left = sh.first(me + 1) - u;
       }
     };
-    if (a.batch <= 32) {                            // every warp for itself
-      const int w = lane < a.batch ? row(lane) : 0, sum = scan(w);
+    if (a.batch <= 256) {                           // every warp for itself, 8 rows a lane
+      int w[8], own = 0;
+      const int per = (a.batch + 31) >> 5, from = lane * per;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i] = i < per && from + i < a.batch ? row(from + i) : 0;
+        own += w[i];
+      }
+      const int sum = scan(own);
       share(__shfl_sync(~0u, sum, 31));
       const uint32_t past = __ballot_sync(~0u, (int64_t)sum * a.items > u);
-      b = past ? __ffs(past) - 1 : 0;
-      weight = __shfl_sync(~0u, w, b);
-      before = __shfl_sync(~0u, sum, b) - weight;
+      const int src = past ? __ffs(past) - 1 : 0;
+      int row_b = from;                             // on lane src: its row that holds u
+      before = sum - own;
+      weight = w[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i)
+        if (row_b == from + i - 1 && i < per && (int64_t)(before + weight) * a.items <= u) {
+          ++row_b;
+          before += weight;
+          weight = w[i];
+        }
+      b = __shfl_sync(~0u, row_b, src);
+      before = __shfl_sync(~0u, before, src);
+      weight = __shfl_sync(~0u, weight, src);
     } else {
       int base = 0;
       for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
@@ -390,7 +408,15 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   int pb = b, pj = j, pblk = blk, pnb = nb;
   int64_t to_issue = left;
   int ids = 0, cached_b = -1, cached_c = -1;        // 32 table entries, one per lane
-  uint32_t issued = 0;
+  uint32_t issued = 0, ps = 0;                      // loads issued, the next one's stage
+  int pkv = a.tiles == 1 ? pj : pj / a.tiles;       // their KV head
+  // lanes 0, 1 copy the K scales, the next D / 8 the V scales: 16 bytes each
+  const __half* scale_src = nullptr;
+  int64_t scale_step = 0;
+  if constexpr (I8) {
+    scale_src = lane < 2 ? a.k_scale + 8 * lane : a.v_scale + 8 * (lane - 2);
+    scale_step = lane < 2 ? 16 : D;
+  }
   auto issue = [&]() {
     const int chunk = pblk >> 5;
     if (pb != cached_b || chunk != cached_c) {
@@ -400,22 +426,19 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
       cached_c = chunk;
     }
     const int id = __shfl_sync(~0u, ids, pblk & 31);
-    const uint32_t s = issued % NS;
-    const uint32_t bar = bar_u + 8 * s, dst = ring_u + s * G::STAGE;
-    const int kvh = a.tiles == 1 ? pj : pj / a.tiles;
+    const uint32_t s = ps, bar = bar_u + 8 * s, dst = ring_u + s * G::STAGE;
+    ps = ps + 1 == NS ? 0 : ps + 1;
     const bool ok = (unsigned)id < (unsigned)a.num_blocks;
     if (lane == 0) {
       mbar_arrive_expect_tx(bar, G::STAGE);
 #pragma unroll
       for (int h = 0; h < G::HALVES; ++h)
-        tma_load_4d(dst + h * G::BOX, &map, h * 64, kvh * 16, 0, ok ? id : -1, bar);
+        tma_load_4d(dst + h * G::BOX, &map, h * 64, pkv * 16, 0, ok ? id : -1, bar);
     }
     if constexpr (I8) {
-      if (ok && lane < 2 + D / 8) {
-        const int64_t bh = (int64_t)id * a.num_kv_heads + kvh;
+      if (ok && lane < 2 + D / 8)
         copy16(scales_u + s * G::SCALES + 16 * lane,
-               lane < 2 ? a.k_scale + bh * 16 + 8 * lane : a.v_scale + bh * D + 8 * (lane - 2));
-      }
+               scale_src + ((int64_t)id * a.num_kv_heads + pkv) * scale_step);
     }
     if (!ok) {                                      // reads as zeros
       if (I8)
@@ -432,9 +455,10 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
         pj = 0;
         do { pnb = (row_len(a, ++pb) + 15) >> 4; } while (pnb == 0);
       }
+      pkv = a.tiles == 1 ? pj : pj / a.tiles;
       // the item's query heads will be wanted NS blocks from now
-      const int kv = a.tiles == 1 ? pj : pj / a.tiles, h = kv * a.group + (pj - kv * a.tiles) * NH + (lane >> 1);
-      if ((lane >> 1) < NH && h < (kv + 1) * a.group)
+      const int h = pkv * a.group + (pj - pkv * a.tiles) * NH + (lane >> 1);
+      if ((lane >> 1) < NH && h < (pkv + 1) * a.group)
         prefetch_l2(static_cast<const T*>(a.q) + pb * a.q_bs + h * a.q_hs + (lane & 1) * (D / 2));
     }
   };
@@ -489,7 +513,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   uint32_t qf[NT][KS][2], qn[NT][KS][2];
   float qx[NT][2];              // what turns S into log2 scores, per head of this lane's columns
   float qb[NT][2];              // int8: -128 * 2^-24 * sum q, the codes' bias in S
-  uint32_t used = 0;
+  uint32_t used = 0, cs = 0, phase = 0;             // loads consumed, the next one's stage and phase
   bool alive = true, fetched = false;
   if (left > 0) load_q(qf, b, j);
   while (left > 0 && alive) {
@@ -551,7 +575,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
 
 #pragma unroll 1
     for (; blk < stop; ++blk) {
-      const uint32_t s = used % NS, base = ring_u + s * G::STAGE, sc = scales_u + s * G::SCALES;
+      const uint32_t base = ring_u + cs * G::STAGE, sc = scales_u + cs * G::SCALES;
       if (blk + 1 == stop && !last) {
         if (j2 == a.items) {
           j2 = 0;
@@ -560,10 +584,11 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
         if constexpr (AHEAD) load_q(qn, b2, j2);
         fetched = true;
       }
-      if (!wait_full(bar_u + 8 * s, (used / NS) & 1, a.status)) {
+      if (!wait_full(bar_u + 8 * cs, phase, a.status)) {
         alive = false;
         break;
       }
+      if (++cs == NS) cs = 0, phase ^= 1;
       const int valid = len - blk * 16;             // >= 1; below 16 in the row's last block
       // S^T: two chains of MMAs
       float sa[NT][2][4];
@@ -840,6 +865,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   // ---- the CTA's pieces, joined item by item: a warp per head, a lane per four features ---------
   const int4 note = lane < 2 * kWarps ? notes[lane] : make_int4(-1, 0, 0, 0);
   uint32_t todo = __ballot_sync(~0u, note.x >= 0);
+  int task = 0;                                     // (item, head) pairs go round the warps
   int4 own = make_int4(0, 0, 0, 0);
   while (todo) {
     const int at = __ffs(todo) - 1;
@@ -860,7 +886,8 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     const float* from = (lane & 1) || !SPLIT
                             ? reinterpret_cast<const float*>(smem + (lane >> 1) * NS * G::STAGE)
                             : a.first + ((int64_t)blockIdx.x * kWarps + (lane >> 1)) * G::PIECE;
-    for (int h = warp; h < heads; h += kWarps) {
+    for (int h = 0; h < heads; ++h) {
+      if (task++ % kWarps != warp) continue;
       const float m = mine ? from[NH * G::OS + h] : -INFINITY, l = mine ? from[NH * G::OS + NH + h] : 0.f;
       float top = m;
 #pragma unroll
@@ -871,18 +898,22 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
 #pragma unroll
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (uint32_t left_of = members; left_of; left_of &= left_of - 1) {
-        const int k = __ffs(left_of) - 1;
-        const float f = __shfl_sync(~0u, w, k);
-        const float* p = (k & 1) || !SPLIT
-                             ? reinterpret_cast<const float*>(smem + (k >> 1) * NS * G::STAGE)
-                             : a.first + ((int64_t)blockIdx.x * kWarps + (k >> 1)) * G::PIECE;
-        if (lane < D / 4) {
-          const float4 v = *reinterpret_cast<const float4*>(p + h * G::OS + 4 * lane);
-          o.x += f * v.x;
-          o.y += f * v.y;
-          o.z += f * v.z;
-          o.w += f * v.w;
+      #pragma unroll 1
+      for (int k0 = 0; k0 < 2 * kWarps; k0 += 4) {
+        if (!((members >> k0) & 15)) continue;
+#pragma unroll
+        for (int k = k0; k < k0 + 4; ++k) {
+          const float f = __shfl_sync(~0u, w, k);
+          const float* p = (k & 1) || !SPLIT
+                               ? reinterpret_cast<const float*>(smem + (k >> 1) * NS * G::STAGE)
+                               : a.first + ((int64_t)blockIdx.x * kWarps + (k >> 1)) * G::PIECE;
+          if (((members >> k) & 1) && lane < D / 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + h * G::OS + 4 * lane);
+            o.x += f * v.x;
+            o.y += f * v.y;
+            o.z += f * v.z;
+            o.w += f * v.w;
+          }
         }
       }
       if (part) {

@@ -17,27 +17,36 @@ length that does not fit, an empty free list) go to the device's status word
 
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _check_tensor, _stream_handle, status_word
+from .ops import _DTYPES, _check_tensor, _status_words, status_word
 
 BLOCK_SIZE = 16
+
+# A decode step calls these operators once per layer, so the host's cost per call is kept
+# to a few checks: the stream handle comes from torch's C binding (2 us less than building a
+# Stream object), the device is switched only where it differs.
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _launch(fn, params, device, what: str) -> None:
     """One library call on the device's current stream."""
-    stream = _stream_handle(device)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(ctypes.byref(params), stream)
+    idx = device.index
+    if torch.cuda.current_device() == idx:
+        rc = fn(params, _raw_stream(idx))
     else:
         with torch.cuda.device(device):
-            rc = fn(ctypes.byref(params), stream)
+            rc = fn(params, _raw_stream(idx))
     _lib.check(rc, what)
+
+
+def _status_ptr(device) -> int:
+    w = _status_words.get(device.index)
+    return (status_word(device) if w is None else w).data_ptr()
 
 
 def _check_int32(name: str, t: torch.Tensor, ndim: int, device) -> None:
@@ -46,18 +55,21 @@ def _check_int32(name: str, t: torch.Tensor, ndim: int, device) -> None:
     if t.dtype != torch.int32 or t.dim() != ndim or t.device != device:
         raise RuntimeError(f"{name} must be a {ndim}-D int32 tensor on {device}, got "
                            f"{t.dim()}-D {t.dtype} on {t.device}")
-    if not (t.is_contiguous() if ndim == 1 else t.stride(-1) == 1 or t.shape[-1] == 1):
-        raise RuntimeError(f"{name} must be contiguous" if ndim == 1 else
-                           f"{name} must have contiguous rows")
+    if not t.is_contiguous():
+        if ndim == 1:
+            raise RuntimeError(f"{name} must be contiguous")
+        if t.stride(-1) != 1 and t.shape[-1] != 1:
+            raise RuntimeError(f"{name} must have contiguous rows")
 
 
 def _check_tables(block_tables: torch.Tensor, batch: int, device) -> int:
     """Row stride of the block tables (rows may be a slice of a wider buffer)."""
     _check_int32("block_tables", block_tables, 2, device)
-    if block_tables.shape[0] != batch or block_tables.shape[1] < 1:
+    rows, width = block_tables.shape
+    if rows != batch or width < 1:
         raise RuntimeError(f"block_tables must be [{batch}, >= 1], got {tuple(block_tables.shape)}")
-    stride = block_tables.stride(0) if batch > 1 else block_tables.shape[1]
-    if stride < block_tables.shape[1]:
+    stride = block_tables.stride(0) if batch > 1 else width
+    if stride < width:
         raise RuntimeError("block_tables rows must not overlap")
     return stride
 
@@ -96,46 +108,52 @@ def extend_block_tables(block_tables: torch.Tensor, seq_lens: torch.Tensor,
     if not block_tables.is_cuda:
         raise RuntimeError("block_tables must be on CUDA (kvboost_b200 has no CPU path)")
     dev = block_tables.device
-    B = block_tables.shape[0]
+    B, width = block_tables.shape if block_tables.dim() == 2 else (0, 0)
     stride = _check_tables(block_tables, B, dev)
-    for name, t, n in (("seq_lens", seq_lens, B), ("new_lens", new_lens, B), ("num_free", num_free, 1),
-                       ("free_blocks", free_blocks, None), ("seq_lens_out", seq_lens_out, B),
-                       ("num_free_out", num_free_out, 1)):
-        if t is None and name.endswith("_out"):
-            continue
-        _check_int32(name, t, 1, dev)
-        if n is not None and t.shape[0] != n:
-            raise RuntimeError(f"{name} must have {n} entries, got {t.shape[0]}")
+    _check_int32("seq_lens", seq_lens, 1, dev)
+    _check_int32("new_lens", new_lens, 1, dev)
+    _check_int32("num_free", num_free, 1, dev)
+    _check_int32("free_blocks", free_blocks, 1, dev)
+    if len(seq_lens) != B or len(new_lens) != B or len(num_free) != 1:
+        raise RuntimeError(f"seq_lens and new_lens must have {B} entries, num_free one")
     if not 1 <= B <= _lib.KVB_MAX_STEP_ROWS:
         raise RuntimeError(f"a step has 1 to {_lib.KVB_MAX_STEP_ROWS} rows, got {B}")
     T = int(max_new_tokens)
     if T < 0:
         raise RuntimeError("max_new_tokens must be >= 0")
-    slots = torch.empty(T, dtype=torch.int32, device=dev)
+    # the int32 results share one allocation: slots first (16-byte aligned)
+    slots, cu, lens_out, free_out = torch.empty(T + 2 * B + 2, dtype=torch.int32, device=dev).split(
+        (T, B + 1, B, 1))
     positions = torch.empty(T, dtype=torch.int64, device=dev)
-    cu = torch.empty(B + 1, dtype=torch.int32, device=dev)
     if seq_lens_out is None:
-        seq_lens_out = torch.empty(B, dtype=torch.int32, device=dev)
+        seq_lens_out = lens_out
+    else:
+        _check_int32("seq_lens_out", seq_lens_out, 1, dev)
     if num_free_out is None:
-        num_free_out = torch.empty(1, dtype=torch.int32, device=dev)
+        num_free_out = free_out
+    else:
+        _check_int32("num_free_out", num_free_out, 1, dev)
+    if len(seq_lens_out) != B or len(num_free_out) != 1:
+        raise RuntimeError(f"seq_lens_out must have {B} entries, num_free_out one")
     p = _lib.KvbExtendTablesParams(
-        B, block_tables.shape[1], BLOCK_SIZE, int(num_blocks), T, free_blocks.shape[0], stride,
+        B, width, BLOCK_SIZE, int(num_blocks), T, len(free_blocks), stride,
         block_tables.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(),
         num_free.data_ptr(), slots.data_ptr(), positions.data_ptr(), cu.data_ptr(),
-        seq_lens_out.data_ptr(), num_free_out.data_ptr(), status_word(dev).data_ptr())
+        seq_lens_out.data_ptr(), num_free_out.data_ptr(), _status_ptr(dev))
     _launch(_lib.load().kvb_extend_block_tables, p, dev, "kvb_extend_block_tables")
     return BlockTableStep(slots, positions, cu, seq_lens_out, num_free_out)
 
 
-def _check_pool(kv_pool: torch.Tensor, device, heads: int, head_dim: int) -> None:
+def _check_pool(kv_pool: torch.Tensor, device):
+    """(num_blocks, kv_heads, head_dim) of one layer's pool."""
     if not isinstance(kv_pool, torch.Tensor):
         raise TypeError("kv_pool must be a torch.Tensor")
-    if kv_pool.dim() != 5 or kv_pool.shape[1] != 2 or kv_pool.shape[3] != BLOCK_SIZE \
-            or not kv_pool.is_contiguous() or kv_pool.device != device:
+    shape = kv_pool.shape
+    if len(shape) != 5 or shape[1] != 2 or shape[3] != BLOCK_SIZE or not kv_pool.is_contiguous() \
+            or kv_pool.device != device:
         raise RuntimeError(f"kv_pool must be a contiguous [num_blocks, 2, kv_heads, 16, head_dim] "
-                           f"tensor on {device}, got {tuple(kv_pool.shape)} on {kv_pool.device}")
-    if kv_pool.shape[2] != heads or kv_pool.shape[4] != head_dim:
-        raise RuntimeError("pool heads / head_dim do not match")
+                           f"tensor on {device}, got {tuple(shape)} on {kv_pool.device}")
+    return shape[0], shape[2], shape[4]
 
 
 def append_paged_kv(k_new: torch.Tensor, v_new: torch.Tensor, kv_pool: torch.Tensor,
@@ -150,31 +168,35 @@ def append_paged_kv(k_new: torch.Tensor, v_new: torch.Tensor, kv_pool: torch.Ten
     """
     _check_tensor("k_new", k_new, 3)
     _check_tensor("v_new", v_new, 3)
-    if k_new.shape != v_new.shape or k_new.device != v_new.device:
+    dev = k_new.device
+    if k_new.shape != v_new.shape or v_new.device != dev:
         raise RuntimeError("k_new and v_new must have the same shape and device")
     T, H, D = k_new.shape
-    dev = k_new.device
-    _check_pool(kv_pool, dev, H, D)
-    if k_new.dtype != kv_pool.dtype or v_new.dtype != kv_pool.dtype:
-        raise RuntimeError(f"k_new and v_new must have the pool's dtype {kv_pool.dtype} "
+    num_blocks, heads, dim = _check_pool(kv_pool, dev)
+    if heads != H or dim != D:
+        raise RuntimeError("pool heads / head_dim do not match k_new")
+    dtype = kv_pool.dtype
+    if k_new.dtype != dtype or v_new.dtype != dtype:
+        raise RuntimeError(f"k_new and v_new must have the pool's dtype {dtype} "
                            "(int8 pools hold whole KIVI chunks)")
     if D % 8 or D > 256:
         raise RuntimeError(f"head_dim must be a multiple of 8 up to 256, got {D}")
     _check_int32("slots", slots, 1, dev)
-    if slots.shape[0] != T:
-        raise RuntimeError(f"slots must have {T} entries, got {slots.shape[0]}")
+    if len(slots) != T:
+        raise RuntimeError(f"slots must have {T} entries, got {len(slots)}")
     if T == 0:
         return
-    ks, vs = k_new.stride(), v_new.stride()
-    if ks[0] % 8 or ks[1] % 8 or k_new.data_ptr() % 16:
+    kt, kh, _ = k_new.stride()
+    vt, vh, _ = v_new.stride()
+    if kt % 8 or kh % 8 or k_new.data_ptr() % 16:
         k_new = k_new.clone(memory_format=torch.contiguous_format)
-        ks = k_new.stride()
-    if vs[0] % 8 or vs[1] % 8 or v_new.data_ptr() % 16:
+        kt, kh, _ = k_new.stride()
+    if vt % 8 or vh % 8 or v_new.data_ptr() % 16:
         v_new = v_new.clone(memory_format=torch.contiguous_format)
-        vs = v_new.stride()
+        vt, vh, _ = v_new.stride()
     p = _lib.KvbAppendPagedParams(
-        D, H, T, kv_pool.shape[0], k_new.data_ptr(), v_new.data_ptr(), ks[0], ks[1], vs[0], vs[1],
-        kv_pool.data_ptr(), slots.data_ptr(), status_word(dev).data_ptr())
+        D, H, T, num_blocks, k_new.data_ptr(), v_new.data_ptr(), kt, kh, vt, vh,
+        kv_pool.data_ptr(), slots.data_ptr(), _status_ptr(dev))
     _launch(_lib.load().kvb_append_paged_kv, p, dev, "kvb_append_paged_kv")
 
 
@@ -203,16 +225,17 @@ def paged_decode_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_tables:
         raise RuntimeError(f"q must hold one token per request [B, Hq, 1, D], got {tuple(q.shape)}")
     if D not in (64, 96, 128):
         raise RuntimeError(f"head_dim must be one of 64, 96, 128, got {D}")
-    Hkv = kv_pool.shape[2] if isinstance(kv_pool, torch.Tensor) and kv_pool.dim() == 5 else 0
-    _check_pool(kv_pool, dev, Hkv, D)
+    num_blocks, Hkv, dim = _check_pool(kv_pool, dev)
+    if dim != D:
+        raise RuntimeError(f"pool head_dim {dim} does not match the query's {D}")
     if Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise RuntimeError(f"num_q_heads ({Hq}) must be divisible by num_kv_heads ({Hkv})")
     stride = _check_tables(block_tables, B, dev)
     _check_int32("seq_lens", seq_lens, 1, dev)
-    if seq_lens.shape[0] != B:
-        raise RuntimeError(f"seq_lens must have {B} entries, got {seq_lens.shape[0]}")
-    num_blocks = kv_pool.shape[0]
-    if kv_pool.dtype == torch.int8:
+    if len(seq_lens) != B:
+        raise RuntimeError(f"seq_lens must have {B} entries, got {len(seq_lens)}")
+    dtype, pool_dtype = q.dtype, kv_pool.dtype
+    if pool_dtype == torch.int8:
         fmt = _lib.KVB_POOL_INT8_KIVI
         for name, t, shape in (("k_scale", k_scale, (num_blocks, Hkv, BLOCK_SIZE)),
                                ("v_scale", v_scale, (num_blocks, Hkv, D))):
@@ -222,32 +245,35 @@ def paged_decode_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_tables:
         ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
     else:
         fmt, ks, vs = _lib.KVB_POOL_COMPUTE, None, None
-        if kv_pool.dtype != q.dtype:
+        if pool_dtype != dtype:
             raise RuntimeError("a 16-bit pool must hold the compute dtype")
         if k_scale is not None or v_scale is not None:
             raise RuntimeError("scales belong to int8 pools")
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(D)
     if out is None:
-        out = torch.empty(B, Hq, 1, D, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(3) != 1 \
-            or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
-        raise RuntimeError("out must match q in shape, dtype and device, with 16-byte aligned heads")
-    lse = torch.empty(B, Hq, 1, dtype=torch.float32, device=dev) if return_lse else None
+        out = q.new_empty((B, Hq, 1, D))
+        ob, oh = Hq * D, D
+    else:
+        ob, oh = out.stride()[:2] if out.dim() == 4 else (1, 1)
+        if out.shape != q.shape or out.dtype != dtype or out.device != dev or out.stride(3) != 1 \
+                or ob % 8 or oh % 8 or out.data_ptr() % 16:
+            raise RuntimeError("out must match q in shape, dtype and device, with 16-byte aligned heads")
+    lse = torch.empty((B, Hq, 1), dtype=torch.float32, device=dev) if return_lse else None
     if B == 0:
         return out, lse
-    qs, os_ = q.stride(), out.stride()
-    if qs[0] % 8 or qs[1] % 8 or q.data_ptr() % 16:
+    qb, qh, _, _ = q.stride()
+    if qb % 8 or qh % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-        qs = q.stride()
+        qb, qh, _, _ = q.stride()
     p = _lib.KvbPagedDecodeParams(
-        _DTYPES[q.dtype], D, B, Hq, Hkv, BLOCK_SIZE, fmt, float(softmax_scale), q.data_ptr(),
-        out.data_ptr(), lse.data_ptr() if return_lse else None, qs[0], qs[1], os_[0], os_[1], Hq,
+        _DTYPES[dtype], D, B, Hq, Hkv, BLOCK_SIZE, fmt, softmax_scale, q.data_ptr(),
+        out.data_ptr(), lse.data_ptr() if return_lse else None, qb, qh, ob, oh, Hq,
         kv_pool.data_ptr(), ks, vs, num_blocks, block_tables.shape[1], stride,
         block_tables.data_ptr(), seq_lens.data_ptr(), 0 if max_seq_len is None else int(max_seq_len),
-        0, status_word(dev).data_ptr(), None, 0)
+        0, _status_ptr(dev), None, 0)
     lib = _lib.load()
-    need = lib.kvb_paged_decode_workspace_bytes(ctypes.byref(p))
+    need = lib.kvb_paged_decode_workspace_bytes(p)
     if need > 0:
         # partial results of this call: torch's caching allocator orders their reuse on the
         # current stream, so calls on concurrent streams never share them
