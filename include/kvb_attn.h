@@ -566,11 +566,12 @@ int kvb_append_paged_kv(const KvbAppendPagedParams* params, void* stream);
  * and pool slots past its last token are never used, whatever they hold.
  *
  * The rows' blocks are divided evenly over the GPU's warps, whatever the
- * lengths (device data); requests that end up on several CTAs are joined by a
- * second launch.  workspace: kvb_paged_decode_workspace_bytes(params) bytes
- * (-1: invalid params), 16-byte aligned, no initialisation needed; calls that
- * may overlap on the GPU must not share one.  max_seq_len (0: unknown) is a hint
- * that only chooses the launch shape; any value gives right results.
+ * lengths (device data), in one launch; requests that end up on several CTAs are
+ * joined through the workspace by the last of them.  workspace:
+ * kvb_paged_decode_workspace_bytes(params) bytes (-1: invalid params), 16-byte
+ * aligned, whatever it holds; calls that may overlap on the GPU must not share
+ * one.  max_seq_len (0: unknown) is a hint that only chooses the launch shape;
+ * any value gives right results (their last bits may differ).
  */
 typedef struct KvbPagedDecodeParams {
   int32_t dtype;

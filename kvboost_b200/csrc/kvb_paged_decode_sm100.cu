@@ -15,8 +15,8 @@
 // by TMA into the warp's ring of stages, several blocks ahead, through the block table;
 // no CTA-wide step sits in the loop.  Items that a warp holds whole it writes itself;
 // the pieces at its range's ends are joined in shared memory at the CTA's end, and what
-// still spans CTAs goes to the workspace for a second launch.  Short tables take one
-// CTA per item instead, whose warps split the item and never need that launch.
+// still spans CTAs goes to the workspace, where the CTA that finds all of an item's pieces
+// joins them.  Short tables take one CTA per item instead, whose warps split the item.
 //
 // Arithmetic (per block, tokens on the MMA's rows, query heads on its columns):
 //   S^T = K Q^T; online softmax down the rows against a maximum that is raised only when
@@ -75,7 +75,8 @@ struct Args {
   int32_t* status;
   float* part;                             // [ctas][2][NH * D + 2 * NH]
   float* first;                            // [ctas * warps][PIECE]: pieces that start a warp's range
-  int4* owner;                             // [ctas]: request, item, CTAs it spans (0: none)
+  uint64_t* flags;                         // [ctas][2][NH]: head's piece is in the workspace
+  uint64_t nonce;                          // what this call's flags read
 };
 
 // ---- warp-level primitives ------------------------------------------------------------------
@@ -214,22 +215,14 @@ struct Geo {
   static_assert(WARPS * NS * STAGE >= kSplitRows * 4, "prefix sums go over the stages");
 };
 
-// x / y for x < 2^63; the 32-bit division where it will do.
-__device__ __forceinline__ int64_t quot(int64_t x, int y) {
-  return (x >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
-}
-
-// total units over `workers`: worker i's first unit, and the worker that holds unit u.
+// total places over `workers`: worker i's first place, and the worker that holds place u.
 struct Shares {
-  int64_t q;
-  int rem;
-  __device__ __forceinline__ Shares(int64_t total, int workers)
-      : q(quot(total, workers)), rem((int)(total - q * workers)) {}
-  __device__ __forceinline__ int64_t first(int i) const { return i * q + min(i, rem); }
-  __device__ __forceinline__ int holder(int64_t u) const {
-    const int64_t big = rem * (q + 1);
-    if (u < big) return (int)((u >> 32) == 0 && q < 0x7fffffff ? (uint32_t)u / (uint32_t)(q + 1) : u / (q + 1));
-    return rem + (int)(((u - big) >> 32) == 0 && q < 0x7fffffff ? (uint32_t)(u - big) / (uint32_t)q : (u - big) / q);
+  int q, rem;
+  __device__ __forceinline__ Shares(int total, int workers) : q(total / workers), rem(total - q * workers) {}
+  __device__ __forceinline__ int first(int i) const { return i * q + min(i, rem); }
+  __device__ __forceinline__ int holder(int u) const {
+    const int big = rem * (q + 1);
+    return u < big ? u / (q + 1) : rem + (u - big) / q;
   }
 };
 
@@ -254,6 +247,18 @@ struct State {
   }
 };
 
+// Writes a joined head: lane i features 4 i .. 4 i + 3; top in log2 units.
+template <typename T, int D>
+__device__ __forceinline__ void write_head(const Args& a, int b, int head, int lane, const float4& o, float top,
+                                           float sum) {
+  const float inv = 1.f / sum;
+  if (lane < D / 4)
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + b * a.o_bs + (int64_t)head * a.o_hs + 4 * lane) =
+        make_uint2(pack<T>(o.x * inv, o.y * inv), pack<T>(o.z * inv, o.w * inv));
+  if (lane == 0 && a.lse)
+    a.lse[b * a.lse_bs + head] = ((top == -INFINITY ? 0.f : top) + log2f(sum)) * 0.6931471805599453f;
+}
+
 template <typename T, int D, bool I8, int NT, bool SPLIT>
 __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     kvb_paged_decode_kernel(const __grid_constant__ CUtensorMap map, const Args a) {
@@ -271,7 +276,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   uint8_t* after = smem + kWarps * NS * (G::STAGE + G::SCALES);
   int32_t* prefix = reinterpret_cast<int32_t*>(smem);                  // before the first load
   uint64_t* bars = reinterpret_cast<uint64_t*>(after);
-  // [kWarps][2] pieces: request (-1: none), item, CTAs the item spans if it begins here (or 0)
+  // [kWarps][2] pieces: request (-1: none), item, the item's first and last CTA
   int4* notes = reinterpret_cast<int4*>(bars + kWarps * NS);
   int32_t* wsum = reinterpret_cast<int32_t*>(notes + 2 * kWarps);
   const uint32_t ring_u = smem_u32(ring), scales_u = smem_u32(scales), bar_u = smem_u32(bars + warp * NS);
@@ -288,8 +293,8 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
 
   // ---- this warp's units -------------------------------------------------------------------
   int b, j, blk, nb;            // the unit to consume: request, item of the request, block
-  int64_t left;                 // units of this warp
-  int64_t u = 0, total = 0;     // split launch: the unit's place among all rows' units
+  int left;                     // what is left of this warp's share
+  int u = 0, total = 0;         // split launch: the unit's place among all rows' units
   int ctas = 1;                 // split launch: CTAs that get units
   if constexpr (SPLIT) {
     // A row weighs its blocks and kItemCost for each of its items; the weights laid end to end
@@ -312,9 +317,9 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
       return x;
     };
     auto share = [&](int rows_weight) {
-      total = (int64_t)rows_weight * a.items;
+      total = rows_weight * a.items;                // below 2^31: the host saw to it
       // no CTA without a block, so an item's CTAs are consecutive
-      ctas = (int)min((int64_t)a.ctas, quot(total + kMinUnits - 1, kMinUnits));
+      ctas = min(a.ctas, (total + kMinUnits - 1) / kMinUnits);
       if ((int)blockIdx.x < ctas) {
         const Shares sh(total, ctas * kWarps);
         u = sh.first(me);
@@ -331,14 +336,14 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
       }
       const int sum = scan(own);
       share(__shfl_sync(~0u, sum, 31));
-      const uint32_t past = __ballot_sync(~0u, (int64_t)sum * a.items > u);
+      const uint32_t past = __ballot_sync(~0u, sum * a.items > u);
       const int src = past ? __ffs(past) - 1 : 0;
       int row_b = from;                             // on lane src: its row that holds u
       before = sum - own;
       weight = w[0];
 #pragma unroll
       for (int i = 1; i < 8; ++i)
-        if (row_b == from + i - 1 && i < per && (int64_t)(before + weight) * a.items <= u) {
+        if (row_b == from + i - 1 && i < per && (before + weight) * a.items <= u) {
           ++row_b;
           before += weight;
           weight = w[i];
@@ -368,7 +373,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
         int lo = 0, hi = a.batch - 1;               // first row whose inclusive sum passes u
         while (lo < hi) {
           const int mid = (lo + hi) >> 1;
-          if ((int64_t)prefix[mid] * a.items > u) hi = mid; else lo = mid + 1;
+          if (prefix[mid] * a.items > u) hi = mid; else lo = mid + 1;
         }
         b = lo;
         before = lo ? prefix[lo - 1] : 0;
@@ -379,9 +384,9 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     }
     if (err && blockIdx.x == 0 && a.status) atomicOr(a.status, err);
     if (left > 0) {
-      const int64_t rel = u - (int64_t)before * a.items;
-      j = (int)quot(rel, weight);
-      blk = (int)(rel - (int64_t)j * weight);
+      const int rel = u - before * a.items;
+      j = rel / weight;
+      blk = rel - j * weight;
       nb = weight - kItemCost;
       if (blk >= nb) {                              // between two items: on to the next
         const int skip = weight - blk;
@@ -406,7 +411,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
 
   // ---- producer: this warp's loads, NS units ahead -------------------------------------------
   int pb = b, pj = j, pblk = blk, pnb = nb;
-  int64_t to_issue = left;
+  int to_issue = left;
   int ids = 0, cached_b = -1, cached_c = -1;        // 32 table entries, one per lane
   uint32_t issued = 0, ps = 0;                      // loads issued, the next one's stage
   int pkv = a.tiles == 1 ? pj : pj / a.tiles;       // their KV head
@@ -462,6 +467,30 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
         prefetch_l2(static_cast<const T*>(a.q) + pb * a.q_bs + h * a.q_hs + (lane & 1) * (D / 2));
     }
   };
+  // An item's query heads as the MMA's B operand: for 16-bit pools features 16 ks + 2c, + 8; for
+  // int8 pools in the order the K codes are read (lane c's 16-byte pieces c, c + 4), still in T.
+  auto load_q = [&](uint32_t (&f)[NT][KS][2], int qb, int qj) {
+    const int kv = a.tiles == 1 ? qj : qj / a.tiles, hq = kv * a.group + (qj - kv * a.tiles) * NH;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const bool on = hq + t * 8 + r < (kv + 1) * a.group;
+      const T* row = static_cast<const T*>(a.q) + qb * a.q_bs + (int64_t)(on ? hq + t * 8 + r : hq) * a.q_hs;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if constexpr (I8) {
+          const int d = 16 * (c + 4 * (ks >> 2)) + 4 * (ks & 3);
+          const uint2 x = on && d < D ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0u, 0u);
+          f[t][ks][0] = x.x;
+          f[t][ks][1] = x.y;
+        } else {
+          f[t][ks][0] = on ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 2 * c) : 0u;
+          f[t][ks][1] = on ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8 + 2 * c) : 0u;
+        }
+      }
+    }
+  };
+  uint32_t qf[NT][KS][2];
+  if (left > 0) load_q(qf, b, j);                   // ahead of the loads that will fill the memory's queues
 #pragma unroll 1
   for (int s = 0; s < NS && to_issue > 0; ++s) issue();
 
@@ -486,36 +515,13 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   }
 
   // ---- consumer ----------------------------------------------------------------------------
-  // An item's query heads as the MMA's B operand: for 16-bit pools features 16 ks + 2c, + 8; for
-  // int8 pools in the order the K codes are read (lane c's 16-byte pieces c, c + 4), still in T.
-  auto load_q = [&](uint32_t (&f)[NT][KS][2], int qb, int qj) {
-    const int kv = a.tiles == 1 ? qj : qj / a.tiles, hq = kv * a.group + (qj - kv * a.tiles) * NH;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const bool on = hq + t * 8 + r < (kv + 1) * a.group;
-      const T* row = static_cast<const T*>(a.q) + qb * a.q_bs + (int64_t)(on ? hq + t * 8 + r : hq) * a.q_hs;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        if constexpr (I8) {
-          const int d = 16 * (c + 4 * (ks >> 2)) + 4 * (ks & 3);
-          const uint2 x = on && d < D ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0u, 0u);
-          f[t][ks][0] = x.x;
-          f[t][ks][1] = x.y;
-        } else {
-          f[t][ks][0] = on ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 2 * c) : 0u;
-          f[t][ks][1] = on ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8 + 2 * c) : 0u;
-        }
-      }
-    }
-  };
   constexpr bool AHEAD = NT == 1 && !I8;                   // the next item's heads fit in registers too
   State<MT, NT> st;
-  uint32_t qf[NT][KS][2], qn[NT][KS][2];
+  uint32_t qn[NT][KS][2];
   float qx[NT][2];              // what turns S into log2 scores, per head of this lane's columns
   float qb[NT][2];              // int8: -128 * 2^-24 * sum q, the codes' bias in S
   uint32_t used = 0, cs = 0, phase = 0;             // loads consumed, the next one's stage and phase
   bool alive = true, fetched = false;
-  if (left > 0) load_q(qf, b, j);
   while (left > 0 && alive) {
     // one item, or the part of it in this warp's range
     const int kvh = a.tiles == 1 ? j : j / a.tiles;
@@ -523,7 +529,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     const int heads = min(NH, (kvh + 1) * a.group - h0);
     const int len = row_len(a, b);
     const int first = blk;
-    const int stop = (int)min((int64_t)nb, blk + left);
+    const int stop = min(nb, blk + left);
     const int past = stop == nb && SPLIT ? kItemCost : 0;
     const bool last = left <= stop - first + past;
     st.clear();
@@ -838,12 +844,13 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
           }
         }
       if (lane == 0) {
-        int span = 0;
-        if (first == 0) {
-          span = 1;
-          if constexpr (SPLIT) span = Shares(total, ctas * kWarps).holder(u + nb - 1) / kWarps - (int)blockIdx.x + 1;
+        int c0 = blockIdx.x, c1 = blockIdx.x;
+        if constexpr (SPLIT) {
+          const Shares sh(total, ctas * kWarps);
+          c0 = sh.holder(u - first) / kWarps;
+          c1 = sh.holder(u - first + nb - 1) / kWarps;
         }
-        notes[2 * warp + (last ? 1 : 0)] = make_int4(b, j, span, 0);
+        notes[2 * warp + (last ? 1 : 0)] = make_int4(b, j, c0, c1);
       }
     }
     u += n + past;
@@ -866,11 +873,12 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   const int4 note = lane < 2 * kWarps ? notes[lane] : make_int4(-1, 0, 0, 0);
   uint32_t todo = __ballot_sync(~0u, note.x >= 0);
   int task = 0;                                     // (item, head) pairs go round the warps
-  int4 own = make_int4(0, 0, 0, 0);
+  int pending = 0;                                  // this warp's heads of items that go on elsewhere
+  int4 wait_for = make_int4(0, 0, 0, 0);            // lane i: the i-th (at most two items, two heads)
   while (todo) {
     const int at = __ffs(todo) - 1;
     const int ib = __shfl_sync(~0u, note.x, at), ij = __shfl_sync(~0u, note.y, at);
-    const int span = __shfl_sync(~0u, note.z, at);
+    const int c0 = __shfl_sync(~0u, note.z, at), c1 = __shfl_sync(~0u, note.w, at);
     const bool mine = note.x == ib && note.y == ij;
     const uint32_t members = __ballot_sync(~0u, mine);
     todo &= ~members;
@@ -879,9 +887,8 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     // an item that continues from the CTA before takes the first workspace slot, one that
     // continues into the next CTA (and began here) the second
     float* part = nullptr;
-    if (SPLIT && span != 1) {                       // 1: all of it is here
-      part = a.part + ((int64_t)blockIdx.x * 2 + (span > 0 ? 1 : 0)) * G::PART;
-      if (span > 0) own = make_int4(ib, ij, span, 0);
+    if (SPLIT && c0 != c1) {
+      part = a.part + (2 * (int64_t)blockIdx.x + (c0 == (int)blockIdx.x ? 1 : 0)) * G::PART;
     }
     const float* from = (lane & 1) || !SPLIT
                             ? reinterpret_cast<const float*>(smem + (lane >> 1) * NS * G::STAGE)
@@ -892,8 +899,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
       float top = m;
 #pragma unroll
       for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-      const float base = top == -INFINITY ? 0.f : top;
-      const float w = ex2(m - base);
+      const float w = ex2(m - (top == -INFINITY ? 0.f : top));
       float sum = mine ? l * w : 0.f;
 #pragma unroll
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
@@ -918,91 +924,77 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
       }
       if (part) {
         if (lane < D / 4) *reinterpret_cast<float4*>(part + h * D + 4 * lane) = o;
-        if (lane == 0) {
-          part[NH * D + h] = top;
-          part[NH * D + NH + h] = sum;
-        }
+        if (lane == 0) *reinterpret_cast<float2*>(part + NH * D + 2 * h) = make_float2(top, sum);
+        if (lane == pending) wait_for = make_int4(ib, ij | h << 24, c0, c1);
+        ++pending;
       } else {
-        const float inv = 1.f / sum;
-        if (lane < D / 4)
-          *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + ib * a.o_bs + (int64_t)(h0 + h) * a.o_hs + 4 * lane) =
-              make_uint2(pack<T>(o.x * inv, o.y * inv), pack<T>(o.z * inv, o.w * inv));
-        if (lane == 0 && a.lse) a.lse[ib * a.lse_bs + h0 + h] = (base + log2f(sum)) * 0.6931471805599453f;
+        write_head<T, D>(a, ib, h0 + h, lane, o, top, sum);
       }
     }
   }
-  if (SPLIT && tid == 0) a.owner[blockIdx.x] = own;
-}
+  if (!SPLIT || pending == 0) return;
 
-// Joins the pieces of an item that spans CTAs: block (c, h) the item that began in CTA c, head
-// h.  Weights first, then 256 threads over (piece group, four features).
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(256) kvb_paged_join_kernel(const Args a) {
-  constexpr int NH = 8 * NT, PART = NH * D + 2 * NH, Q = D / 4, GROUPS = 256 / Q;
-  __shared__ float w[kSms], red[8], sums[GROUPS][D];
-  const int tid = threadIdx.x, h = blockIdx.y;
-  griddep_wait();
-  griddep_launch_dependents();
-  // What an item of this CTA would read is loaded before the note that says whether there is
-  // one: piece k > 0 is the first slot of CTA blockIdx.x + k.
-  const int most = a.ctas - (int)blockIdx.x;
-  const float* first = a.part + ((int64_t)blockIdx.x * 2 + 1) * PART;
-  auto at = [&](int k) { return k == 0 ? first : first + ((int64_t)2 * k - 1) * PART; };
-  const int g = tid / Q, x = tid - g * Q;
-  float m = -INFINITY, l = 0.f;
-  float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int4 own = a.owner[blockIdx.x];
-  if (tid < most) {
-    m = at(tid)[NH * D + h];
-    l = at(tid)[NH * D + NH + h];
+  // ---- items that span CTAs: whoever finds all pieces of a head there joins them ---------------
+  // A warp raises a flag for each head whose piece it wrote, passes a fence and looks at the
+  // flags of all CTAs of the item: the last to raise its flag sees all of them.  More than one
+  // may, and each then joins the same pieces into the same values.  Nobody waits.  A flag holds
+  // this call's nonce, so the workspace needs no clearing; whoever joins takes the flags back,
+  // so a replayed graph starts afresh.
+  asm volatile("fence.acq_rel.gpu;" ::: "memory");
+  __syncwarp();
+  if (lane < pending) {
+    const int64_t at = (2 * (int)blockIdx.x + (wait_for.z == (int)blockIdx.x ? 1 : 0)) * NH + (wait_for.y >> 24);
+    asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(a.flags + at), "l"(a.nonce) : "memory");
   }
-  if (g < min(GROUPS, most)) v0 = *reinterpret_cast<const float4*>(at(g) + h * D + 4 * x);
-  const int span = min(own.z, most);
-  const int kvh = own.y / a.tiles, h0 = kvh * a.group + (own.y - kvh * a.tiles) * NH;
-  if (span <= 0 || h >= (kvh + 1) * a.group - h0) return;
-  if (tid >= span) {
-    m = -INFINITY;
-    l = 0.f;
-  }
-  float top = m;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-  if ((tid & 31) == 0) red[tid >> 5] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i]);
-  const float base = top == -INFINITY ? 0.f : top;
-  const float f = ex2(m - base);
-  if (tid < span) w[tid] = f;
-  float total = tid < span ? l * f : 0.f;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
-  __syncthreads();
-  if ((tid & 31) == 0) red[tid >> 5] = total;
-  __syncthreads();
-  total = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) total += red[i];
-  if (g < GROUPS) {
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (g < span) acc = make_float4(w[g] * v0.x, w[g] * v0.y, w[g] * v0.z, w[g] * v0.w);
-#pragma unroll 4
-    for (int k = g + GROUPS; k < span; k += GROUPS) {
-      const float4 v = *reinterpret_cast<const float4*>(at(k) + h * D + 4 * x);
-      acc.x += w[k] * v.x;
-      acc.y += w[k] * v.y;
-      acc.z += w[k] * v.z;
-      acc.w += w[k] * v.w;
+  __syncwarp();
+  asm volatile("fence.sc.gpu;" ::: "memory");
+  for (int i = 0; i < pending; ++i) {
+    const int ib = __shfl_sync(~0u, wait_for.x, i), jh = __shfl_sync(~0u, wait_for.y, i);
+    const int c0 = __shfl_sync(~0u, wait_for.z, i), c1 = __shfl_sync(~0u, wait_for.w, i);
+    const int ij = jh & 0xffffff, h = jh >> 24, n = c1 - c0 + 1;
+    bool all = true;
+    for (int k = c0 + lane; k <= c1; k += 32) {
+      uint64_t f;
+      asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];"
+                   : "=l"(f) : "l"(a.flags + (2 * k + (k == c0 ? 1 : 0)) * NH + h) : "memory");
+      all &= f == a.nonce;
     }
-    *reinterpret_cast<float4*>(&sums[g][4 * x]) = acc;
-  }
-  __syncthreads();
-  if (tid < D) {
-    float o = 0.f;
+    if (!__all_sync(~0u, all)) continue;
+    asm volatile("fence.acq_rel.gpu;" ::: "memory");
+    // pieces c0 .. c1, twelve at a time in flight
+    const float* head = a.part + (2 * (int64_t)c0 + 1) * G::PART;       // piece k > 0: (2 k - 1) further
+    auto piece = [&](int k) { return k == 0 ? head : head + (2 * (int64_t)k - 1) * G::PART; };
+    float top = -INFINITY, sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int k0 = 0; k0 < n; k0 += 12) {
+      const bool on = lane < 12 && k0 + lane < n;
+      const float2 ml = on ? __ldcg(reinterpret_cast<const float2*>(piece(k0 + lane) + NH * D + 2 * h))
+                           : make_float2(-INFINITY, 0.f);
+      float4 v[12];
 #pragma unroll
-    for (int i = 0; i < GROUPS; ++i) o += sums[i][tid];
-    static_cast<T*>(a.o)[own.x * a.o_bs + (int64_t)(h0 + h) * a.o_hs + tid] = T(o / total);
-    if (tid == 0 && a.lse) a.lse[own.x * a.lse_bs + h0 + h] = (base + log2f(total)) * 0.6931471805599453f;
+      for (int k = 0; k < 12; ++k)
+        v[k] = k0 + k < n && lane < D / 4 ? __ldcg(reinterpret_cast<const float4*>(piece(k0 + k) + h * D) + lane)
+                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+      float up = fmaxf(top, ml.x);
+#pragma unroll
+      for (int x = 8; x; x >>= 1) up = fmaxf(up, __shfl_xor_sync(~0u, up, x));
+      up = __shfl_sync(~0u, up, 0);
+      const float zero = up == -INFINITY ? 0.f : up, keep = ex2(top - zero), w = ex2(ml.x - zero);
+      top = up;
+      sum = sum * keep + (on ? ml.y * w : 0.f);                         // lane 0 .. 11: shares of the sum
+      o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
+#pragma unroll
+      for (int k = 0; k < 12; ++k) {
+        const float f = __shfl_sync(~0u, w, k);
+        if (k0 + k < n) o.x += f * v[k].x, o.y += f * v[k].y, o.z += f * v[k].z, o.w += f * v[k].w;
+      }
+    }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
+    for (int k = c0 + lane; k <= c1; k += 32) a.flags[(2 * k + (k == c0 ? 1 : 0)) * NH + h] = 0;
+    const int kvh = ij / a.tiles;
+    write_head<T, D>(a, ib, kvh * a.group + (ij - kvh * a.tiles) * NH + h, lane, o, top, sum);
   }
 }
 
@@ -1020,18 +1012,20 @@ bool split(const KvbPagedDecodeParams* p) {
   const int64_t width = p->max_seq_len > 0
                             ? std::min<int64_t>(p->max_blocks_per_seq, ((int64_t)p->max_seq_len + 15) / 16)
                             : p->max_blocks_per_seq;
+  // 32-bit places: wider than any pool
+  if ((int64_t)p->batch * (p->max_blocks_per_seq + kItemCost) * p->num_q_heads > 0x7fffffff) return false;
   return width > kItemBlocks;
 }
 
-// Workspace of a split launch: joined pieces, warps' first pieces, owners.
+// Workspace of a split launch: CTAs' pieces, warps' first pieces, flags.
 struct Room {
-  int64_t part, first, owner, bytes;
+  int64_t part, first, flags, bytes;
   explicit Room(const KvbPagedDecodeParams* p) {
     const int64_t nh = 8 * head_tiles(p);
     part = 0;
     first = part + 4 * kSms * 2 * (nh * p->head_dim + 2 * nh);
-    owner = first + 4 * kSms * std::max(8, kWarpsI8) * (nh * (p->head_dim + 4) + 2 * nh);
-    bytes = owner + kSms * (int64_t)sizeof(int4);
+    flags = first + 4 * kSms * std::max(8, kWarpsI8) * (nh * (p->head_dim + 4) + 2 * nh);
+    bytes = flags + kSms * 2 * nh * (int64_t)sizeof(uint64_t);
   }
 };
 
@@ -1136,9 +1130,7 @@ cudaError_t launch(const CUtensorMap& map, const Args& a, bool is_split, cudaStr
     if (e != cudaSuccess) return e;
     ready[is_split].fetch_or(bit, std::memory_order_release);
   }
-  e = launch_pdl(kern, dim3(is_split ? a.ctas : a.batch * a.items), G::THREADS, G::SMEM, s, map, a);
-  if (e != cudaSuccess || !is_split || a.ctas == 1) return e;
-  return launch_pdl(kvb_paged_join_kernel<T, D, NT>, dim3(a.ctas, std::min(a.group, 8 * NT)), 256, 0, s, a);
+  return launch_pdl(kern, dim3(is_split ? a.ctas : a.batch * a.items), G::THREADS, G::SMEM, s, map, a);
 }
 
 template <typename T, bool I8, int NT>
@@ -1211,7 +1203,10 @@ extern "C" int kvb_paged_decode_fwd(const KvbPagedDecodeParams* p, void* stream)
     uint8_t* w = static_cast<uint8_t*>(p->workspace);
     a.part = reinterpret_cast<float*>(w + room.part);
     a.first = reinterpret_cast<float*>(w + room.first);
-    a.owner = reinterpret_cast<int4*>(w + room.owner);
+    a.flags = reinterpret_cast<uint64_t*>(w + room.flags);
+    // a different odd number for every call of the process (the odd factor permutes 2^64)
+    static std::atomic<uint64_t> calls{0};
+    a.nonce = (2 * calls.fetch_add(1, std::memory_order_relaxed) + 1) * 0x9e3779b97f4a7c15ull;
   }
   CUtensorMap map;
   std::string err;
