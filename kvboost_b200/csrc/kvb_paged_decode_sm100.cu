@@ -247,6 +247,14 @@ struct State {
   }
 };
 
+// The largest of the warp's values: a float's bits, the negative ones' turned over, order as
+// integers.
+__device__ __forceinline__ float warp_max(float x) {
+  const int i = __float_as_int(x);
+  const int top = __reduce_max_sync(~0u, i < 0 ? i ^ 0x7fffffff : i);
+  return __int_as_float(top < 0 ? top ^ 0x7fffffff : top);
+}
+
 // Writes a joined head: lane i features 4 i .. 4 i + 3; top in log2 units.
 template <typename T, int D>
 __device__ __forceinline__ void write_head(const Args& a, int b, int head, int lane, const float4& o, float top,
@@ -304,9 +312,9 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     const int me = blockIdx.x * kWarps + warp;
     int before = 0, weight = 0, err = 0;
     auto row = [&](int i) {
-      const int n = (row_len(a, i) + 15) >> 4;
-      if ((int64_t)a.lens[i] > (int64_t)a.width * 16) err = KVB_STATUS_BAD_LENGTH;
-      return n ? n + kItemCost : 0;
+      const int len = max(a.lens[i], 0), n = (len >> 4) + ((len & 15) != 0);
+      if (n > a.width) err = KVB_STATUS_BAD_LENGTH;
+      return n ? min(n, a.width) + kItemCost : 0;
     };
     auto scan = [&](int x) {
 #pragma unroll
@@ -326,7 +334,14 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
         left = sh.first(me + 1) - u;
       }
     };
-    if (a.batch <= 256) {                           // every warp for itself, 8 rows a lane
+    if (a.batch <= 32) {                            // every warp for itself, a row a lane
+      const int w = lane < a.batch ? row(lane) : 0, sum = scan(w);
+      share(__shfl_sync(~0u, sum, 31));
+      const uint32_t past = __ballot_sync(~0u, sum * a.items > u);
+      b = past ? __ffs(past) - 1 : 0;
+      weight = __shfl_sync(~0u, w, b);
+      before = __shfl_sync(~0u, sum, b) - weight;
+    } else if (a.batch <= 256) {                    // 8 rows a lane
       int w[8], own = 0;
       const int per = (a.batch + 31) >> 5, from = lane * per;
 #pragma unroll
@@ -872,7 +887,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   // ---- the CTA's pieces, joined item by item: a warp per head, a lane per four features ---------
   const int4 note = lane < 2 * kWarps ? notes[lane] : make_int4(-1, 0, 0, 0);
   uint32_t todo = __ballot_sync(~0u, note.x >= 0);
-  int task = 0;                                     // (item, head) pairs go round the warps
+  int turn = 0;                                     // (item, head) pairs go round the warps
   int pending = 0;                                  // this warp's heads of items that go on elsewhere
   int4 wait_for = make_int4(0, 0, 0, 0);            // lane i: the i-th (at most two items, two heads)
   while (todo) {
@@ -882,46 +897,53 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     const bool mine = note.x == ib && note.y == ij;
     const uint32_t members = __ballot_sync(~0u, mine);
     todo &= ~members;
-    const int kvh = ij / a.tiles, h0 = kvh * a.group + (ij - kvh * a.tiles) * NH;
+    const int kvh = a.tiles == 1 ? ij : ij / a.tiles, h0 = kvh * a.group + (ij - kvh * a.tiles) * NH;
     const int heads = min(NH, (kvh + 1) * a.group - h0);
     // an item that continues from the CTA before takes the first workspace slot, one that
     // continues into the next CTA (and began here) the second
     float* part = nullptr;
-    if (SPLIT && c0 != c1) {
+    if (SPLIT && c0 != c1)
       part = a.part + (2 * (int64_t)blockIdx.x + (c0 == (int)blockIdx.x ? 1 : 0)) * G::PART;
-    }
-    const float* from = (lane & 1) || !SPLIT
-                            ? reinterpret_cast<const float*>(smem + (lane >> 1) * NS * G::STAGE)
-                            : a.first + ((int64_t)blockIdx.x * kWarps + (lane >> 1)) * G::PIECE;
-    for (int h = 0; h < heads; ++h) {
-      if (task++ % kWarps != warp) continue;
-      const float m = mine ? from[NH * G::OS + h] : -INFINITY, l = mine ? from[NH * G::OS + NH + h] : 0.f;
-      float top = m;
+    const int begin = warp >= turn ? warp - turn : warp - turn + kWarps;
+    turn = (turn + heads) % kWarps;
+    for (int h = begin; h < heads; h += kWarps) {
+      // this lane's piece (lane 2 w + 1: warp w's last, over its stages; 2 w: its first, in the
+      // workspace), and every last piece's four features, members or not
+      float4 v[kWarps];
 #pragma unroll
-      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-      const float w = ex2(m - (top == -INFINITY ? 0.f : top));
-      float sum = mine ? l * w : 0.f;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      #pragma unroll 1
-      for (int k0 = 0; k0 < 2 * kWarps; k0 += 4) {
-        if (!((members >> k0) & 15)) continue;
-#pragma unroll
-        for (int k = k0; k < k0 + 4; ++k) {
-          const float f = __shfl_sync(~0u, w, k);
-          const float* p = (k & 1) || !SPLIT
-                               ? reinterpret_cast<const float*>(smem + (k >> 1) * NS * G::STAGE)
-                               : a.first + ((int64_t)blockIdx.x * kWarps + (k >> 1)) * G::PIECE;
-          if (((members >> k) & 1) && lane < D / 4) {
-            const float4 v = *reinterpret_cast<const float4*>(p + h * G::OS + 4 * lane);
-            o.x += f * v.x;
-            o.y += f * v.y;
-            o.z += f * v.z;
-            o.w += f * v.w;
-          }
+      for (int k = 0; k < kWarps; ++k)
+        v[k] = *reinterpret_cast<const float4*>(smem + k * NS * G::STAGE + (h * G::OS + 4 * (lane % (D / 4))) * 4);
+      float m = -INFINITY, l = 0.f;
+      if (mine) {
+        if ((lane & 1) || !SPLIT) {
+          const float* p = reinterpret_cast<const float*>(smem + (lane >> 1) * NS * G::STAGE) + NH * G::OS + h;
+          m = p[0];
+          l = p[NH];
+        } else {
+          const float* p = a.first + ((int64_t)blockIdx.x * kWarps + (lane >> 1)) * G::PIECE + NH * G::OS + h;
+          m = p[0];
+          l = p[NH];
         }
       }
+      const float top = warp_max(m), w = ex2(m - (top == -INFINITY ? 0.f : top));
+      float sum = mine ? l * w : 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float f = __shfl_sync(~0u, w, 2 * k + 1);
+        if ((members >> (2 * k + 1)) & 1) o.x += f * v[k].x, o.y += f * v[k].y, o.z += f * v[k].z, o.w += f * v[k].w;
+      }
+      if constexpr (SPLIT) {
+        for (uint32_t firsts = members & 0x55555555u; firsts; firsts &= firsts - 1) {
+          const int k = __ffs(firsts) - 1;
+          const float f = __shfl_sync(~0u, w, k);
+          const float4 x = *reinterpret_cast<const float4*>(
+              a.first + ((int64_t)blockIdx.x * kWarps + (k >> 1)) * G::PIECE + h * G::OS + 4 * (lane % (D / 4)));
+          o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
+        }
+      }
+#pragma unroll
+      for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
       if (part) {
         if (lane < D / 4) *reinterpret_cast<float4*>(part + h * D + 4 * lane) = o;
         if (lane == 0) *reinterpret_cast<float2*>(part + NH * D + 2 * h) = make_float2(top, sum);
@@ -961,39 +983,36 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     }
     if (!__all_sync(~0u, all)) continue;
     asm volatile("fence.acq_rel.gpu;" ::: "memory");
-    // pieces c0 .. c1, twelve at a time in flight
-    const float* head = a.part + (2 * (int64_t)c0 + 1) * G::PART;       // piece k > 0: (2 k - 1) further
-    auto piece = [&](int k) { return k == 0 ? head : head + (2 * (int64_t)k - 1) * G::PART; };
+    // pieces c0 .. c1, eight at a time in flight; a first one is CTA c0's second slot, the others
+    // the first slots of the CTAs after it
+    const float* part = a.part + 2 * (int64_t)c0 * G::PART;
+    auto piece = [&](int k) { return part + (k == 0 ? 1 : 2 * k) * G::PART; };
+    const int x4 = h * D + 4 * (lane % (D / 4));
     float top = -INFINITY, sum = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-    for (int k0 = 0; k0 < n; k0 += 12) {
-      const bool on = lane < 12 && k0 + lane < n;
-      const float2 ml = on ? __ldcg(reinterpret_cast<const float2*>(piece(k0 + lane) + NH * D + 2 * h))
-                           : make_float2(-INFINITY, 0.f);
-      float4 v[12];
+    for (int k0 = 0; k0 < n; k0 += 8) {
+      const int mine = min(k0 + (lane & 7), n - 1);
+      float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(mine) + NH * D + 2 * h));
+      float4 v[8];
 #pragma unroll
-      for (int k = 0; k < 12; ++k)
-        v[k] = k0 + k < n && lane < D / 4 ? __ldcg(reinterpret_cast<const float4*>(piece(k0 + k) + h * D) + lane)
-                                          : make_float4(0.f, 0.f, 0.f, 0.f);
-      float up = fmaxf(top, ml.x);
-#pragma unroll
-      for (int x = 8; x; x >>= 1) up = fmaxf(up, __shfl_xor_sync(~0u, up, x));
-      up = __shfl_sync(~0u, up, 0);
-      const float zero = up == -INFINITY ? 0.f : up, keep = ex2(top - zero), w = ex2(ml.x - zero);
+      for (int k = 0; k < 8; ++k) v[k] = __ldcg(reinterpret_cast<const float4*>(piece(min(k0 + k, n - 1)) + x4));
+      const float up = fmaxf(top, warp_max(ml.x)), zero = up == -INFINITY ? 0.f : up;
+      const float keep = ex2(top - zero), w = ex2(ml.x - zero);
       top = up;
-      sum = sum * keep + (on ? ml.y * w : 0.f);                         // lane 0 .. 11: shares of the sum
+      sum = sum * keep + (lane < 8 && k0 + lane < n ? ml.y * w : 0.f);  // lanes 0 .. 7: shares of the sum
       o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
 #pragma unroll
-      for (int k = 0; k < 12; ++k) {
+      for (int k = 0; k < 8; ++k) {
         const float f = __shfl_sync(~0u, w, k);
         if (k0 + k < n) o.x += f * v[k].x, o.y += f * v[k].y, o.z += f * v[k].z, o.w += f * v[k].w;
       }
     }
 #pragma unroll
-    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
+    for (int x = 4; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
+    sum = __shfl_sync(~0u, sum, 0);
     for (int k = c0 + lane; k <= c1; k += 32) a.flags[(2 * k + (k == c0 ? 1 : 0)) * NH + h] = 0;
-    const int kvh = ij / a.tiles;
+    const int kvh = a.tiles == 1 ? ij : ij / a.tiles;
     write_head<T, D>(a, ib, kvh * a.group + (ij - kvh * a.tiles) * NH + h, lane, o, top, sum);
   }
 }
