@@ -516,8 +516,8 @@ typedef struct KvbExtendTablesParams {
   const int32_t* new_lens;       /* device [batch] */
   const int32_t* free_blocks;    /* device [free_capacity] */
   const int32_t* num_free;       /* device [1] */
-  int32_t* slots;                /* device [max_new_tokens], written */
-  int64_t* positions;            /* device [max_new_tokens], written */
+  int32_t* slots;                /* device [max_new_tokens], written; 16-byte aligned */
+  int64_t* positions;            /* device [max_new_tokens], written; 16-byte aligned */
   int32_t* cu_new;               /* device [batch + 1], written */
   int32_t* seq_lens_out;         /* device [batch], written */
   int32_t* num_free_out;         /* device [1], written */

@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <string>
 
@@ -50,19 +51,38 @@ struct TablesArgs {
   int32_t* status;
 };
 
-// One CTA: a scan over the rows gives each row's place in the packed arrays and in the
-// free list, then one thread per token writes its slot, its position and, for the first
-// token of a new block, the table entry.
+// Sums that stop at 2^31 - 1: exact where they are compared with something below.
+__device__ __forceinline__ uint32_t add_sat(uint32_t x, uint32_t y) { return min(x + y, 0x7fffffffu); }
+
+__device__ __forceinline__ uint2 scan_sat(uint2 x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t p = __shfl_up_sync(~0u, x.x, o), q = __shfl_up_sync(~0u, x.y, o);
+    if (lane >= o) x = make_uint2(add_sat(x.x, p), add_sat(x.y, q));
+  }
+  return x;
+}
+
+// A scan over the rows gives each row's place in the packed arrays and in the free list (one
+// scan for both: a row that does not fit in the packed arrays is followed only by rows that
+// do not either, or that need nothing).  Then a thread takes four consecutive tokens: one
+// search for the row of the first, slots and positions in 16-byte stores, and the table entry
+// of each block that a token begins.
+// Latency is all there is: two dependent reads, a scan and the stores.  One cluster of up to
+// eight CTAs shares the tokens; every CTA scans for itself, and since the new lengths may go
+// over the old ones, no CTA writes before all have read.
 __global__ void __launch_bounds__(1024) kvb_extend_tables_kernel(const TablesArgs a) {
   extern __shared__ int32_t sm[];
   int32_t* cu = sm;                        // [batch + 1] place of the row's tokens
   int32_t* start = cu + a.batch + 1;       // [batch] pops before the row's, -1: does not fit
   int32_t* len = start + a.batch;          // [batch]
-  __shared__ int64_t wsum[2][32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nt = blockDim.x;
+  __shared__ uint2 wsum[32];
+  __shared__ int taken;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nt = blockDim.x, warps = nt >> 5;
   const int nfree = min(max(*a.num_free, 0), a.capacity);
-  int64_t base_tok = 0, base_need = 0;
+  uint2 base = make_uint2(0, 0);
   int err = 0;
+  if (tid == 0) cu[0] = taken = 0;
   for (int b0 = 0; b0 < a.batch; b0 += nt) {
     const int b = b0 + tid;
     int l = 0, n = 0;
@@ -71,113 +91,112 @@ __global__ void __launch_bounds__(1024) kvb_extend_tables_kernel(const TablesArg
       l = a.seq_lens[b];
       n = a.new_lens[b];
       ok = l >= 0 && n >= 0 && n <= a.max_tokens;
-      if (!ok) {
-        err |= KVB_STATUS_BAD_LENGTH;
-        n = 0;
-      }
+      if (!ok) n = 0;
+      ok = ok && (int64_t)l + n <= (int64_t)a.width * 16;
+      if (!ok) err |= KVB_STATUS_BAD_LENGTH;
     }
-    const bool wide = ok && (int64_t)l + n <= (int64_t)a.width * 16;
-    if (ok && !wide) err |= KVB_STATUS_BAD_LENGTH;
-    const int64_t end0 = n;
-    int64_t need = wide ? ((int64_t)l + n + 15) / 16 - ((int64_t)l + 15) / 16 : 0;
-    // inclusive scans of tokens and needs over the CTA
-    int64_t t_in = end0;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(~0u, t_in, o);
-      if (lane >= o) t_in += x;
-    }
-    if (lane == 31) wsum[0][warp] = t_in;
+    const int need = ok ? (l + n + 15) / 16 - (l + 15) / 16 : 0;
+    uint2 x = scan_sat(make_uint2(n, need), lane);
+    if (lane == 31) wsum[warp] = x;
     __syncthreads();
-    int64_t tot_tok = 0;
-    for (int w = 0; w < (nt >> 5); ++w) {
-      if (w < warp) t_in += wsum[0][w];
-      tot_tok += wsum[0][w];
-    }
-    const int64_t tok_end = base_tok + t_in;
-    const bool packed = wide && (n == 0 || tok_end <= a.max_tokens);
-    if (wide && !packed) {
-      err |= KVB_STATUS_BAD_LENGTH;
-      need = 0;
-    }
-    int64_t n_in = need;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(~0u, n_in, o);
-      if (lane >= o) n_in += x;
-    }
-    if (lane == 31) wsum[1][warp] = n_in;
-    __syncthreads();
-    int64_t tot_need = 0;
-    for (int w = 0; w < (nt >> 5); ++w) {
-      if (w < warp) n_in += wsum[1][w];
-      tot_need += wsum[1][w];
-    }
-    const int64_t need_end = base_need + n_in;
-    const bool fits = packed && (need == 0 || need_end <= nfree);
+    const uint2 w = scan_sat(lane < warps ? wsum[lane] : make_uint2(0, 0), lane);
+    const uint32_t before_t = __shfl_sync(~0u, w.x, max(warp - 1, 0));
+    const uint32_t before_n = __shfl_sync(~0u, w.y, max(warp - 1, 0));
+    if (warp > 0) x = make_uint2(add_sat(x.x, before_t), add_sat(x.y, before_n));
+    x = make_uint2(add_sat(x.x, base.x), add_sat(x.y, base.y));
+    base = make_uint2(add_sat(base.x, __shfl_sync(~0u, w.x, 31)), add_sat(base.y, __shfl_sync(~0u, w.y, 31)));
+    const bool packed = ok && (n == 0 || x.x <= (uint32_t)a.max_tokens);
+    const bool fits = packed && (need == 0 || x.y <= (uint32_t)nfree);
+    if (ok && !packed) err |= KVB_STATUS_BAD_LENGTH;
     if (packed && !fits) err |= KVB_STATUS_POOL_EMPTY;
     if (b < a.batch) {
-      cu[b + 1] = (int32_t)min(tok_end, (int64_t)a.max_tokens);
-      start[b] = fits ? (int32_t)(need_end - need) : -1;
+      cu[b + 1] = (int)min(x.x, (uint32_t)a.max_tokens);
+      start[b] = fits ? (int)x.y - need : -1;
       len[b] = l;
     }
-    base_tok += tot_tok;
-    base_need += tot_need;
+    // rows that fit and need blocks come before all others that need some: the last one's end
+    const int end = __reduce_max_sync(~0u, fits && need ? (int)x.y : 0);
+    if (lane == 0 && end) atomicMax(&taken, end);
     __syncthreads();
   }
-  if (tid == 0) cu[0] = 0;
-  __syncthreads();
-  // every read of seq_lens and num_free is done: the outputs may alias them
-  if (tid == 0) a.cu_new[0] = 0;
-  int taken = 0;
-  for (int b = tid; b < a.batch; b += nt) {
-    const int n = cu[b + 1] - cu[b], l = len[b];
-    a.cu_new[b + 1] = cu[b + 1];
-    a.seq_lens_out[b] = start[b] >= 0 ? l + n : l;
-    if (start[b] >= 0) taken += (l + n + 15) / 16 - (l + 15) / 16;
+  if (gridDim.x > 1) {                     // every CTA has read the lengths and the free list's
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
-  for (int o = 16; o; o >>= 1) taken += __shfl_xor_sync(~0u, taken, o);
-  if (lane == 0) wsum[0][warp] = taken;
-  __syncthreads();
-  if (tid == 0) {
-    int64_t t = 0;
-    for (int w = 0; w < (nt >> 5); ++w) t += wsum[0][w];
-    *a.num_free_out = nfree - (int)t;
+  if (blockIdx.x == 0) {
+    for (int b = tid; b < a.batch; b += nt) {
+      a.cu_new[b + 1] = cu[b + 1];
+      a.seq_lens_out[b] = start[b] >= 0 ? len[b] + cu[b + 1] - cu[b] : len[b];
+    }
+    if (tid == 0) {
+      a.cu_new[0] = 0;
+      *a.num_free_out = nfree - taken;
+    }
   }
-  const int total = cu[a.batch];
-  for (int t = tid; t < a.max_tokens; t += nt) {
-    int slot = -1;
-    int64_t pos = 0;
-    if (t < total) {
-      int lo = 0, hi = a.batch - 1;   // the row with cu[row] <= t < cu[row + 1]
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (cu[mid + 1] <= t) lo = mid + 1; else hi = mid;
-      }
-      const int s = start[lo];
-      if (s >= 0) {
-        const int l = len[lo], p = l + t - cu[lo], have = (l + 15) >> 4, blk = p >> 4;
-        int32_t* row = a.tables + (int64_t)lo * a.stride;
-        int id;
-        if (blk < have) {
-          id = row[blk];
-        } else {
-          id = a.free_blocks[nfree - 1 - s - (blk - have)];
-          if ((p & 15) == 0) row[blk] = id;
-        }
-        pos = p;
-        if (id >= 0 && id < a.num_blocks) slot = id * 16 + (p & 15);
-        else err |= KVB_STATUS_BAD_BLOCK;
+  const int total = cu[a.batch], step = gridDim.x * nt * 4;
+  for (int t0 = (blockIdx.x * nt + tid) * 4; t0 < a.max_tokens; t0 += step) {
+    int row = 0;
+    if (t0 < total) {                      // the row with cu[row] <= t0 < cu[row + 1]
+      int hi = a.batch - 1;
+      while (row < hi) {
+        const int mid = (row + hi) >> 1;
+        if (cu[mid + 1] <= t0) row = mid + 1; else hi = mid;
       }
     }
-    a.slots[t] = slot;
-    a.positions[t] = pos;
+    int slot[4];
+    int64_t pos[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = t0 + i;
+      slot[i] = -1;
+      pos[i] = 0;
+      if (t >= total) continue;
+      while (cu[row + 1] <= t) ++row;
+      const int s = start[row];
+      if (s < 0) continue;
+      const int l = len[row], p = l + t - cu[row], have = (l + 15) >> 4, blk = p >> 4;
+      int32_t* table = a.tables + (int64_t)row * a.stride;
+      int id;
+      if (blk < have) {
+        id = table[blk];
+      } else {
+        id = a.free_blocks[nfree - 1 - s - (blk - have)];
+        if ((p & 15) == 0) table[blk] = id;
+      }
+      pos[i] = p;
+      if (id >= 0 && id < a.num_blocks) slot[i] = id * 16 + (p & 15);
+      else err |= KVB_STATUS_BAD_BLOCK;
+    }
+    if (t0 + 4 <= a.max_tokens) {
+      *reinterpret_cast<int4*>(a.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      *reinterpret_cast<longlong2*>(a.positions + t0) = make_longlong2(pos[0], pos[1]);
+      *reinterpret_cast<longlong2*>(a.positions + t0 + 2) = make_longlong2(pos[2], pos[3]);
+    } else {
+      for (int i = 0; i < 4 && t0 + i < a.max_tokens; ++i) {
+        a.slots[t0 + i] = slot[i];
+        a.positions[t0 + i] = pos[i];
+      }
+    }
   }
   if (err && a.status) atomicOr(a.status, err);
 }
 
 // ---- append ---------------------------------------------------------------------------------
 
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery's round-up method).
+struct Div {
+  uint32_t d, mul, shift;
+  explicit Div(uint32_t by) : d(by), shift(0) {
+    while ((1ull << shift) < by) ++shift;
+    mul = (uint32_t)(((((uint64_t)1 << shift) - by) << 32) / by + 1);
+  }
+  __device__ __forceinline__ uint32_t quot(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
 struct AppendArgs {
-  int vecs, heads, tokens, num_blocks;   // vecs: 16-byte pieces of a head's vector
+  Div per, vecs;                             // 16-byte pieces of a token, of a head's vector
+  uint32_t pieces;                           // of all tokens
+  int heads, num_blocks;
   const uint4* src[2];
   int64_t token_stride[2], head_stride[2];   // in 16-byte pieces
   uint4* pool;
@@ -185,27 +204,39 @@ struct AppendArgs {
   int32_t* status;
 };
 
-// One thread per 16-byte piece; blockIdx.y picks K or V.
+// A thread moves U 16-byte pieces, all read before the first is written; blockIdx.y picks K or
+// V.  Byte work: with one piece a thread the 8192-token prefill of 8 heads ran at 2.3 TB/s,
+// waiting on each piece's slot before its store; with four in flight the loads cover the
+// slots' latency.  Small appends keep one piece a thread, to spread over the SMs.
+template <int U>
 __global__ void __launch_bounds__(256) kvb_append_paged_kernel(const AppendArgs a) {
   const int kv = blockIdx.y;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int per = a.heads * a.vecs;
-  const int64_t t = i / per;
-  if (t >= a.tokens) return;
-  const int r = (int)(i - t * per), h = r / a.vecs, x = r - h * a.vecs;
-  const int slot = a.slots[t];
-  if (slot < 0 || slot >= (int64_t)a.num_blocks * 16) {
-    if (slot != -1 && r == 0 && kv == 0 && a.status) atomicOr(a.status, KVB_STATUS_BAD_BLOCK);
-    return;
+  const uint32_t first = blockIdx.x * (256 * U) + threadIdx.x;
+  uint4 data[U];
+  int64_t dst[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t i = first + u * 256;
+    dst[u] = -1;
+    if (i < a.pieces) {
+      const uint32_t t = a.per.quot(i), r = i - t * a.per.d, h = a.vecs.quot(r), x = r - h * a.vecs.d;
+      data[u] = __ldcs(a.src[kv] + t * a.token_stride[kv] + h * a.head_stride[kv] + x);
+      const int slot = a.slots[t];
+      if (slot >= 0 && slot < (int64_t)a.num_blocks * 16)
+        dst[u] = ((((int64_t)(slot >> 4) * 2 + kv) * a.heads + h) * 16 + (slot & 15)) * a.vecs.d + x;
+      else if (slot != -1 && r == 0 && kv == 0 && a.status)
+        atomicOr(a.status, KVB_STATUS_BAD_BLOCK);
+    }
   }
-  const int64_t row = (((int64_t)(slot >> 4) * 2 + kv) * a.heads + h) * 16 + (slot & 15);
-  a.pool[row * a.vecs + x] = a.src[kv][t * a.token_stride[kv] + h * a.head_stride[kv] + x];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (dst[u] >= 0) a.pool[dst[u]] = data[u];
 }
 
 // ---- logits -----------------------------------------------------------------------------------
 
 struct LogitsArgs {
-  int vocab, history_len, num_bias, slice;
+  int vocab, history_len, num_bias;
   const void* logits;
   void* out;
   int64_t logits_stride, out_stride, history_stride, mask_stride;
@@ -228,64 +259,143 @@ __device__ __forceinline__ void from_f32(float* p, float x) { *p = x; }
 __device__ __forceinline__ void from_f32(__half* p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void from_f32(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-constexpr uint32_t kHasBias = 1u << 31;   // a seen word: bit 0 seen, bits 1..30 count, bit 31
+// Eight consecutive values, 16 bytes at a time.
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+  T h[8];
+  memcpy(h, &v, 16);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = to_f32(h[i]);
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  __stcs(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3]));
+  __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(x[4], x[5], x[6], x[7]));
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  T h[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) from_f32(h + i, x[i]);
+  uint4 v;
+  memcpy(&v, h, 16);
+  __stcs(reinterpret_cast<uint4*>(p), v);
+}
 
-// A CTA takes one slice of one row: it notes the history's tokens that fall into the slice
-// in shared memory (seen bit and count, integer adds: any order gives the same), then
-// streams the slice.
-template <typename TI, typename TO>
+constexpr uint32_t kHasBias = 1u << 31;   // a note: bit 0 seen, bits 1..30 count, bit 31 biased
+
+// A CTA takes one slice of a row, 8 ITER tokens a thread: it notes the history's tokens that
+// fall into the slice in shared memory (seen bit and count, integer adds: any order gives the
+// same), then streams the slice 16 bytes at a time.  Byte work for large batches (the logits
+// once, the float32 result once; the history is read by every slice's CTA, from L2); the
+// logits are on their way while the history is read.  A row whose pointers or tail do not sit
+// on 16 bytes goes value by value.  The quotient by the temperature is a product with its
+// reciprocal: one more rounding of float32.
+template <typename TI, typename TO, int ITER>
 __global__ void __launch_bounds__(256) kvb_logits_kernel(const LogitsArgs a) {
-  extern __shared__ uint32_t note[];
+  constexpr int kSlice = 256 * 8 * ITER;
+  __shared__ __align__(16) uint32_t note[kSlice];
   const int b = blockIdx.y, tid = threadIdx.x;
-  const int v0 = blockIdx.x * a.slice, v1 = min(a.vocab, v0 + a.slice);
+  const int v0 = blockIdx.x * kSlice, v1 = min(a.vocab, v0 + kSlice);
+  const TI* in = static_cast<const TI*>(a.logits) + b * a.logits_stride;
+  TO* out = static_cast<TO*>(a.out) + b * a.out_stride;
+  const uint8_t* mask = a.mask ? reinterpret_cast<const uint8_t*>(a.mask + b * a.mask_stride) : nullptr;
+  const bool wide = ((reinterpret_cast<uintptr_t>(in + v0) | reinterpret_cast<uintptr_t>(out + v0)) & 15) == 0;
+  float x[ITER][8];
+  uint32_t open[ITER];
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const int v = v0 + (i * 256 + tid) * 8;
+    open[i] = 0xff;
+    if (wide && v + 8 <= v1) load8(in + v, x[i]);
+    else
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[i][k] = v + k < v1 ? to_f32(in[v + k]) : 0.f;
+    if (mask && v < v1) open[i] = mask[v >> 3];
+  }
   const int32_t* bias_ids = a.bias_ids ? a.bias_ids + (int64_t)b * a.num_bias : nullptr;
-  const bool noted = a.token_ids || bias_ids;
+  const int total = a.token_ids ? min(max(a.total_lens[b], 0), a.history_len) : 0;
+  const bool noted = total > 0 || bias_ids;
   if (noted) {
-    for (int i = tid; i < v1 - v0; i += 256) note[i] = 0;
+#pragma unroll
+    for (int i = 0; i < 2 * ITER; ++i) reinterpret_cast<uint4*>(note)[i * 256 + tid] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    if (a.token_ids) {
-      const int total = min(max(a.total_lens[b], 0), a.history_len);
+    if (total > 0) {
       const int prompt = a.prompt_lens ? min(max(a.prompt_lens[b], 0), total) : 0;
-      const int32_t* ids = a.token_ids + (int64_t)b * a.history_stride;
-      for (int i = tid; i < total; i += 256) {
-        const int id = ids[i];
-        if (id >= v0 && id < v1) {
-          if (i < prompt) atomicOr(&note[id - v0], 1u);
-          else atomicAdd(&note[id - v0], 2u);
+      const int32_t* ids = a.token_ids + b * a.history_stride;
+      auto see = [&](int i, int id) {
+        const uint32_t at = (uint32_t)id - (uint32_t)v0;
+        if (id >= 0 && at < (uint32_t)(v1 - v0)) {
+          if (i < prompt) atomicOr(&note[at], 1u);
+          else atomicAdd(&note[at], 2u);
         }
+      };
+      int i = tid;
+      for (; i + 768 < total; i += 1024) {
+        const int p = ids[i], q = ids[i + 256], r = ids[i + 512], s = ids[i + 768];
+        see(i, p);
+        see(i + 256, q);
+        see(i + 512, r);
+        see(i + 768, s);
       }
+      for (; i < total; i += 256) see(i, ids[i]);
     }
-    if (bias_ids) {
-      __syncthreads();
+    if (bias_ids)
       for (int i = tid; i < a.num_bias; i += 256) {
         const int id = bias_ids[i];
         if (id >= v0 && id < v1) atomicOr(&note[id - v0], kHasBias);
       }
-    }
     __syncthreads();
   }
   const float r = a.repetition ? a.repetition[b] : 1.f;
   const float freq = a.frequency ? a.frequency[b] : 0.f;
   const float pres = a.presence ? a.presence[b] : 0.f;
-  const float temp = a.temperature ? fmaxf(a.temperature[b], 1e-5f) : 1.f;
-  const TI* in = static_cast<const TI*>(a.logits) + (int64_t)b * a.logits_stride;
-  TO* out = static_cast<TO*>(a.out) + (int64_t)b * a.out_stride;
-  for (int v = v0 + tid; v < v1; v += 256) {
-    float x = to_f32(in[v]);
-    const uint32_t n = noted ? note[v - v0] : 0;
-    if (n) {
-      const uint32_t count = (n & ~kHasBias) >> 1;
-      if ((n & ~kHasBias) && a.repetition) x = x > 0.f ? x / r : x * r;
-      if (count) x = x - freq * (float)count - pres;
-      if (n & kHasBias)
-        for (int i = 0; i < a.num_bias; ++i)
-          if (bias_ids[i] == v) x += a.bias_values[(int64_t)b * a.num_bias + i];
+  const float inv = a.temperature ? 1.f / fmaxf(a.temperature[b], 1e-5f) : 1.f;
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const int v = v0 + (i * 256 + tid) * 8;
+    if (v >= v1) break;
+    if (noted) {
+      const uint4 p = reinterpret_cast<const uint4*>(note)[(i * 256 + tid) * 2];
+      const uint4 q = reinterpret_cast<const uint4*>(note)[(i * 256 + tid) * 2 + 1];
+      const uint32_t n[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+      if (p.x | p.y | p.z | p.w | q.x | q.y | q.z | q.w) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (!n[k]) continue;
+          const uint32_t seen = n[k] & ~kHasBias, count = seen >> 1;
+          float y = x[i][k];
+          if (seen && a.repetition) y = y > 0.f ? y / r : y * r;
+          if (count) y = y - freq * (float)count - pres;
+          if (n[k] & kHasBias)
+            for (int e = 0; e < a.num_bias; ++e)
+              if (bias_ids[e] == v + k) y += a.bias_values[(int64_t)b * a.num_bias + e];
+          x[i][k] = y;
+        }
+      }
     }
-    x = x / temp;
-    if (a.mask && !((a.mask[(int64_t)b * a.mask_stride + (v >> 5)] >> (v & 31)) & 1))
-      x = __uint_as_float(0xff800000u);
-    from_f32(out + v, x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      x[i][k] = (open[i] >> k) & 1 ? x[i][k] * inv : __uint_as_float(0xff800000u);
+    if (wide && v + 8 <= v1) store8(out + v, x[i]);
+    else
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (v + k < v1) from_f32(out + v + k, x[i][k]);
   }
+}
+
+template <typename TI, typename TO>
+void launch_logits(const LogitsArgs& a, int batch, cudaStream_t s) {
+  // slices of 8192 tokens read the history least often; small batches take 2048 to spread it
+  if ((int64_t)batch * ((a.vocab + 8191) / 8192) >= 2 * 148)
+    kvb_logits_kernel<TI, TO, 4><<<dim3((a.vocab + 8191) / 8192, batch), 256, 0, s>>>(a);
+  else
+    kvb_logits_kernel<TI, TO, 1><<<dim3((a.vocab + 2047) / 2048, batch), 256, 0, s>>>(a);
 }
 
 }  // namespace kvb_step
@@ -307,6 +417,8 @@ extern "C" int kvb_extend_block_tables(const KvbExtendTablesParams* p, void* str
     return fail(KVB_ERR_INVALID, "num_blocks must be in [1, 2^27 - 1] (32-bit slots)");
   if (p->max_new_tokens < 0 || p->free_capacity < 0)
     return fail(KVB_ERR_INVALID, "max_new_tokens and free_capacity must be >= 0");
+  if (p->max_new_tokens > (1 << 30) || p->free_capacity > (1 << 30))
+    return fail(KVB_ERR_UNSUPPORTED, "max_new_tokens and free_capacity must be <= 2^30");
   if (!p->block_tables || !p->seq_lens || !p->new_lens || !p->num_free || !p->cu_new ||
       !p->seq_lens_out || !p->num_free_out || (p->free_capacity && !p->free_blocks) ||
       (p->max_new_tokens && (!p->slots || !p->positions)))
@@ -315,11 +427,32 @@ extern "C" int kvb_extend_block_tables(const KvbExtendTablesParams* p, void* str
                             p->free_capacity, p->block_table_stride, p->block_tables, p->seq_lens,
                             p->new_lens, p->free_blocks, p->num_free, p->slots, p->positions,
                             p->cu_new, p->seq_lens_out, p->num_free_out, p->status};
+  // 16-byte stores of slots and positions
+  if (!aligned(p->slots, 16) || !aligned(p->positions, 16))
+    return fail(KVB_ERR_INVALID, "slots and positions must be 16-byte aligned");
   const int smem = (3 * p->batch + 1) * 4;
-  if (smem > 40 * 1024)
-    cudaFuncSetAttribute(kvb_step::kvb_extend_tables_kernel,
-                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  kvb_step::kvb_extend_tables_kernel<<<1, 1024, smem, static_cast<cudaStream_t>(stream)>>>(a);
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kvb_step::kvb_extend_tables_kernel,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess)
+      return fail(KVB_ERR_CUDA, std::string("kvb_extend_block_tables: ") + cudaGetErrorString(e));
+  }
+  // a decode step of up to 256 rows is one small CTA's scan; long prefills take up to eight
+  // CTAs of four tokens a thread
+  const int threads = p->batch <= 256 && p->max_new_tokens <= 4096 ? 256 : 1024;
+  const int ctas = std::min(8, std::max(1, p->max_new_tokens / (threads * 4)));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ctas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kvb_step::kvb_extend_tables_kernel, a);
   return kvb_step::launched("kvb_extend_block_tables");
 }
 
@@ -340,11 +473,12 @@ extern "C" int kvb_append_paged_kv(const KvbAppendPagedParams* p, void* stream) 
   if (p->k_token_stride % 8 || p->k_head_stride % 8 || p->v_token_stride % 8 ||
       p->v_head_stride % 8)
     return fail(KVB_ERR_INVALID, "strides must be multiples of 8 elements");
-  kvb_step::AppendArgs a = {};
-  a.vecs = p->head_dim / 8;
-  a.heads = p->num_kv_heads;
-  a.tokens = p->num_tokens;
-  a.num_blocks = p->num_blocks;
+  const int vecs = p->head_dim / 8;
+  const int64_t pieces = (int64_t)p->num_tokens * p->num_kv_heads * vecs;
+  if (pieces >= (1ll << 31) - 1024 * 256)
+    return fail(KVB_ERR_UNSUPPORTED, "too many tokens for one call (2^31 16-byte pieces)");
+  kvb_step::AppendArgs a = {kvb_step::Div(p->num_kv_heads * vecs), kvb_step::Div(vecs), (uint32_t)pieces,
+                            p->num_kv_heads, p->num_blocks};
   a.src[0] = static_cast<const uint4*>(p->k_new);
   a.src[1] = static_cast<const uint4*>(p->v_new);
   a.token_stride[0] = p->k_token_stride / 8;
@@ -354,11 +488,11 @@ extern "C" int kvb_append_paged_kv(const KvbAppendPagedParams* p, void* stream) 
   a.pool = static_cast<uint4*>(p->kv_pool);
   a.slots = p->slots;
   a.status = p->status;
-  const int64_t pieces = (int64_t)p->num_tokens * p->num_kv_heads * a.vecs;
-  const int64_t ctas = (pieces + 255) / 256;
-  if (ctas > 0x7fffffff) return fail(KVB_ERR_UNSUPPORTED, "too many tokens for one call");
-  kvb_step::kvb_append_paged_kernel<<<dim3((unsigned)ctas, 2), 256, 0,
-                                      static_cast<cudaStream_t>(stream)>>>(a);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (pieces >= 148 * 4 * 1024)
+    kvb_step::kvb_append_paged_kernel<4><<<dim3((unsigned)((pieces + 1023) / 1024), 2), 256, 0, s>>>(a);
+  else
+    kvb_step::kvb_append_paged_kernel<1><<<dim3((unsigned)((pieces + 255) / 256), 2), 256, 0, s>>>(a);
   return kvb_step::launched("kvb_append_paged_kv");
 }
 
@@ -393,7 +527,6 @@ extern "C" int kvb_process_logits(const KvbLogitsParams* p, void* stream) {
   a.vocab = p->vocab;
   a.history_len = p->history_len;
   a.num_bias = p->num_bias;
-  a.slice = 4096;
   a.logits = p->logits;
   a.out = p->out;
   a.logits_stride = p->logits_stride;
@@ -410,15 +543,13 @@ extern "C" int kvb_process_logits(const KvbLogitsParams* p, void* stream) {
   a.bias_ids = p->num_bias ? p->bias_ids : nullptr;
   a.bias_values = p->bias_values;
   a.mask = p->allowed_mask;
-  void (*kern)(kvb_step::LogitsArgs) = nullptr;
   const bool f32 = p->out_dtype == KVB_DTYPE_FP32;
-  if (p->dtype == KVB_DTYPE_FP32) kern = kvb_step::kvb_logits_kernel<float, float>;
-  else if (p->dtype == KVB_DTYPE_FP16)
-    kern = f32 ? kvb_step::kvb_logits_kernel<__half, float> : kvb_step::kvb_logits_kernel<__half, __half>;
-  else
-    kern = f32 ? kvb_step::kvb_logits_kernel<__nv_bfloat16, float>
-               : kvb_step::kvb_logits_kernel<__nv_bfloat16, __nv_bfloat16>;
-  kern<<<dim3((p->vocab + a.slice - 1) / a.slice, p->batch), 256, a.slice * 4,
-         static_cast<cudaStream_t>(stream)>>>(a);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  using bf16 = __nv_bfloat16;
+  if (p->dtype == KVB_DTYPE_FP32) kvb_step::launch_logits<float, float>(a, p->batch, s);
+  else if (p->dtype == KVB_DTYPE_FP16 && f32) kvb_step::launch_logits<__half, float>(a, p->batch, s);
+  else if (p->dtype == KVB_DTYPE_FP16) kvb_step::launch_logits<__half, __half>(a, p->batch, s);
+  else if (f32) kvb_step::launch_logits<bf16, float>(a, p->batch, s);
+  else kvb_step::launch_logits<bf16, bf16>(a, p->batch, s);
   return kvb_step::launched("kvb_process_logits");
 }

@@ -52,7 +52,7 @@ def _status_ptr(device) -> int:
 def _check_int32(name: str, t: torch.Tensor, ndim: int, device) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype != torch.int32 or t.dim() != ndim or t.device != device:
+    if t.dtype is not torch.int32 or t.dim() != ndim or t.device != device:
         raise RuntimeError(f"{name} must be a {ndim}-D int32 tensor on {device}, got "
                            f"{t.dim()}-D {t.dtype} on {t.device}")
     if not t.is_contiguous():
