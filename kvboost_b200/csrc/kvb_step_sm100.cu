@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(256) kvb_append_paged_kernel(const AppendArgs 
 
 struct LogitsArgs {
   int vocab, history_len, num_bias;
+  int iters;                              // a CTA's slice in 2048 tokens
   const void* logits;
   void* out;
   int64_t logits_stride, out_stride, history_stride, mask_stride;
@@ -259,143 +260,193 @@ __device__ __forceinline__ void from_f32(float* p, float x) { *p = x; }
 __device__ __forceinline__ void from_f32(__half* p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void from_f32(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-// Eight consecutive values, 16 bytes at a time.
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
+// Eight consecutive values as they are stored, and as float32.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
-  T h[8];
-  memcpy(h, &v, 16);
+struct Eight {
+  static constexpr int N = sizeof(T) / 2;
+  uint4 raw[N];
+  __device__ __forceinline__ void load(const T* p, bool wide, int left) {
+    if (wide && left >= 8) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_f32(h[i]);
-}
-__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
-  __stcs(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3]));
-  __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(x[4], x[5], x[6], x[7]));
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
-  T h[8];
+      for (int i = 0; i < N; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+      T h[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) from_f32(h + i, x[i]);
-  uint4 v;
-  memcpy(&v, h, 16);
-  __stcs(reinterpret_cast<uint4*>(p), v);
-}
+      for (int k = 0; k < 8; ++k) from_f32(h + k, k < left ? to_f32(p[k]) : 0.f);
+      memcpy(raw, h, sizeof(raw));
+    }
+  }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+    T h[8];
+    memcpy(h, raw, sizeof(raw));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = to_f32(h[k]);
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&x)[8], bool wide, int left) {
+    T h[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) from_f32(h + k, x[k]);
+    if (wide && left >= 8) {
+      uint4 v[N];
+      memcpy(v, h, sizeof(v));
+#pragma unroll
+      for (int i = 0; i < N; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, v[i]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < left) p[k] = h[k];
+    }
+  }
+};
 
-constexpr uint32_t kHasBias = 1u << 31;   // a note: bit 0 seen, bits 1..30 count, bit 31 biased
+constexpr int kBiasRoom = 256;            // a slice's bias entries kept in shared memory
+constexpr int kCounts16 = 16383;          // the longest history that a 16-bit note can count
 
-// A CTA takes one slice of a row, 8 ITER tokens a thread: it notes the history's tokens that
-// fall into the slice in shared memory (seen bit and count, integer adds: any order gives the
-// same), then streams the slice 16 bytes at a time.  Byte work for large batches (the logits
-// once, the float32 result once; the history is read by every slice's CTA, from L2); the
-// logits are on their way while the history is read.  A row whose pointers or tail do not sit
-// on 16 bytes goes value by value.  The quotient by the temperature is a product with its
-// reciprocal: one more rounding of float32.
-template <typename TI, typename TO, int ITER>
-__global__ void __launch_bounds__(256) kvb_logits_kernel(const LogitsArgs a) {
-  constexpr int kSlice = 256 * 8 * ITER;
-  __shared__ __align__(16) uint32_t note[kSlice];
+// A CTA takes one slice of a row.  It notes the history's tokens that fall into the slice in
+// shared memory (per token a seen bit, a count and a bias bit, in 16 bits, or 32 for long
+// histories; integer adds: any order gives the same) and the slice's bias entries in their
+// order, then streams the slice, 2048 tokens a turn, 8 a thread, 16 bytes at a time, the next
+// turn's logits on their way.  Byte work for large batches: the logits once, the result once;
+// the history is read by every slice's CTA (from L2), so slices are long there, and short
+// (2048) where few rows have to spread over the GPU.  The stream's own work has to stay small
+// beside 6 bytes a token: with the penalties' divisions and the bias list in the unrolled
+// stream it took 124 us for 192 rows of 151936, waiting for instructions; with 32-bit notes
+// of shorter slices, all of a thread's logits in registers, 68 us; so XX us.  The quotients by
+// the repetition penalty and the temperature are products with their reciprocals: one more
+// rounding of float32 each.  A row whose pointers or tail do not sit on 16 bytes goes value by
+// value.
+template <typename TI, typename TO, typename NT>
+__global__ void __launch_bounds__(256, 5) kvb_logits_kernel(const LogitsArgs a) {
+  constexpr int PER = 4 / sizeof(NT), BITS = 8 * sizeof(NT);   // notes a word, bits a note
+  constexpr uint32_t kBias = 1u << (BITS - 1), kAll = BITS == 32 ? ~0u : 0xffffu;
+  extern __shared__ __align__(16) uint32_t note[];
+  __shared__ int32_t list_ids[kBiasRoom];
+  __shared__ float list_values[kBiasRoom];
+  __shared__ int list_len;
   const int b = blockIdx.y, tid = threadIdx.x;
-  const int v0 = blockIdx.x * kSlice, v1 = min(a.vocab, v0 + kSlice);
+  const int v0 = blockIdx.x * a.iters * 2048, v1 = min(a.vocab, v0 + a.iters * 2048);
   const TI* in = static_cast<const TI*>(a.logits) + b * a.logits_stride;
   TO* out = static_cast<TO*>(a.out) + b * a.out_stride;
   const uint8_t* mask = a.mask ? reinterpret_cast<const uint8_t*>(a.mask + b * a.mask_stride) : nullptr;
-  const bool wide = ((reinterpret_cast<uintptr_t>(in + v0) | reinterpret_cast<uintptr_t>(out + v0)) & 15) == 0;
-  float x[ITER][8];
-  uint32_t open[ITER];
-#pragma unroll
-  for (int i = 0; i < ITER; ++i) {
-    const int v = v0 + (i * 256 + tid) * 8;
-    open[i] = 0xff;
-    if (wide && v + 8 <= v1) load8(in + v, x[i]);
-    else
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[i][k] = v + k < v1 ? to_f32(in[v + k]) : 0.f;
-    if (mask && v < v1) open[i] = mask[v >> 3];
+  const bool wide_in = (reinterpret_cast<uintptr_t>(in + v0) & 15) == 0;
+  const bool wide_out = (reinterpret_cast<uintptr_t>(out + v0) & 15) == 0;
+  int v = v0 + tid * 8;
+  Eight<TI> next;
+  uint32_t next_open = 0xff;
+  if (v < v1) {
+    next.load(in + v, wide_in, v1 - v);
+    if (mask) next_open = mask[v >> 3];
   }
   const int32_t* bias_ids = a.bias_ids ? a.bias_ids + (int64_t)b * a.num_bias : nullptr;
+  const float* bias_values = a.bias_values + (int64_t)b * a.num_bias;
   const int total = a.token_ids ? min(max(a.total_lens[b], 0), a.history_len) : 0;
   const bool noted = total > 0 || bias_ids;
   if (noted) {
-#pragma unroll
-    for (int i = 0; i < 2 * ITER; ++i) reinterpret_cast<uint4*>(note)[i * 256 + tid] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < a.iters * 512 / PER; i += 256) reinterpret_cast<uint4*>(note)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     if (total > 0) {
       const int prompt = a.prompt_lens ? min(max(a.prompt_lens[b], 0), total) : 0;
       const int32_t* ids = a.token_ids + b * a.history_stride;
-      auto see = [&](int i, int id) {
-        const uint32_t at = (uint32_t)id - (uint32_t)v0;
-        if (id >= 0 && at < (uint32_t)(v1 - v0)) {
-          if (i < prompt) atomicOr(&note[at], 1u);
-          else atomicAdd(&note[at], 2u);
+      for (int i = tid; i < total; i += 8 * 256) {
+        int id[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) id[k] = i + k * 256 < total ? ids[i + k * 256] : -1;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t at = (uint32_t)id[k] - (uint32_t)v0;
+          if (id[k] >= 0 && at < (uint32_t)(v1 - v0)) {
+            const uint32_t shift = (at % PER) * BITS;
+            if (i + k * 256 < prompt) atomicOr(&note[at / PER], 1u << shift);
+            else atomicAdd(&note[at / PER], 2u << shift);
+          }
         }
-      };
-      int i = tid;
-      for (; i + 768 < total; i += 1024) {
-        const int p = ids[i], q = ids[i + 256], r = ids[i + 512], s = ids[i + 768];
-        see(i, p);
-        see(i + 256, q);
-        see(i + 512, r);
-        see(i + 768, s);
       }
-      for (; i < total; i += 256) see(i, ids[i]);
     }
-    if (bias_ids)
-      for (int i = tid; i < a.num_bias; i += 256) {
-        const int id = bias_ids[i];
-        if (id >= v0 && id < v1) atomicOr(&note[id - v0], kHasBias);
+    if (bias_ids && tid < 32) {           // the slice's entries, in their order
+      int n = 0;
+      for (int e0 = 0; e0 < a.num_bias; e0 += 32) {
+        const int id = e0 + tid < a.num_bias ? bias_ids[e0 + tid] : -1;
+        const bool here = id >= v0 && id < v1;
+        const uint32_t some = __ballot_sync(~0u, here);
+        if (here) {
+          const uint32_t at = id - v0;
+          atomicOr(&note[at / PER], kBias << ((at % PER) * BITS));
+          const int place = n + __popc(some & ((1u << tid) - 1));
+          if (place < kBiasRoom) {
+            list_ids[place] = id;
+            list_values[place] = bias_values[e0 + tid];
+          }
+        }
+        n += __popc(some);
       }
+      if (tid == 0) list_len = n;
+    }
     __syncthreads();
   }
-  const float r = a.repetition ? a.repetition[b] : 1.f;
+  const float r = a.repetition ? a.repetition[b] : 1.f, ir = 1.f / r;
   const float freq = a.frequency ? a.frequency[b] : 0.f;
   const float pres = a.presence ? a.presence[b] : 0.f;
   const float inv = a.temperature ? 1.f / fmaxf(a.temperature[b], 1e-5f) : 1.f;
-#pragma unroll
-  for (int i = 0; i < ITER; ++i) {
-    const int v = v0 + (i * 256 + tid) * 8;
-    if (v >= v1) break;
+#pragma unroll 1
+  for (; v < v1; v += 2048) {
+    float x[8];
+    next.values(x);
+    const uint32_t open = next_open;
+    if (v + 2048 < v1) {
+      next.load(in + v + 2048, wide_in, v1 - v - 2048);
+      if (mask) next_open = mask[(v + 2048) >> 3];
+    }
     if (noted) {
-      const uint4 p = reinterpret_cast<const uint4*>(note)[(i * 256 + tid) * 2];
-      const uint4 q = reinterpret_cast<const uint4*>(note)[(i * 256 + tid) * 2 + 1];
-      const uint32_t n[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
-      if (p.x | p.y | p.z | p.w | q.x | q.y | q.z | q.w) {
+      uint32_t n[8 / PER];
+#pragma unroll
+      for (int i = 0; i < 2 / PER; ++i) {
+        const uint4 q = reinterpret_cast<const uint4*>(note)[(v - v0) / 4 / PER + i];
+        n[4 * i] = q.x, n[4 * i + 1] = q.y, n[4 * i + 2] = q.z, n[4 * i + 3] = q.w;
+      }
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < 8 / PER; ++i) any |= n[i];
+      if (any) {
+        bool biased = false;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          if (!n[k]) continue;
-          const uint32_t seen = n[k] & ~kHasBias, count = seen >> 1;
-          float y = x[i][k];
-          if (seen && a.repetition) y = y > 0.f ? y / r : y * r;
-          if (count) y = y - freq * (float)count - pres;
-          if (n[k] & kHasBias)
-            for (int e = 0; e < a.num_bias; ++e)
-              if (bias_ids[e] == v + k) y += a.bias_values[(int64_t)b * a.num_bias + e];
-          x[i][k] = y;
+          const uint32_t one = (n[k / PER] >> ((k % PER) * BITS)) & kAll, count = (one & ~kBias) >> 1;
+          if ((one & ~kBias) && a.repetition) x[k] *= x[k] > 0.f ? ir : r;
+          if (count) x[k] = x[k] - freq * (float)count - pres;
+          biased |= (one & kBias) != 0;
+        }
+        if (biased) {
+          const bool all = list_len <= kBiasRoom;
+          const int len = all ? list_len : a.num_bias;
+#pragma unroll 1
+          for (int e = 0; e < len; ++e) {
+            const uint32_t at = (uint32_t)((all ? list_ids[e] : bias_ids[e]) - v);
+            if (at < 8) {
+              const float w = all ? list_values[e] : bias_values[e];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) x[k] += at == k ? w : 0.f;
+            }
+          }
         }
       }
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      x[i][k] = (open[i] >> k) & 1 ? x[i][k] * inv : __uint_as_float(0xff800000u);
-    if (wide && v + 8 <= v1) store8(out + v, x[i]);
-    else
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (v + k < v1) from_f32(out + v + k, x[i][k]);
+    for (int k = 0; k < 8; ++k) x[k] = (open >> k) & 1 ? x[k] * inv : __uint_as_float(0xff800000u);
+    Eight<TO>::store(out + v, x, wide_out, v1 - v);
   }
 }
 
 template <typename TI, typename TO>
-void launch_logits(const LogitsArgs& a, int batch, cudaStream_t s) {
-  // slices of 8192 tokens read the history least often; small batches take 2048 to spread it
-  if ((int64_t)batch * ((a.vocab + 8191) / 8192) >= 2 * 148)
-    kvb_logits_kernel<TI, TO, 4><<<dim3((a.vocab + 8191) / 8192, batch), 256, 0, s>>>(a);
+void launch_logits(LogitsArgs a, int batch, cudaStream_t s) {
+  // the longest slices that still give every SM four CTAs
+  const int most = a.history_len <= kCounts16 ? 8 : 4;
+  for (a.iters = most; a.iters > 1; a.iters /= 2)
+    if ((int64_t)batch * ((a.vocab + a.iters * 2048 - 1) / (a.iters * 2048)) >= 4 * 148) break;
+  const dim3 grid((a.vocab + a.iters * 2048 - 1) / (a.iters * 2048), batch);
+  if (a.history_len <= kCounts16)
+    kvb_logits_kernel<TI, TO, uint16_t><<<grid, 256, a.iters * 4096, s>>>(a);
   else
-    kvb_logits_kernel<TI, TO, 1><<<dim3((a.vocab + 2047) / 2048, batch), 256, 0, s>>>(a);
+    kvb_logits_kernel<TI, TO, uint32_t><<<grid, 256, a.iters * 8192, s>>>(a);
 }
 
 }  // namespace kvb_step
