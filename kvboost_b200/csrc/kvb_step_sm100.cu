@@ -311,12 +311,12 @@ constexpr int kCounts16 = 16383;          // the longest history that a 16-bit n
 // (2048) where few rows have to spread over the GPU.  The stream's own work has to stay small
 // beside 6 bytes a token: with the penalties' divisions and the bias list in the unrolled
 // stream it took 124 us for 192 rows of 151936, waiting for instructions; with 32-bit notes
-// of shorter slices, all of a thread's logits in registers, 68 us; so XX us.  The quotients by
+// of shorter slices, all of a thread's logits in registers, 68 us; so 41 us.  The quotients by
 // the repetition penalty and the temperature are products with their reciprocals: one more
 // rounding of float32 each.  A row whose pointers or tail do not sit on 16 bytes goes value by
 // value.
 template <typename TI, typename TO, typename NT>
-__global__ void __launch_bounds__(256, 5) kvb_logits_kernel(const LogitsArgs a) {
+__global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) {
   constexpr int PER = 4 / sizeof(NT), BITS = 8 * sizeof(NT);   // notes a word, bits a note
   constexpr uint32_t kBias = 1u << (BITS - 1), kAll = BITS == 32 ? ~0u : 0xffffu;
   extern __shared__ __align__(16) uint32_t note[];
@@ -342,39 +342,56 @@ __global__ void __launch_bounds__(256, 5) kvb_logits_kernel(const LogitsArgs a) 
   const int total = a.token_ids ? min(max(a.total_lens[b], 0), a.history_len) : 0;
   const bool noted = total > 0 || bias_ids;
   if (noted) {
+    // the first 2048 of the history and 64 of the bias list are on their way while the notes
+    // are cleared
+    const int prompt = a.prompt_lens ? min(max(a.prompt_lens[b], 0), total) : 0;
+    const int32_t* ids = a.token_ids + b * a.history_stride;
+    int id[8], bias_id[2] = {-1, -1};
+    float bias_value[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) id[k] = tid + k * 256 < total ? ids[tid + k * 256] : -1;
+    if (bias_ids && tid < 32)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (tid + 32 * k < a.num_bias) {
+          bias_id[k] = bias_ids[tid + 32 * k];
+          bias_value[k] = bias_values[tid + 32 * k];
+        }
     for (int i = tid; i < a.iters * 512 / PER; i += 256) reinterpret_cast<uint4*>(note)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    if (total > 0) {
-      const int prompt = a.prompt_lens ? min(max(a.prompt_lens[b], 0), total) : 0;
-      const int32_t* ids = a.token_ids + b * a.history_stride;
-      for (int i = tid; i < total; i += 8 * 256) {
-        int id[8];
+    for (int i = tid; i < total; i += 8 * 256) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) id[k] = i + k * 256 < total ? ids[i + k * 256] : -1;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t at = (uint32_t)id[k] - (uint32_t)v0;
-          if (id[k] >= 0 && at < (uint32_t)(v1 - v0)) {
-            const uint32_t shift = (at % PER) * BITS;
-            if (i + k * 256 < prompt) atomicOr(&note[at / PER], 1u << shift);
-            else atomicAdd(&note[at / PER], 2u << shift);
-          }
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t at = (uint32_t)id[k] - (uint32_t)v0, shift = (at % PER) * BITS;
+        if (id[k] >= 0 && at < (uint32_t)(v1 - v0)) {
+          if (i + k * 256 < prompt) atomicOr(&note[at / PER], 1u << shift);
+          else atomicAdd(&note[at / PER], 2u << shift);
         }
       }
+      if (i + 8 * 256 < total)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) id[k] = i + (k + 8) * 256 < total ? ids[i + (k + 8) * 256] : -1;
     }
     if (bias_ids && tid < 32) {           // the slice's entries, in their order
       int n = 0;
       for (int e0 = 0; e0 < a.num_bias; e0 += 32) {
-        const int id = e0 + tid < a.num_bias ? bias_ids[e0 + tid] : -1;
-        const bool here = id >= v0 && id < v1;
+        int mine = bias_id[0];
+        float value = bias_value[0];
+        bias_id[0] = bias_id[1];
+        bias_value[0] = bias_value[1];
+        if (e0 >= 64) {
+          mine = e0 + tid < a.num_bias ? bias_ids[e0 + tid] : -1;
+          value = e0 + tid < a.num_bias ? bias_values[e0 + tid] : 0.f;
+        }
+        const bool here = mine >= v0 && mine < v1;
         const uint32_t some = __ballot_sync(~0u, here);
         if (here) {
-          const uint32_t at = id - v0;
+          const uint32_t at = mine - v0;
           atomicOr(&note[at / PER], kBias << ((at % PER) * BITS));
           const int place = n + __popc(some & ((1u << tid) - 1));
           if (place < kBiasRoom) {
-            list_ids[place] = id;
-            list_values[place] = bias_values[e0 + tid];
+            list_ids[place] = mine;
+            list_values[place] = value;
           }
         }
         n += __popc(some);
@@ -409,11 +426,15 @@ __global__ void __launch_bounds__(256, 5) kvb_logits_kernel(const LogitsArgs a) 
       if (any) {
         bool biased = false;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t one = (n[k / PER] >> ((k % PER) * BITS)) & kAll, count = (one & ~kBias) >> 1;
-          if ((one & ~kBias) && a.repetition) x[k] *= x[k] > 0.f ? ir : r;
-          if (count) x[k] = x[k] - freq * (float)count - pres;
-          biased |= (one & kBias) != 0;
+        for (int w = 0; w < 8 / PER; ++w) {   // a word at a time: few of a warp's 256 tokens are noted
+          if (!n[w]) continue;
+#pragma unroll
+          for (int k = w * PER; k < (w + 1) * PER; ++k) {
+            const uint32_t one = (n[w] >> ((k % PER) * BITS)) & kAll, count = (one & ~kBias) >> 1;
+            if ((one & ~kBias) && a.repetition) x[k] *= x[k] > 0.f ? ir : r;
+            if (count) x[k] = x[k] - freq * (float)count - pres;
+            biased |= (one & kBias) != 0;
+          }
         }
         if (biased) {
           const bool all = list_len <= kBiasRoom;
@@ -439,7 +460,7 @@ __global__ void __launch_bounds__(256, 5) kvb_logits_kernel(const LogitsArgs a) 
 template <typename TI, typename TO>
 void launch_logits(LogitsArgs a, int batch, cudaStream_t s) {
   // the longest slices that still give every SM four CTAs
-  const int most = a.history_len <= kCounts16 ? 8 : 4;
+  const int most = 4;
   for (a.iters = most; a.iters > 1; a.iters /= 2)
     if ((int64_t)batch * ((a.vocab + a.iters * 2048 - 1) / (a.iters * 2048)) >= 4 * 148) break;
   const dim3 grid((a.vocab + a.iters * 2048 - 1) / (a.iters * 2048), batch);
