@@ -962,11 +962,10 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   // may, and each then joins the same pieces into the same values.  Nobody waits.  A flag holds
   // this call's nonce, so the workspace needs no clearing; whoever joins takes the flags back,
   // so a replayed graph starts afresh.
-  asm volatile("fence.acq_rel.gpu;" ::: "memory");
   __syncwarp();
   if (lane < pending) {
     const int64_t at = (2 * (int)blockIdx.x + (wait_for.z == (int)blockIdx.x ? 1 : 0)) * NH + (wait_for.y >> 24);
-    asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(a.flags + at), "l"(a.nonce) : "memory");
+    asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(a.flags + at), "l"(a.nonce) : "memory");
   }
   __syncwarp();
   asm volatile("fence.sc.gpu;" ::: "memory");
@@ -977,12 +976,12 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     bool all = true;
     for (int k = c0 + lane; k <= c1; k += 32) {
       uint64_t f;
-      asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];"
+      asm volatile("ld.acquire.gpu.global.u64 %0, [%1];"
                    : "=l"(f) : "l"(a.flags + (2 * k + (k == c0 ? 1 : 0)) * NH + h) : "memory");
       all &= f == a.nonce;
     }
     if (!__all_sync(~0u, all)) continue;
-    asm volatile("fence.acq_rel.gpu;" ::: "memory");
+    __syncwarp();                                   // what one lane acquired, all lanes may read
     // pieces c0 .. c1, eight at a time in flight; a first one is CTA c0's second slot, the others
     // the first slots of the CTAs after it
     const float* part = a.part + 2 * (int64_t)c0 * G::PART;

@@ -294,12 +294,27 @@ def _make_paged_attn_fn(layer_idx: int, state: dict):
     table and the new K/V straight from the call (``kvb_paged_prefill_fwd``), with
     bottom-right causality; ``state["top_left"] = True`` selects the reference's
     SDPA ``is_causal`` alignment instead.
+
+    With ``state["slots"]`` set, the forward is one decode step of a batch: row b's K/V
+    goes to pool slot ``slots[b]`` and its query attends to the ``seq_lens[b]`` tokens of
+    row b of ``block_tables`` (device tensors, as ``extend_block_tables`` leaves them);
+    ``max_seq_len`` is a host-known bound of the lengths.
     """
     from .paged import block_table_tensor, paged_attention_fwd, paged_prefill_attention
+    from .paged_decode import append_paged_kv, paged_decode_attention
 
     def paged_fn(module, query, key, value, attention_mask=None, dropout=0.0, scaling=None,
                  is_causal=None, **kwargs):
         allocator = state["allocator"]
+        if state.get("slots") is not None:
+            if query.size(2) != 1 or key.size(2) != 1:
+                raise NotImplementedError("a batched paged step takes one token per request")
+            pool = allocator.pools[layer_idx]
+            append_paged_kv(key[:, :, 0], value[:, :, 0], pool, state["slots"])
+            out, _ = paged_decode_attention(query, pool, state["block_tables"], state["seq_lens"],
+                                            softmax_scale=scaling, return_lse=False,
+                                            max_seq_len=state.get("max_seq_len"))
+            return out.transpose(1, 2), None
         write_slot = int(state["_write_slot"])
         if query.size(0) != 1:
             raise NotImplementedError("paged attention serves one sequence per forward")
@@ -334,8 +349,10 @@ def install_paged_attention(model: torch.nn.Module, state: dict) -> int:
 
     ``state``: ``allocator`` (a 16-bit ``DeviceBlockAllocator`` with one pool per
     layer), ``block_table`` (list of block ids, extended in place), ``_write_slot``
-    (logical slot of the next token, advanced by the caller after each forward).
-    Layers are numbered in module order, as in the reference.
+    (logical slot of the next token, advanced by the caller after each forward); or,
+    for decode steps of a batch, ``slots``, ``block_tables`` and ``seq_lens`` (device
+    tensors, renewed by the caller before each forward).  Layers are numbered in module
+    order, as in the reference.
     """
     _require_library()
     patched = 0

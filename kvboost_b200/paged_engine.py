@@ -29,18 +29,24 @@ reference class raises under transformers 5.x (it indexes the returned
 layers.  ``generate_batch`` / ``generate_many`` are ``KVBoost``'s (the
 reference's paged engine inherits them unchanged), and ``BASELINE`` mode runs
 the whole prompt as in ``KVBoost``.
+
+``generate_paged`` has no counterpart in the reference: it decodes several prompts
+over the pool at once, each step's block tables, slots, K/V writes, attention and
+logits on the device (``paged_decode``, ``logits``).
 """
 
 from __future__ import annotations
 
 import time
-from typing import List, Optional, Sequence, Tuple, Union
+from typing import Callable, Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
 from .engine import GenerationMode, GenerationResult, KVBoost, TokenIds
 from .flash_attn_ext import install_paged_attention, uninstall_paged_attention
-from .paged import BLOCK_SIZE, DeviceBlockAllocator, DeviceChunkMapper
+from .logits import process_logits
+from .paged import BLOCK_SIZE, DeviceBlockAllocator, DeviceChunkMapper, block_table_tensor
+from .paged_decode import append_paged_kv, extend_block_tables
 
 
 def _model_dims(model) -> Tuple[int, int, int]:
@@ -171,6 +177,177 @@ class PagedEngine(KVBoost):
             tokens_per_sec=len(generated) / max(t1 - t0, 1e-9), kv_reuse_ratio=hit_ratio,
             prompt_tokens=len(token_ids), cached_tokens=cached_len,
             first_token_logits=first_logits.cpu().numpy(), generated_ids=generated)
+
+    # ── several prompts over the pool at once ──────────────────────────────────
+    def generate_paged(self, prompts: List[Union[str, Sequence[int]]], max_new_tokens: int = 64,
+                       temperature: float = 1.0, do_sample: bool = False,
+                       repetition_penalty: float = 1.0, frequency_penalty: float = 0.0,
+                       presence_penalty: float = 0.0,
+                       logit_bias: Optional[Dict[int, float]] = None,
+                       allowed_tokens: Optional[Callable[[int, List[int]],
+                                                         Optional[Sequence[int]]]] = None,
+                       ) -> List[GenerationResult]:
+        """Decode several prompts together, their K/V in the block pool.
+
+        Each prompt reuses its cached chunks as ``generate`` does (seams repaired, chunk
+        blocks shared through the mapper; a chunk's part-filled last block is copied) and
+        prefills its new tokens; then every step runs one token of every prompt: block
+        tables and slots from the lengths (``extend_block_tables``), K/V into the pool and
+        attention over it in every layer, and the logits' processing
+        (``process_logits``): ``repetition_penalty`` over prompt and output,
+        ``frequency_penalty`` and ``presence_penalty`` over the output, ``logit_bias`` by
+        token id, and ``allowed_tokens(i, output ids)``, the ids prompt i may continue with
+        (None: any).  A prompt that has met the end id keeps its place in the steps until
+        all have ended.  The blocks of the longest outputs are reserved before the first
+        step and returned at the end; the prompts' new chunks are then stored.
+        """
+        if self.allocator.dtype == torch.int8:
+            raise RuntimeError("generate_paged needs a 16-bit pool")
+        if not prompts:
+            return []
+        self._sync()
+        t0 = time.perf_counter()
+        all_ids = [self._encode(p) for p in prompts]
+        if any(not ids for ids in all_ids):
+            raise ValueError("empty prompt")
+        B, bs, dev = len(prompts), self._block_size, self.device
+        prefixes: List[List[int]] = []     # each prompt's blocks of reused chunks
+        forked: List[int] = []             # references to hand back
+        reserved: List[int] = []
+        try:
+            first_logits, kv_new, cached, reused = [], [], [], []
+            for ids in all_ids:
+                keys, values, cached_len, _, chunks = self._assemble_run(ids)
+                table: List[int] = []
+                for c in chunks:
+                    shared = c.chunk_id in self.chunk_mapper._chunk_blocks
+                    k, v = self._chunk_kv([c])
+                    blocks = self.chunk_mapper.load_chunk(
+                        c.chunk_id, [(k[l][None], v[l][None]) for l in range(k.shape[0])])
+                    table.extend(blocks)
+                    if shared:
+                        forked.extend(blocks)
+                reuse = min(cached_len, len(ids) - 1)   # a fully cached prompt's last token runs again
+                if reuse < len(table) * bs:       # the new tokens begin inside a chunk's last block
+                    own = self.allocator.allocate(1)
+                    reserved.extend(own)
+                    for pool in self.allocator.pools:
+                        pool[own[0]].copy_(pool[table[-1]])
+                    table[-1] = own[0]
+                prefixes.append(table)
+                cached.append(cached_len)
+                reused.append(reuse)
+                logits, layers = self._prefill_suffix(ids, keys, values, reuse)
+                first_logits.append(logits)
+                kv_new.append([(k[0, :, reuse:], v[0, :, reuse:]) for k, v in layers])
+            lens = [len(ids) for ids in all_ids]
+            want = [-(-(n + max_new_tokens) // bs) for n in lens]
+            free = self.allocator.allocate(sum(w - len(t) for w, t in zip(want, prefixes)))
+            reserved.extend(free)
+            i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+            tables = block_table_tensor([t + [0] * (w - len(t)) for t, w in zip(prefixes, want)], dev)
+            seq_lens, free_blocks, num_free = i32(reused), i32(free), i32([len(free)])
+            new = [n - c for n, c in zip(lens, reused)]
+            # the prompts' new tokens, packed, layer by layer
+            step = extend_block_tables(tables, seq_lens, i32(new), free_blocks, num_free,
+                                       self.allocator.num_blocks, sum(new), seq_lens_out=seq_lens,
+                                       num_free_out=num_free)
+            for layer, pool in enumerate(self.allocator.pools):
+                parts = [kv[layer] for kv in kv_new]
+                append_paged_kv(torch.cat([k for k, _ in parts], 1).transpose(0, 1).to(pool.dtype),
+                                torch.cat([v for _, v in parts], 1).transpose(0, 1).to(pool.dtype),
+                                pool, step.slots)
+            del kv_new
+            logits = torch.stack(first_logits)
+            V = logits.shape[-1]
+            history = torch.zeros(B, max(lens) + max_new_tokens, dtype=torch.int32, device=dev)
+            for b, ids in enumerate(all_ids):
+                history[b, :lens[b]] = i32(ids)
+            prompt_lens, total_lens = i32(lens), i32(lens)
+            f32 = lambda x: torch.full((B,), float(x), dtype=torch.float32, device=dev)  # noqa: E731
+            penalised = repetition_penalty != 1.0 or frequency_penalty or presence_penalty
+            kw = {}
+            if penalised:
+                kw.update(token_ids=history, prompt_lens=prompt_lens, total_lens=total_lens,
+                          repetition_penalty=f32(repetition_penalty),
+                          frequency_penalty=f32(frequency_penalty),
+                          presence_penalty=f32(presence_penalty))
+            if logit_bias:
+                kw.update(bias_ids=i32([list(logit_bias)] * B),
+                          bias_values=torch.tensor([[float(w) for w in logit_bias.values()]] * B,
+                                                   dtype=torch.float32, device=dev))
+            if do_sample:
+                kw["temperature"] = f32(temperature)
+            generated: List[List[int]] = [[] for _ in range(B)]
+            done = [False] * B
+            ones, rows = i32([1] * B), torch.arange(B, device=dev)
+            eos = self._eos
+            state = {"allocator": self.allocator, "block_tables": tables, "seq_lens": seq_lens}
+            install_paged_attention(self.model, state)
+            try:
+                t_first = 0.0
+                while True:
+                    if allowed_tokens is not None:
+                        kw["allowed_mask"] = self._token_masks(
+                            [allowed_tokens(b, list(generated[b])) for b in range(B)], V)
+                    nxt = self._sample(process_logits(logits.contiguous(), **kw), 1.0, do_sample)
+                    history[rows, total_lens.long()] = nxt.to(torch.int32)
+                    total_lens += 1
+                    for b, t in enumerate(nxt.tolist()):
+                        if not done[b]:
+                            generated[b].append(int(t))
+                            done[b] = eos is not None and int(t) == eos
+                    t_first = t_first or time.perf_counter()
+                    n_out = int(max(len(g) for g in generated))
+                    if all(done) or n_out >= max_new_tokens:
+                        break
+                    step = extend_block_tables(tables, seq_lens, ones, free_blocks, num_free,
+                                               self.allocator.num_blocks, B, seq_lens_out=seq_lens,
+                                               num_free_out=num_free)
+                    state["slots"], state["max_seq_len"] = step.slots, max(lens) + n_out
+                    with torch.no_grad():
+                        logits = self.model(input_ids=nxt[:, None], position_ids=step.positions[:, None],
+                                            use_cache=False, logits_to_keep=1).logits[:, -1]
+            finally:
+                uninstall_paged_attention(self.model)
+            t1 = time.perf_counter()
+        finally:
+            self.allocator.free(reserved)
+            self.allocator.free(forked)
+        results = [GenerationResult(
+            mode="paged_batch", prompt=p if isinstance(p, str) else "",
+            output_text=self._decode_text(generated[b]), generated_tokens=len(generated[b]),
+            ttft_ms=(t_first - t0) * 1e3, total_ms=(t1 - t0) * 1e3,
+            tokens_per_sec=len(generated[b]) / max(t1 - t0, 1e-9),
+            kv_reuse_ratio=cached[b] / max(lens[b], 1), prompt_tokens=lens[b],
+            cached_tokens=cached[b], first_token_logits=first_logits[b].float().cpu().numpy(),
+            generated_ids=generated[b]) for b, p in enumerate(prompts)]
+        for ids in all_ids:
+            self._store_prompt_chunks(ids)
+        return results
+
+    def _prefill_suffix(self, ids: TokenIds, keys, values, reuse: int):
+        """The prompt's tokens from ``reuse`` on over its reused prefix: the last logits
+        ``[V]`` and the cache's layers."""
+        from transformers import DynamicCache
+        cache = (self._cache_from(keys[:, :, :reuse].contiguous(), values[:, :, :reuse].contiguous())
+                 if reuse else DynamicCache())
+        x = torch.tensor([ids[reuse:]], dtype=torch.long, device=self.device)
+        pos = torch.arange(reuse, len(ids), device=self.device)[None]
+        out = self._forward(x, pos, cache)
+        return out.logits[0, -1], self._layers(out.past_key_values)
+
+    def _token_masks(self, allowed: List[Optional[Sequence[int]]], vocab: int) -> torch.Tensor:
+        """Bit masks ``[B, ceil(vocab / 32)]`` of the ids each row may take (None: any)."""
+        words = -(-vocab // 32)
+        bits = torch.zeros(len(allowed), words * 32, dtype=torch.int64)
+        for row, ids in zip(bits, allowed):
+            if ids is None:
+                row.fill_(1)
+            else:
+                row[torch.as_tensor(list(ids), dtype=torch.long)] = 1
+        masks = (bits.view(len(allowed), words, 32) << torch.arange(32)).sum(-1)
+        return (masks - ((masks >> 31) << 32)).to(torch.int32).to(self.device)
 
     def paged_stats(self) -> dict:
         """``paged_stats`` (``cpu_engine.py:514-522``)."""
