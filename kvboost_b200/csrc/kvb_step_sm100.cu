@@ -577,6 +577,7 @@ extern "C" int kvb_process_logits(const KvbLogitsParams* p, void* stream) {
   if (p->batch < 0 || p->vocab < 1 || p->history_len < 0 || p->num_bias < 0)
     return fail(KVB_ERR_INVALID, "batch, history_len and num_bias must be >= 0, vocab >= 1");
   if (p->batch > 65535) return fail(KVB_ERR_UNSUPPORTED, "batch must be <= 65535");
+  if (p->vocab > (1 << 30)) return fail(KVB_ERR_UNSUPPORTED, "vocab must be <= 2^30");
   if (p->batch == 0) return KVB_OK;
   if (!p->logits || !p->out) return fail(KVB_ERR_INVALID, "logits and out must be non-null");
   const size_t el_in = p->dtype == KVB_DTYPE_FP32 ? 4 : 2;

@@ -68,7 +68,7 @@ def process_logits(logits: torch.Tensor, token_ids: Optional[torch.Tensor] = Non
     if V < 1 or (logits.stride(1) != 1 and V > 1):
         raise RuntimeError("logits must have contiguous, non-empty rows")
     if out is None:
-        out = torch.empty(B, V, dtype=torch.float32, device=dev)
+        out = logits.new_empty((B, V), dtype=torch.float32)
     elif out.shape != logits.shape or out.device != dev or (out.stride(1) != 1 and V > 1) \
             or out.dtype not in (torch.float32, logits.dtype):
         raise RuntimeError("out must be float32 or the logits' dtype, of their shape and device, "

@@ -122,9 +122,8 @@ def extend_block_tables(block_tables: torch.Tensor, seq_lens: torch.Tensor,
     if T < 0:
         raise RuntimeError("max_new_tokens must be >= 0")
     # the int32 results share one allocation: slots first (16-byte aligned)
-    slots, cu, lens_out, free_out = torch.empty(T + 2 * B + 2, dtype=torch.int32, device=dev).split(
-        (T, B + 1, B, 1))
-    positions = torch.empty(T, dtype=torch.int64, device=dev)
+    slots, cu, lens_out, free_out = seq_lens.new_empty(T + 2 * B + 2).split_with_sizes((T, B + 1, B, 1))
+    positions = seq_lens.new_empty(T, dtype=torch.int64)
     if seq_lens_out is None:
         seq_lens_out = lens_out
     else:
@@ -259,7 +258,7 @@ def paged_decode_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_tables:
         if out.shape != q.shape or out.dtype != dtype or out.device != dev or out.stride(3) != 1 \
                 or ob % 8 or oh % 8 or out.data_ptr() % 16:
             raise RuntimeError("out must match q in shape, dtype and device, with 16-byte aligned heads")
-    lse = torch.empty((B, Hq, 1), dtype=torch.float32, device=dev) if return_lse else None
+    lse = q.new_empty((B, Hq, 1), dtype=torch.float32) if return_lse else None
     if B == 0:
         return out, lse
     qb, qh, _, _ = q.stride()
@@ -277,7 +276,7 @@ def paged_decode_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_tables:
     if need > 0:
         # partial results of this call: torch's caching allocator orders their reuse on the
         # current stream, so calls on concurrent streams never share them
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = q.new_empty(need, dtype=torch.uint8)
         p.workspace, p.workspace_bytes = ws.data_ptr(), need
     _launch(lib.kvb_paged_decode_fwd, p, dev, "kvb_paged_decode_fwd")
     return out, lse

@@ -201,8 +201,8 @@ class PagedEngine(KVBoost):
         all have ended.  The blocks of the longest outputs are reserved before the first
         step and returned at the end; the prompts' new chunks are then stored.
         """
-        if self.allocator.dtype == torch.int8:
-            raise RuntimeError("generate_paged needs a 16-bit pool")
+        if self.allocator.dtype != next(self.model.parameters()).dtype:
+            raise RuntimeError("generate_paged needs a pool in the model's dtype")
         if not prompts:
             return []
         self._sync()
@@ -290,10 +290,17 @@ class PagedEngine(KVBoost):
                     if allowed_tokens is not None:
                         kw["allowed_mask"] = self._token_masks(
                             [allowed_tokens(b, list(generated[b])) for b in range(B)], V)
-                    nxt = self._sample(process_logits(logits.contiguous(), **kw), 1.0, do_sample)
+                    x = process_logits(logits.contiguous(), **kw)
+                    # a row without a finite best (all masked, NaN) cannot be sampled from
+                    lost = ~torch.isfinite(x.amax(-1))
+                    nxt = self._sample(x.masked_fill_(lost[:, None], 0.0), 1.0, do_sample)
                     history[rows, total_lens.long()] = nxt.to(torch.int32)
                     total_lens += 1
-                    for b, t in enumerate(nxt.tolist()):
+                    picked, lost = torch.stack([nxt, lost.long()]).tolist()
+                    if any(lost):
+                        raise ValueError(f"no token is left for prompt {lost.index(1)}: its logits "
+                                         "are all masked or not finite")
+                    for b, t in enumerate(picked):
                         if not done[b]:
                             generated[b].append(int(t))
                             done[b] = eos is not None and int(t) == eos
@@ -344,8 +351,11 @@ class PagedEngine(KVBoost):
         for row, ids in zip(bits, allowed):
             if ids is None:
                 row.fill_(1)
-            else:
-                row[torch.as_tensor(list(ids), dtype=torch.long)] = 1
+                continue
+            at = torch.as_tensor(list(ids), dtype=torch.long)
+            if at.numel() and not 0 <= int(at.min()) <= int(at.max()) < vocab:
+                raise ValueError(f"allowed token ids must lie in [0, {vocab})")
+            row[at] = 1
         masks = (bits.view(len(allowed), words, 32) << torch.arange(32)).sum(-1)
         return (masks - ((masks >> 31) << 32)).to(torch.int32).to(self.device)
 

@@ -147,3 +147,17 @@ def test_pool_too_small_leaves_the_pool_as_it_was():
     with pytest.raises(RuntimeError, match="OOM"):
         eng.generate_paged(_prompts([100, 100], 0), max_new_tokens=10)
     assert eng.allocator.free_blocks == 8
+
+
+def test_a_prompt_without_a_token_left_is_refused():
+    from kvboost_b200.paged_engine import PagedEngine
+    eng = PagedEngine(_model(), num_blocks=64, recompute_strategy="none")
+    p = _prompts([20, 30], 0)
+    for sample in (False, True):
+        with pytest.raises(ValueError, match="prompt 1"):
+            eng.generate_paged(p, max_new_tokens=4, do_sample=sample, allowed_tokens=lambda i, out: [3, 4] if i == 0 else [])
+    with pytest.raises(ValueError, match="lie in"):
+        eng.generate_paged(p, max_new_tokens=4, allowed_tokens=lambda i, out: [501])
+    assert eng.allocator.free_blocks == 64
+    twice = eng.generate_paged([p[0], p[0]], max_new_tokens=6)
+    assert twice[0].generated_ids == twice[1].generated_ids

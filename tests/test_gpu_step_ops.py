@@ -406,6 +406,35 @@ def test_paged_decode_shapes_of_the_launch_agree():
             _check_attention(o, lse, q, pool, tables, ln, 0.125)
 
 
+@pytest.mark.parametrize("pool_kind", ["same", "int8"])
+@pytest.mark.parametrize("B,longest", [(40, 3000), (256, 1400), (257, 1400), (700, 1200), (8193, 1100)])
+def test_paged_decode_batch_sizes(pool_kind, B, longest):
+    """Every way the rows are divided: a row per lane, eight, sums over the CTA, a CTA per item;
+    idle rows between, one long row."""
+    g = torch.Generator().manual_seed(B)
+    ln = (torch.randint(0, 50, (B,), generator=g) * (torch.rand(B, generator=g) < 0.7)).tolist()
+    ln[B // 3] = longest
+    ln[-1] = 0
+    pool, tables, ks, vs = _pool(g, ln, 1, 64, torch.bfloat16, pool_kind == "int8")
+    q = torch.randn(B, 2, 1, 64, generator=g).to(torch.bfloat16)
+    o, lse = _attend(q, pool, tables, ln, ks, vs)
+    _check_attention(o, lse, q, pool, tables, ln, 0.125, ks, vs)
+
+
+@pytest.mark.parametrize("ln", [[50, 20], [5000, 3000, 9]])
+def test_paged_decode_over_its_own_query(ln):
+    """out=q: the output takes the query's place."""
+    from kvboost_b200.paged_decode import paged_decode_attention
+    g = torch.Generator().manual_seed(17)
+    pool, tables, _, _ = _pool(g, ln, 2, 128, torch.float16, False)
+    q = torch.randn(len(ln), 16, 1, 128, generator=g).to(torch.float16)
+    want, _ = _attend(q, pool, tables, ln)
+    qc = q.cuda()
+    o, _ = paged_decode_attention(qc, pool.cuda(), tables.cuda(),
+                                  torch.tensor(ln, dtype=torch.int32, device=DEV), out=qc)
+    assert o is qc and torch.equal(qc, want)
+
+
 def test_paged_decode_offsets_past_32_bits():
     """A pool of 2.6e9 elements: the last blocks are written and read."""
     from kvboost_b200.paged_decode import append_paged_kv, paged_decode_attention
@@ -488,7 +517,8 @@ def _check_logits(got, want, c, dtype):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("B,V,L,N", [(1, 1, 3, 1), (1, 31, 0, 0), (2, 33, 40, 5), (3, 1000, 1, 0),
                                      (5, 4097, 300, 17), (2, 50001, 5000, 300), (1, 151936, 77, 3),
-                                     (70, 2048, 33, 2)])
+                                     (70, 2048, 33, 2), (2, 33, 9, 300), (200, 20000, 50, 3),
+                                     (100, 30000, 17000, 2)])
 def test_process_logits(dtype, B, V, L, N):
     from kvboost_b200.logits import process_logits
     c = _logits_case(B, V, L, N, dtype, V + L)
@@ -509,6 +539,23 @@ def test_process_logits(dtype, B, V, L, N):
     assert process_logits(**d, out=d["logits"]) is d["logits"]
     _check_logits(d["logits"], want, c, dtype)
     assert (wide[:, :3] == 7).all() and (wide[:, 3 + V:] == 7).all()
+
+
+def test_process_logits_captured():
+    """A captured call follows its inputs' new values at each replay."""
+    from kvboost_b200.logits import process_logits
+    c = _logits_case(3, 5000, 60, 4, torch.bfloat16, 8)
+    d = {k: t.cuda() for k, t in c.items()}
+    process_logits(**d)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = process_logits(**d)
+    for seed in (1, 2):
+        c = _logits_case(3, 5000, 60, 4, torch.bfloat16, seed)
+        for k, t in c.items():
+            d[k].copy_(t)
+        graph.replay()
+        _check_logits(o, _oracle_logits(c), c, torch.float32)
 
 
 def test_process_logits_special_values():

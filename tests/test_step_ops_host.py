@@ -85,6 +85,10 @@ INV, UNS = _lib.KVB_ERR_INVALID, _lib.KVB_ERR_UNSUPPORTED
     (_logits, "kvb_process_logits", "out_dtype", 1, INV, "out_dtype"),
     (_logits, "kvb_process_logits", "vocab", 0, INV, "vocab"),
     (_logits, "kvb_process_logits", "batch", 65536, UNS, "batch"),
+    (_logits, "kvb_process_logits", "vocab", (1 << 30) + 1, UNS, "vocab"),
+    (_tables, "kvb_extend_block_tables", "max_new_tokens", (1 << 30) + 1, UNS, "max_new_tokens"),
+    (_tables, "kvb_extend_block_tables", "positions", 4104, INV, "aligned"),
+    (_decode, "kvb_paged_decode_fwd", "max_blocks_per_seq", 1 << 30, INV, "block_table_stride"),
     (_logits, "kvb_process_logits", "logits", 4097, INV, "aligned"),
     (_logits, "kvb_process_logits", "out_stride", 999, INV, "strides"),
     (_logits, "kvb_process_logits", "out", 4096, INV, "in place"),
@@ -119,6 +123,34 @@ def test_python_ops_refuse_cpu_tensors():
         paged_decode_attention(h[:, :, None], pool, torch.zeros(1, 2, dtype=torch.int32), i)
     with pytest.raises(RuntimeError, match="CUDA"):
         process_logits(torch.zeros(1, 8))
+
+
+def test_decode_split_launch_needs_its_workspace(lib):
+    p = _decode(max_blocks_per_seq=4096, block_table_stride=4096)
+    need = lib.kvb_paged_decode_workspace_bytes(ctypes.byref(p))
+    assert need > 0
+    assert lib.kvb_paged_decode_fwd(ctypes.byref(p), None) == INV
+    assert b"workspace" in lib.kvb_last_error()
+    p.workspace, p.workspace_bytes = 4100, need
+    assert lib.kvb_paged_decode_fwd(ctypes.byref(p), None) == INV
+    assert b"aligned" in lib.kvb_last_error()
+    p = _decode(max_blocks_per_seq=(1 << 27) - 1, block_table_stride=1 << 27, batch=100)
+    assert lib.kvb_paged_decode_fwd(ctypes.byref(p), None) == UNS
+
+
+def test_token_masks():
+    """Bit v % 32 of word v // 32, the sign bit included."""
+    from types import SimpleNamespace
+
+    from kvboost_b200.paged_engine import PagedEngine
+    eng = SimpleNamespace(device="cpu")
+    m = PagedEngine._token_masks(eng, [None, [0, 31, 32, 69], []], 70)
+    assert m.dtype == torch.int32 and m.shape == (3, 3)
+    assert m[0].tolist() == [-1, -1, -1]
+    assert m[1].tolist() == [1 - 2 ** 31, 1, 32] and m[2].tolist() == [0, 0, 0]
+    for bad in ([70], [-1]):
+        with pytest.raises(ValueError):
+            PagedEngine._token_masks(eng, [bad], 70)
 
 
 def test_struct_layouts_match_the_header(tmp_path):
