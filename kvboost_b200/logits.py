@@ -30,7 +30,8 @@ def _per_row(name: str, t: Optional[torch.Tensor], batch: int, device, dtype) ->
         return None
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype != dtype or t.device != device or t.shape != (batch,) or not t.is_contiguous():
+    if t.dtype is not dtype or t.device != device or t.dim() != 1 or t.numel() != batch \
+            or not t.is_contiguous():
         raise RuntimeError(f"{name} must be a contiguous {dtype} tensor of {batch} entries on {device}")
     return t.data_ptr()
 
@@ -68,24 +69,26 @@ def process_logits(logits: torch.Tensor, token_ids: Optional[torch.Tensor] = Non
     if V < 1 or (logits.stride(1) != 1 and V > 1):
         raise RuntimeError("logits must have contiguous, non-empty rows")
     if out is None:
-        out = logits.new_empty((B, V), dtype=torch.float32)
+        out = logits.new_empty(B, V, dtype=torch.float32)
     elif out.shape != logits.shape or out.device != dev or (out.stride(1) != 1 and V > 1) \
             or out.dtype not in (torch.float32, logits.dtype):
         raise RuntimeError("out must be float32 or the logits' dtype, of their shape and device, "
                            "with contiguous rows")
-    penalties = [_per_row(n, t, B, dev, torch.float32) for n, t in (
-        ("repetition_penalty", repetition_penalty), ("frequency_penalty", frequency_penalty),
-        ("presence_penalty", presence_penalty), ("temperature", temperature))]
+    f32 = torch.float32
+    rep = _per_row("repetition_penalty", repetition_penalty, B, dev, f32)
+    freq = _per_row("frequency_penalty", frequency_penalty, B, dev, f32)
+    pres = _per_row("presence_penalty", presence_penalty, B, dev, f32)
+    temp = _per_row("temperature", temperature, B, dev, f32)
     L = history_stride = 0
     if token_ids is not None:
         _check_int32("token_ids", token_ids, 2, dev)
-        if token_ids.shape[0] != B or total_lens is None:
+        rows, L = token_ids.shape
+        if rows != B or total_lens is None:
             raise RuntimeError(f"token_ids must be [{B}, L] with total_lens")
-        L = token_ids.shape[1]
-        history_stride = max(L, token_ids.stride(0)) if B > 1 else L
-        if B > 1 and token_ids.stride(0) < L:
+        history_stride = token_ids.stride()[0] if B > 1 else L
+        if history_stride < L:
             raise RuntimeError("token_ids rows must not overlap")
-    elif any(x is not None for x in (prompt_lens, total_lens, *penalties[:3])):
+    elif any(x is not None for x in (prompt_lens, total_lens, rep, freq, pres)):
         raise RuntimeError("lengths and penalties need token_ids")
     prompt = _per_row("prompt_lens", prompt_lens, B, dev, torch.int32)
     total = _per_row("total_lens", total_lens, B, dev, torch.int32)
@@ -104,21 +107,21 @@ def process_logits(logits: torch.Tensor, token_ids: Optional[torch.Tensor] = Non
     if allowed_mask is not None:
         _check_int32("allowed_mask", allowed_mask, 2, dev)
         words = (V + 31) // 32
-        if allowed_mask.shape[0] != B or allowed_mask.shape[1] < words:
+        rows, width = allowed_mask.shape
+        if rows != B or width < words:
             raise RuntimeError(f"allowed_mask must be [{B}, >= {words}]")
-        mask_stride = allowed_mask.stride(0) if B > 1 else allowed_mask.shape[1]
+        mask_stride = allowed_mask.stride()[0] if B > 1 else width
         if mask_stride < words:
             raise RuntimeError("allowed_mask rows must not overlap")
     if B == 0:
         return out
     ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    ls, os_ = (logits.stride(0), out.stride(0)) if B > 1 else (V, V)
+    ls, os_ = (logits.stride()[0], out.stride()[0]) if B > 1 else (V, V)
     if ls < V or os_ < V:
         raise RuntimeError("rows of logits and out must not overlap")
     p = _lib.KvbLogitsParams(
         _LOGIT_DTYPES[logits.dtype], _LOGIT_DTYPES[out.dtype], B, V, L, N, logits.data_ptr(),
-        out.data_ptr(), ls, os_, ptr(token_ids), history_stride, prompt, total, penalties[0],
-        penalties[1], penalties[2], penalties[3], ptr(bias_ids), ptr(bias_values),
-        ptr(allowed_mask), mask_stride)
+        out.data_ptr(), ls, os_, ptr(token_ids), history_stride, prompt, total, rep, freq, pres,
+        temp, ptr(bias_ids), ptr(bias_values), ptr(allowed_mask), mask_stride)
     _launch(_lib.load().kvb_process_logits, p, dev, "kvb_process_logits")
     return out

@@ -68,7 +68,7 @@ def _check_tables(block_tables: torch.Tensor, batch: int, device) -> int:
     rows, width = block_tables.shape
     if rows != batch or width < 1:
         raise RuntimeError(f"block_tables must be [{batch}, >= 1], got {tuple(block_tables.shape)}")
-    stride = block_tables.stride(0) if batch > 1 else width
+    stride = block_tables.stride()[0] if batch > 1 else width
     if stride < width:
         raise RuntimeError("block_tables rows must not overlap")
     return stride
@@ -114,7 +114,7 @@ def extend_block_tables(block_tables: torch.Tensor, seq_lens: torch.Tensor,
     _check_int32("new_lens", new_lens, 1, dev)
     _check_int32("num_free", num_free, 1, dev)
     _check_int32("free_blocks", free_blocks, 1, dev)
-    if len(seq_lens) != B or len(new_lens) != B or len(num_free) != 1:
+    if seq_lens.numel() != B or new_lens.numel() != B or num_free.numel() != 1:
         raise RuntimeError(f"seq_lens and new_lens must have {B} entries, num_free one")
     if not 1 <= B <= _lib.KVB_MAX_STEP_ROWS:
         raise RuntimeError(f"a step has 1 to {_lib.KVB_MAX_STEP_ROWS} rows, got {B}")
@@ -132,10 +132,10 @@ def extend_block_tables(block_tables: torch.Tensor, seq_lens: torch.Tensor,
         num_free_out = free_out
     else:
         _check_int32("num_free_out", num_free_out, 1, dev)
-    if len(seq_lens_out) != B or len(num_free_out) != 1:
+    if seq_lens_out.numel() != B or num_free_out.numel() != 1:
         raise RuntimeError(f"seq_lens_out must have {B} entries, num_free_out one")
     p = _lib.KvbExtendTablesParams(
-        B, width, BLOCK_SIZE, int(num_blocks), T, len(free_blocks), stride,
+        B, width, BLOCK_SIZE, int(num_blocks), T, free_blocks.numel(), stride,
         block_tables.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(),
         num_free.data_ptr(), slots.data_ptr(), positions.data_ptr(), cu.data_ptr(),
         seq_lens_out.data_ptr(), num_free_out.data_ptr(), _status_ptr(dev))
@@ -181,8 +181,8 @@ def append_paged_kv(k_new: torch.Tensor, v_new: torch.Tensor, kv_pool: torch.Ten
     if D % 8 or D > 256:
         raise RuntimeError(f"head_dim must be a multiple of 8 up to 256, got {D}")
     _check_int32("slots", slots, 1, dev)
-    if len(slots) != T:
-        raise RuntimeError(f"slots must have {T} entries, got {len(slots)}")
+    if slots.numel() != T:
+        raise RuntimeError(f"slots must have {T} entries, got {slots.numel()}")
     if T == 0:
         return
     kt, kh, _ = k_new.stride()
@@ -231,8 +231,8 @@ def paged_decode_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_tables:
         raise RuntimeError(f"num_q_heads ({Hq}) must be divisible by num_kv_heads ({Hkv})")
     stride = _check_tables(block_tables, B, dev)
     _check_int32("seq_lens", seq_lens, 1, dev)
-    if len(seq_lens) != B:
-        raise RuntimeError(f"seq_lens must have {B} entries, got {len(seq_lens)}")
+    if seq_lens.numel() != B:
+        raise RuntimeError(f"seq_lens must have {B} entries, got {seq_lens.numel()}")
     dtype, pool_dtype = q.dtype, kv_pool.dtype
     if pool_dtype == torch.int8:
         fmt = _lib.KVB_POOL_INT8_KIVI
@@ -251,14 +251,14 @@ def paged_decode_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_tables:
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(D)
     if out is None:
-        out = q.new_empty((B, Hq, 1, D))
+        out = q.new_empty(B, Hq, 1, D)
         ob, oh = Hq * D, D
     else:
         ob, oh = out.stride()[:2] if out.dim() == 4 else (1, 1)
         if out.shape != q.shape or out.dtype != dtype or out.device != dev or out.stride(3) != 1 \
                 or ob % 8 or oh % 8 or out.data_ptr() % 16:
             raise RuntimeError("out must match q in shape, dtype and device, with 16-byte aligned heads")
-    lse = q.new_empty((B, Hq, 1), dtype=torch.float32) if return_lse else None
+    lse = q.new_empty(B, Hq, 1, dtype=torch.float32) if return_lse else None
     if B == 0:
         return out, lse
     qb, qh, _, _ = q.stride()
