@@ -16,16 +16,25 @@
 // no CTA-wide step sits in the loop.  Items that a warp holds whole it writes itself;
 // the pieces at its range's ends are joined in shared memory at the CTA's end, and what
 // still spans CTAs goes to the workspace, where the CTA that finds all of an item's pieces
-// joins them.  Short tables take one CTA per item instead, whose warps split the item.
+// joins them.  Short tables take one CTA per item instead, whose warps split the item (split()
+// below says when).
 //
 // Arithmetic (per block, tokens on the MMA's rows, query heads on its columns):
 //   S^T = K Q^T; online softmax down the rows against a maximum that is raised only when
 //   a score passes it by 2^8 (one vote instead of shuffles); O^T += V^T P^T.
 // P is carried in two 16-bit halves (p = hi + lo), so the weights keep 16 bits and the
 // result's error is that of its final rounding; the second MMA is free here.
-// KIVI int8 pools: codes are exact in float16, so Q (scaled by a power of two per row)
-// and P are float16 and the scales act in float32 on S (K, per token) and on each
-// block's product (V, per channel): nothing is rounded to 16 bits in between.
+// KIVI int8 pools: a code is exact in float16 (as a subnormal, biased by 128; the bias leaves
+// through the accumulators' start), so Q (scaled by a power of two per row) and P are float16
+// and the scales act in float32 on S (K, per token) and on each block's product (V, per
+// channel): the dequantised values are never rounded.  Under bfloat16, whose output rounds by
+// 2^-8, P is one float16 number (2^-11) there.
+//
+// Measured (B200, us per call in a CUDA graph, of the measured 6.48 TB/s copy): 64 requests of
+// 700 .. 16381 tokens, 32/8 heads, D 128, bfloat16: 207 (6.28 TB/s, 97 %); 8 x 4096, 16/2 heads:
+// 14.7 (start, joins); int8 4 x 32768, 64/8 heads: 56.5 (5.1 TB/s, 78 %: the same compute-free, so
+// start and end of the one wave); 24 requests of 1 .. 2051 tokens, 32 heads of D 96, float16: 23.3
+// (3.8 TB/s).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -51,12 +60,22 @@ using namespace kvb::ptx;
 int fail(int code, const std::string& msg) { return kvb_detail_fail(code, msg); }
 
 constexpr int kSms = 148;
-constexpr float kRaise = 8.f;              // log2 units a score may pass the running maximum by
 constexpr uint64_t kWaitNs = 2000000000ull;
-constexpr int kWarpsI8 = 12;               // warps per CTA over int8 pools (8 otherwise)
-constexpr int kItemCost = 1;               // an item's start and end, in blocks
-constexpr int kItemBlocks = 64;            // tables up to this wide take one CTA per item
-constexpr int kMinUnits = 8;               // blocks per CTA below which fewer CTAs share them
+// Log2 units that a score may pass the running maximum by before it is raised.  (0, raising at
+// every new maximum: int8 4 x 32768 tokens 56.9 us instead of 56.4.)
+constexpr float kRaise = 8.f;
+// Warps per CTA over int8 pools (8 otherwise): a block is half the bytes and twice the
+// instructions.  int8 4 x 32768 tokens, 64/8 heads: 65.0 us with 8, 57.2 with 12, 60.5 with 16
+// (which spill).
+constexpr int kWarpsI8 = 12;
+// What an item's start and end weigh in the split, in blocks: 24 requests of 1 to 2051 tokens,
+// 32 heads of D 96: 24.2 us with 0, 19.6 with 1 and 2.
+constexpr int kItemCost = 1;
+// Places per CTA below which fewer CTAs share a split (one request of 2000 tokens, 2 KV heads:
+// 10.3 us with 8, 9.2 with 16, 12.1 with 32), and the most CTAs per item (the join reads them
+// all: one request of 32768 tokens, 1 KV head: 20.3 us on 148 CTAs, 13.7 on 64).
+constexpr int kMinUnits = 16;
+constexpr int kSpan = 64;
 constexpr int kSplitRows = 8192;           // most rows of a split launch (prefix sums in shared memory)
 
 struct Args {
@@ -982,7 +1001,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     }
     if (!__all_sync(~0u, all)) continue;
     __syncwarp();                                   // what one lane acquired, all lanes may read
-    // pieces c0 .. c1, eight at a time in flight; a first one is CTA c0's second slot, the others
+    // pieces c0 .. c1, sixteen at a time in flight; a first one is CTA c0's second slot, the others
     // the first slots of the CTAs after it
     const float* part = a.part + 2 * (int64_t)c0 * G::PART;
     auto piece = [&](int k) { return part + (k == 0 ? 1 : 2 * k) * G::PART; };
@@ -990,25 +1009,25 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     float top = -INFINITY, sum = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-    for (int k0 = 0; k0 < n; k0 += 8) {
-      const int mine = min(k0 + (lane & 7), n - 1);
+    for (int k0 = 0; k0 < n; k0 += 16) {
+      const int mine = min(k0 + (lane & 15), n - 1);
       float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(mine) + NH * D + 2 * h));
-      float4 v[8];
+      float4 v[16];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = __ldcg(reinterpret_cast<const float4*>(piece(min(k0 + k, n - 1)) + x4));
+      for (int k = 0; k < 16; ++k) v[k] = __ldcg(reinterpret_cast<const float4*>(piece(min(k0 + k, n - 1)) + x4));
       const float up = fmaxf(top, warp_max(ml.x)), zero = up == -INFINITY ? 0.f : up;
       const float keep = ex2(top - zero), w = ex2(ml.x - zero);
       top = up;
-      sum = sum * keep + (lane < 8 && k0 + lane < n ? ml.y * w : 0.f);  // lanes 0 .. 7: shares of the sum
+      sum = sum * keep + (lane < 16 && k0 + lane < n ? ml.y * w : 0.f);  // lanes 0 .. 15: shares of the sum
       o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 16; ++k) {
         const float f = __shfl_sync(~0u, w, k);
         if (k0 + k < n) o.x += f * v[k].x, o.y += f * v[k].y, o.z += f * v[k].z, o.w += f * v[k].w;
       }
     }
 #pragma unroll
-    for (int x = 4; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
+    for (int x = 8; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
     sum = __shfl_sync(~0u, sum, 0);
     for (int k = c0 + lane; k <= c1; k += 32) a.flags[(2 * k + (k == c0 ? 1 : 0)) * NH + h] = 0;
     const int kvh = a.tiles == 1 ? ij : ij / a.tiles;
@@ -1023,16 +1042,29 @@ bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) &
 // Query heads per item: 8, or 16 where a group has more.
 int head_tiles(const KvbPagedDecodeParams* p) { return p->num_q_heads / p->num_kv_heads > 8 ? 2 : 1; }
 
-// One CTA per item, or the units split over the GPU.  Short tables: an item is a few blocks
-// per warp, and a launch to join pieces would cost more than it spreads.
+int64_t items(const KvbPagedDecodeParams* p) {
+  const int nh = 8 * head_tiles(p), group = p->num_q_heads / p->num_kv_heads;
+  return (int64_t)p->batch * p->num_kv_heads * ((group + nh - 1) / nh);
+}
+
+// One CTA per item, or the blocks split over the GPU.  A CTA per item needs no places to be
+// found and no joins, and the hardware hands items to SMs as they come free; but a long row
+// keeps its CTA for long, and very many items are as many starts.  What the host knows is the
+// table's width (or the caller's bound).  Measured, us per call (CTA per item / split), KV
+// heads x requests = items, D 128, 16 bits: 2 items of 256 tokens 5.1 / 7.7, of 1024 9.2 / 8.0,
+// of 2048 15.0 / 8.9; 32 of 1024 9.8 / 10.7; 128 of 2048 25.1 / 31.3; 512 of 64 13.7 / 15.3, of
+// 2048 85.7 / 95.9; 2048 of 64 54.5 / 26.4, of 256 73.0 / 62.7, of 1024 164 / 188.  int8: 256 of
+// 1024 25.0 / 26.8; 512 of 256 27.1 / 22.8, of 1024 45.6 / 41.0.
 bool split(const KvbPagedDecodeParams* p) {
   if (p->batch > kSplitRows) return false;
+  // 32-bit places: wider than any pool
+  if ((int64_t)p->batch * (p->max_blocks_per_seq + kItemCost) * p->num_q_heads > 0x7fffffff) return false;
   const int64_t width = p->max_seq_len > 0
                             ? std::min<int64_t>(p->max_blocks_per_seq, ((int64_t)p->max_seq_len + 15) / 16)
                             : p->max_blocks_per_seq;
-  // 32-bit places: wider than any pool
-  if ((int64_t)p->batch * (p->max_blocks_per_seq + kItemCost) * p->num_q_heads > 0x7fffffff) return false;
-  return width > kItemBlocks;
+  const int64_t n = items(p);
+  if (n > (p->pool_format == KVB_POOL_INT8_KIVI ? 2 : 4) * kSms) return true;
+  return width > (n < 64 ? 64 : 128);
 }
 
 // Workspace of a split launch: CTAs' pieces, warps' first pieces, flags.
@@ -1216,7 +1248,9 @@ extern "C" int kvb_paged_decode_fwd(const KvbPagedDecodeParams* p, void* stream)
   a.status = p->status;
   if (is_split) {
     const int64_t most = (int64_t)p->batch * p->max_blocks_per_seq * a.items;
-    a.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(kvb_pd::kSms, (most + kvb_pd::kMinUnits - 1) / kvb_pd::kMinUnits));
+    a.ctas = (int)std::max<int64_t>(
+        1, std::min({(int64_t)kvb_pd::kSms, (most + kvb_pd::kMinUnits - 1) / kvb_pd::kMinUnits,
+                     kvb_pd::kSpan * kvb_pd::items(p)}));
     const kvb_pd::Room room(p);
     uint8_t* w = static_cast<uint8_t*>(p->workspace);
     a.part = reinterpret_cast<float*>(w + room.part);
