@@ -31,8 +31,8 @@
 // 2^-8, P is one float16 number (2^-11) there.
 //
 // Measured (B200, us per call in a CUDA graph, of the measured 6.48 TB/s copy): 64 requests of
-// 700 .. 16381 tokens, 32/8 heads, D 128, bfloat16: 207 (6.28 TB/s, 97 %); 8 x 4096, 16/2 heads:
-// 14.7 (start, joins); int8 4 x 32768, 64/8 heads: 56.5 (5.1 TB/s, 78 %: the same compute-free, so
+// 700 .. 16381 tokens, 32/8 heads, D 128, bfloat16: 206 (6.3 TB/s, 97 %); 8 x 4096, 16/2 heads:
+// 14.4 (start, joins); int8 4 x 32768, 64/8 heads: 56.5 (5.1 TB/s, 78 %: the same compute-free, so
 // start and end of the one wave); 24 requests of 1 .. 2051 tokens, 32 heads of D 96, float16: 23.3
 // (3.8 TB/s).
 
@@ -64,10 +64,11 @@ constexpr uint64_t kWaitNs = 2000000000ull;
 // Log2 units that a score may pass the running maximum by before it is raised.  (0, raising at
 // every new maximum: int8 4 x 32768 tokens 56.9 us instead of 56.4.)
 constexpr float kRaise = 8.f;
-// Warps per CTA over int8 pools (8 otherwise): a block is half the bytes and twice the
-// instructions.  int8 4 x 32768 tokens, 64/8 heads: 65.0 us with 8, 57.2 with 12, 60.5 with 16
-// (which spill).
-constexpr int kWarpsI8 = 12;
+// Warps per CTA for items of up to 8 heads.  64 requests of 700 .. 16381 tokens in bfloat16: 211
+// us with 8 warps of three stages, 209 with 10, 206 with 12 of two; int8 4 x 32768 tokens, 64/8
+// heads: 65.0 with 8, 63.4 with 10, 57.0 with 12, 60.6 with 14, 60.5 with 16 (which spill).
+// Items of 16 heads hold twice the accumulators: 8 warps.
+constexpr int kWarps8Heads = 12, kWarps16Heads = 8;
 // What an item's start and end weigh in the split, in blocks: 24 requests of 1 to 2051 tokens,
 // 32 heads of D 96: 24.2 us with 0, 19.6 with 1 and 2.
 constexpr int kItemCost = 1;
@@ -211,7 +212,7 @@ __device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity, int32_t
 // ---- geometry -------------------------------------------------------------------------------
 template <int D, bool I8, int NT>
 struct Geo {
-  static constexpr int WARPS = I8 && NT == 1 ? kWarpsI8 : 8;
+  static constexpr int WARPS = NT == 1 ? kWarps8Heads : kWarps16Heads;
   static constexpr int THREADS = WARPS * 32;
   static constexpr int NH = 8 * NT;                          // query heads per item
   static constexpr int DP = I8 ? (D == 64 ? 64 : 128) : D;   // features the MMAs cover
@@ -1074,7 +1075,7 @@ struct Room {
     const int64_t nh = 8 * head_tiles(p);
     part = 0;
     first = part + 4 * kSms * 2 * (nh * p->head_dim + 2 * nh);
-    flags = first + 4 * kSms * std::max(8, kWarpsI8) * (nh * (p->head_dim + 4) + 2 * nh);
+    flags = first + 4 * kSms * std::max(kWarps8Heads, kWarps16Heads) * (nh * (p->head_dim + 4) + 2 * nh);
     bytes = flags + kSms * 2 * nh * (int64_t)sizeof(uint64_t);
   }
 };
