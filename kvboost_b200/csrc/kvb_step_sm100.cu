@@ -450,9 +450,9 @@ __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) 
 
 template <typename TI, typename TO>
 void launch_logits(LogitsArgs a, int batch, cudaStream_t s) {
-  // the longest slices that still give every SM four CTAs
-  const int most = 4;
-  for (a.iters = most; a.iters > 1; a.iters /= 2)
+  // Slices of up to 8192 tokens, as long as every SM gets four CTAs (192 x 151936: 41.2 us with
+  // 8192, 44.0 with 16384, 47.0 with 4096; one row: 3.9 us with 2048, 19 CTAs of 8192 5.4).
+  for (a.iters = 4; a.iters > 1; a.iters /= 2)
     if ((int64_t)batch * ((a.vocab + a.iters * 2048 - 1) / (a.iters * 2048)) >= 4 * 148) break;
   const dim3 grid((a.vocab + a.iters * 2048 - 1) / (a.iters * 2048), batch);
   if (a.history_len <= kCounts16)
