@@ -570,7 +570,7 @@ int kvb_append_paged_kv(const KvbAppendPagedParams* params, void* stream);
  * joined through the workspace by the last of them.  workspace:
  * kvb_paged_decode_workspace_bytes(params) bytes (-1: invalid params), 16-byte
  * aligned, whatever it holds; calls that may overlap on the GPU must not share
- * one.  max_seq_len (0: unknown) is a hint that only chooses the launch shape;
+ * one, and one of a call that set KVB_STATUS_LOAD_WAIT must not be used again.  max_seq_len (0: unknown) is a hint that only chooses the launch shape;
  * any value gives right results (their last bits may differ).
  */
 typedef struct KvbPagedDecodeParams {
