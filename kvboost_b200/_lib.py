@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import struct
 import threading
 
 from . import _build
@@ -187,6 +188,23 @@ class KvbLogitsParams(ctypes.Structure):
     ]
 
 
+def packer(cls):
+    """A function that packs the values of a structure's fields, in order, into the bytes the C
+    compiler would lay out (0 for a null pointer): a third of the time that filling the
+    ctypes structure takes, for calls made once per layer and token."""
+    codes = {_i32: "i", _i64: "q", _f32: "f", _vp: "P"}
+    layout = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_))
+    if layout.size != ctypes.sizeof(cls):
+        raise TypeError(f"{cls.__name__} ends in padding")
+    return layout.pack
+
+
+pack_extend_tables = packer(KvbExtendTablesParams)
+pack_append_paged = packer(KvbAppendPagedParams)
+pack_paged_decode = packer(KvbPagedDecodeParams)
+pack_logits = packer(KvbLogitsParams)
+
+
 def pointer_array(ptrs):
     """A ctypes ``void*[n]`` of device addresses (keep it alive across the call)."""
     arr = (ctypes.c_void_p * len(ptrs))(*[int(p) if p else None for p in ptrs])
@@ -247,15 +265,15 @@ def load() -> ctypes.CDLL:
         lib.kvb_quantize_store_batch.restype = ctypes.c_int
         lib.kvb_cacheblend_fwd.argtypes = [ctypes.POINTER(KvbCacheBlendParams), _vp]
         lib.kvb_cacheblend_fwd.restype = ctypes.c_int
-        lib.kvb_extend_block_tables.argtypes = [ctypes.POINTER(KvbExtendTablesParams), _vp]
+        lib.kvb_extend_block_tables.argtypes = [_vp, _vp]   # packed bytes or a pointer
         lib.kvb_extend_block_tables.restype = ctypes.c_int
-        lib.kvb_append_paged_kv.argtypes = [ctypes.POINTER(KvbAppendPagedParams), _vp]
+        lib.kvb_append_paged_kv.argtypes = [_vp, _vp]   # packed bytes or a pointer
         lib.kvb_append_paged_kv.restype = ctypes.c_int
-        lib.kvb_paged_decode_fwd.argtypes = [ctypes.POINTER(KvbPagedDecodeParams), _vp]
+        lib.kvb_paged_decode_fwd.argtypes = [_vp, _vp]   # packed bytes or a pointer
         lib.kvb_paged_decode_fwd.restype = ctypes.c_int
-        lib.kvb_paged_decode_workspace_bytes.argtypes = [ctypes.POINTER(KvbPagedDecodeParams)]
+        lib.kvb_paged_decode_workspace_bytes.argtypes = [_vp]
         lib.kvb_paged_decode_workspace_bytes.restype = ctypes.c_int64
-        lib.kvb_process_logits.argtypes = [ctypes.POINTER(KvbLogitsParams), _vp]
+        lib.kvb_process_logits.argtypes = [_vp, _vp]   # packed bytes or a pointer
         lib.kvb_process_logits.restype = ctypes.c_int
         lib.kvb_last_error.argtypes = []
         lib.kvb_last_error.restype = ctypes.c_char_p

@@ -25,9 +25,10 @@ _LOGIT_DTYPES = {torch.bfloat16: _lib.KVB_DTYPE_BF16, torch.float16: _lib.KVB_DT
                  torch.float32: _lib.KVB_DTYPE_FP32}
 
 
-def _per_row(name: str, t: Optional[torch.Tensor], batch: int, device, dtype) -> Optional[int]:
+def _per_row(name: str, t: Optional[torch.Tensor], batch: int, device, dtype) -> int:
+    """Address of a row parameter, 0 for one that is not given."""
     if t is None:
-        return None
+        return 0
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype is not dtype or t.device != device or t.dim() != 1 or t.numel() != batch \
@@ -88,7 +89,7 @@ def process_logits(logits: torch.Tensor, token_ids: Optional[torch.Tensor] = Non
         history_stride = token_ids.stride()[0] if B > 1 else L
         if history_stride < L:
             raise RuntimeError("token_ids rows must not overlap")
-    elif any(x is not None for x in (prompt_lens, total_lens, rep, freq, pres)):
+    elif prompt_lens is not None or total_lens is not None or rep or freq or pres:
         raise RuntimeError("lengths and penalties need token_ids")
     prompt = _per_row("prompt_lens", prompt_lens, B, dev, torch.int32)
     total = _per_row("total_lens", total_lens, B, dev, torch.int32)
@@ -115,11 +116,11 @@ def process_logits(logits: torch.Tensor, token_ids: Optional[torch.Tensor] = Non
             raise RuntimeError("allowed_mask rows must not overlap")
     if B == 0:
         return out
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     ls, os_ = (logits.stride()[0], out.stride()[0]) if B > 1 else (V, V)
     if ls < V or os_ < V:
         raise RuntimeError("rows of logits and out must not overlap")
-    p = _lib.KvbLogitsParams(
+    p = _lib.pack_logits(
         _LOGIT_DTYPES[logits.dtype], _LOGIT_DTYPES[out.dtype], B, V, L, N, logits.data_ptr(),
         out.data_ptr(), ls, os_, ptr(token_ids), history_stride, prompt, total, rep, freq, pres,
         temp, ptr(bias_ids), ptr(bias_values), ptr(allowed_mask), mask_stride)

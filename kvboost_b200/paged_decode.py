@@ -134,7 +134,7 @@ def extend_block_tables(block_tables: torch.Tensor, seq_lens: torch.Tensor,
         _check_int32("num_free_out", num_free_out, 1, dev)
     if seq_lens_out.numel() != B or num_free_out.numel() != 1:
         raise RuntimeError(f"seq_lens_out must have {B} entries, num_free_out one")
-    p = _lib.KvbExtendTablesParams(
+    p = _lib.pack_extend_tables(
         B, width, BLOCK_SIZE, int(num_blocks), T, free_blocks.numel(), stride,
         block_tables.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(),
         num_free.data_ptr(), slots.data_ptr(), positions.data_ptr(), cu.data_ptr(),
@@ -193,7 +193,7 @@ def append_paged_kv(k_new: torch.Tensor, v_new: torch.Tensor, kv_pool: torch.Ten
     if vt % 8 or vh % 8 or v_new.data_ptr() % 16:
         v_new = v_new.clone(memory_format=torch.contiguous_format)
         vt, vh, _ = v_new.stride()
-    p = _lib.KvbAppendPagedParams(
+    p = _lib.pack_append_paged(
         D, H, T, num_blocks, k_new.data_ptr(), v_new.data_ptr(), kt, kh, vt, vh,
         kv_pool.data_ptr(), slots.data_ptr(), _status_ptr(dev))
     _launch(_lib.load().kvb_append_paged_kv, p, dev, "kvb_append_paged_kv")
@@ -243,13 +243,15 @@ def paged_decode_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_tables:
                 raise RuntimeError(f"int8 pools need {name}: contiguous float16 {list(shape)} on {dev}")
         ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
     else:
-        fmt, ks, vs = _lib.KVB_POOL_COMPUTE, None, None
+        fmt, ks, vs = _lib.KVB_POOL_COMPUTE, 0, 0
         if pool_dtype != dtype:
             raise RuntimeError("a 16-bit pool must hold the compute dtype")
         if k_scale is not None or v_scale is not None:
             raise RuntimeError("scales belong to int8 pools")
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(D)
+    if max_seq_len is not None and not 0 <= max_seq_len < 1 << 31:
+        raise RuntimeError(f"max_seq_len must be in [0, 2^31), got {max_seq_len}")
     if out is None:
         out = q.new_empty(B, Hq, 1, D)
         ob, oh = Hq * D, D
@@ -265,18 +267,17 @@ def paged_decode_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_tables:
     if qb % 8 or qh % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
         qb, qh, _, _ = q.stride()
-    p = _lib.KvbPagedDecodeParams(
-        _DTYPES[dtype], D, B, Hq, Hkv, BLOCK_SIZE, fmt, softmax_scale, q.data_ptr(),
-        out.data_ptr(), lse.data_ptr() if return_lse else None, qb, qh, ob, oh, Hq,
-        kv_pool.data_ptr(), ks, vs, num_blocks, block_tables.shape[1], stride,
-        block_tables.data_ptr(), seq_lens.data_ptr(), 0 if max_seq_len is None else int(max_seq_len),
-        0, _status_ptr(dev), None, 0)
+    fields = (_DTYPES[dtype], D, B, Hq, Hkv, BLOCK_SIZE, fmt, softmax_scale, q.data_ptr(),
+              out.data_ptr(), lse.data_ptr() if return_lse else 0, qb, qh, ob, oh, Hq,
+              kv_pool.data_ptr(), ks, vs, num_blocks, block_tables.shape[1], stride,
+              block_tables.data_ptr(), seq_lens.data_ptr(), max_seq_len or 0, 0, _status_ptr(dev))
     lib = _lib.load()
+    p = _lib.pack_paged_decode(*fields, 0, 0)
     need = lib.kvb_paged_decode_workspace_bytes(p)
     if need > 0:
         # partial results of this call: torch's caching allocator orders their reuse on the
         # current stream, so calls on concurrent streams never share them
         ws = q.new_empty(need, dtype=torch.uint8)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), need
+        p = _lib.pack_paged_decode(*fields, ws.data_ptr(), need)
     _launch(lib.kvb_paged_decode_fwd, p, dev, "kvb_paged_decode_fwd")
     return out, lse

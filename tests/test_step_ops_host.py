@@ -184,3 +184,16 @@ def test_oracle_tables_follow_the_host_allocator():
     assert out[0][0, 2:4].tolist() == model.allocate(2)
     assert out[0][1, :1].tolist() == model.allocate(1)
     assert out[5] == 15 and out[-1] == 0
+
+
+def test_packed_parameters_equal_the_structures(lib):
+    """``packer`` lays the fields out as the ctypes mirrors do."""
+    for cls, pack in ((_lib.KvbExtendTablesParams, _lib.pack_extend_tables),
+                      (_lib.KvbAppendPagedParams, _lib.pack_append_paged),
+                      (_lib.KvbPagedDecodeParams, _lib.pack_paged_decode),
+                      (_lib.KvbLogitsParams, _lib.pack_logits)):
+        values = [0.25 if t is ctypes.c_float else 3 + i + (1 << 40 if ctypes.sizeof(t) == 8 else 0)
+                  for i, (_, t) in enumerate(cls._fields_)]
+        assert pack(*values) == bytes(cls(*values))
+    p = _lib.pack_paged_decode(*[0] * len(_lib.KvbPagedDecodeParams._fields_))
+    assert lib.kvb_paged_decode_workspace_bytes(p) == -1 and b"head_dim" in lib.kvb_last_error()
