@@ -64,11 +64,16 @@ constexpr uint64_t kWaitNs = 2000000000ull;
 // Log2 units that a score may pass the running maximum by before it is raised.  (0, raising at
 // every new maximum: int8 4 x 32768 tokens 56.9 us instead of 56.4.)
 constexpr float kRaise = 8.f;
-// Warps per CTA for items of up to 8 heads.  64 requests of 700 .. 16381 tokens in bfloat16: 211
-// us with 8 warps of three stages, 209 with 10, 206 with 12 of two; int8 4 x 32768 tokens, 64/8
-// heads: 65.0 with 8, 63.4 with 10, 57.0 with 12, 60.6 with 14, 60.5 with 16 (which spill).
-// Items of 16 heads hold twice the accumulators: 8 warps.
-constexpr int kWarps8Heads = 12, kWarps16Heads = 8;
+// Warps per CTA, as registers allow.  Items of up to 8 heads: 64 requests of 700 .. 16381 tokens in
+// bfloat16 took 211 us with 8 warps of three stages, 209 with 10, 206 with 12 of two; int8 4 x
+// 32768 tokens, 64/8 heads: 65.0 with 8, 63.4 with 10, 57.0 with 12, 60.6 with 14, 60.5 with 16
+// (which spill).  D 64 needs fewer registers: 16 warps instead of 12 took 32 x 16384 tokens, 8 KV
+// heads, from 6.28 to 6.43 TB/s, 64 x 16384 in int8 from 4.36 to 4.96.  Items of 16 heads hold twice
+// the accumulators: 8 warps (10: 5.81 TB/s instead of 5.89), 12 for int8 of D 64 (3.68, with 8 2.94).
+constexpr int warps_of(int D, bool i8, int tiles8) {
+  return tiles8 == 1 ? (D == 64 ? 16 : 12) : (D == 64 && i8 ? 12 : 8);
+}
+constexpr int kMostWarps = 16;
 // What an item's start and end weigh in the split, in blocks: 24 requests of 1 to 2051 tokens,
 // 32 heads of D 96: 24.2 us with 0, 19.6 with 1 and 2.
 constexpr int kItemCost = 1;
@@ -117,6 +122,11 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
@@ -212,12 +222,11 @@ __device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity, int32_t
 // ---- geometry -------------------------------------------------------------------------------
 template <int D, bool I8, int NT>
 struct Geo {
-  static constexpr int WARPS = NT == 1 ? kWarps8Heads : kWarps16Heads;
+  static constexpr int WARPS = warps_of(D, I8, NT);
   static constexpr int THREADS = WARPS * 32;
   static constexpr int NH = 8 * NT;                          // query heads per item
-  static constexpr int DP = I8 ? (D == 64 ? 64 : 128) : D;   // features the MMAs cover
   static constexpr int HALVES = I8 ? 1 : (D + 63) / 64;      // TMA boxes per block
-  static constexpr int ROW = I8 ? DP : 128;                  // bytes of a box row = its swizzle
+  static constexpr int ROW = I8 && D == 64 ? 64 : 128;       // bytes of a box row = its swizzle
   static constexpr int BOX = 2 * 16 * ROW;                   // K and V, 16 tokens
   static constexpr int STAGE = HALVES * BOX;
   static constexpr int SCALES = I8 ? 32 + 256 : 0;           // K then V scales of the block
@@ -294,7 +303,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   using E = typename std::conditional<I8, __half, T>::type;   // MMA operand type
   // int8 pools under bfloat16: float16 weights (2^-11) are well below the output's own 2^-8
   constexpr bool LOW = !(I8 && std::is_same<T, __nv_bfloat16>::value);
-  constexpr int MT = G::DP / 16, KS = G::DP / 16, NS = G::NS, NH = G::NH;
+  constexpr int MT = D / 16, KS = D / 16, NS = G::NS, NH = G::NH;
   constexpr int kWarps = G::WARPS, kThreads = G::THREADS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -503,7 +512,8 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     }
   };
   // An item's query heads as the MMA's B operand: for 16-bit pools features 16 ks + 2c, + 8; for
-  // int8 pools in the order the K codes are read (lane c's 16-byte pieces c, c + 4), still in T.
+  // int8 pools in the order the K codes are read (lane c's 16-byte pieces c, c + 4; of D 96 its words
+  // 4 ks + c), still in T.
   auto load_q = [&](uint32_t (&f)[NT][KS][2], int qb, int qj) {
     const int kv = a.tiles == 1 ? qj : qj / a.tiles, hq = kv * a.group + (qj - kv * a.tiles) * NH;
 #pragma unroll
@@ -513,8 +523,8 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         if constexpr (I8) {
-          const int d = 16 * (c + 4 * (ks >> 2)) + 4 * (ks & 3);
-          const uint2 x = on && d < D ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0u, 0u);
+          const int d = D == 96 ? 16 * ks + 4 * c : 16 * (c + 4 * (ks >> 2)) + 4 * (ks & 3);
+          const uint2 x = on ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0u, 0u);
           f[t][ks][0] = x.x;
           f[t][ks][1] = x.y;
         } else {
@@ -648,20 +658,28 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
           for (int t = 0; t < NT; ++t) mma<E>(sa[t][ks & 1], f, qf[t][ks][0], qf[t][ks][1]);
         }
       } else {
+        auto codes = [&](int ks, uint32_t p, uint32_t v) {   // tokens r and r + 8, four features
+          p ^= 0x80808080u;
+          v ^= 0x80808080u;
+          const uint32_t f[4] = {codes_to_half(p, 0x4140), codes_to_half(v, 0x4140),
+                                 codes_to_half(p, 0x4342), codes_to_half(v, 0x4342)};
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma<E>(sa[t][ks & 1], f, qf[t][ks][0], qf[t][ks][1]);
+        };
+        if constexpr (D == 96) {                    // 24 words a row: lane c the words 4 ks + c
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            const uint32_t at = base + r * 128 + ((ks ^ (r & 7)) << 4) + 4 * c;
+            codes(ks, lds32(at), lds32(at + 8 * 128));
+          }
+        } else
 #pragma unroll
         for (int i = 0; i < KS / 4; ++i) {
           const uint32_t at = G::ROW == 128 ? (((c + 4 * i) ^ (r & 7)) << 4) : ((c ^ ((r >> 1) & 3)) << 4);
           const uint4 x = lds128(base + r * G::ROW + at), y = lds128(base + (r + 8) * G::ROW + at);
           const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t p = xs[w] ^ 0x80808080u, v = ys[w] ^ 0x80808080u;
-            const uint32_t f[4] = {codes_to_half(p, 0x4140), codes_to_half(v, 0x4140),
-                                   codes_to_half(p, 0x4342), codes_to_half(v, 0x4342)};
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-              mma<E>(sa[t][w & 1], f, qf[t][4 * i + w][0], qf[t][4 * i + w][1]);
-          }
+          for (int w = 0; w < 4; ++w) codes(4 * i + w, xs[w], ys[w]);
         }
       }
       // log2 scores: [t][0..1] token r, [2..3] token r + 8; heads 2c, 2c + 1
@@ -748,13 +766,17 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
       } else {
         // lane r reads features [PR r, PR r + PR) of tokens 2c, 2c + 1, 2c + 8, 2c + 9; MMA row
         // r of tile jj is feature PR r + 2 jj, row r + 8 the next one
-        constexpr int W = G::DP / 32;               // 32-bit words of a lane's features
+        constexpr int W = D / 32;               // 32-bit words of a lane's features
         uint32_t v[4][W];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int row = 2 * c + (k & 1) + (k >> 1) * 8;
           const uint32_t at = base + 16 * G::ROW + row * G::ROW;
-          if constexpr (G::ROW == 128) {
+          if constexpr (D == 96) {
+#pragma unroll
+            for (int w = 0; w < 3; ++w)
+              v[k][w] = lds32(at + ((((3 * r + w) >> 2) ^ (row & 7)) << 4) + ((3 * r + w) & 3) * 4) ^ 0x80808080u;
+          } else if constexpr (G::ROW == 128) {
             const uint4 z = lds128(at + ((r ^ (row & 7)) << 4));
             v[k][0] = z.x ^ 0x80808080u, v[k][1] = z.y ^ 0x80808080u;
             v[k][2] = z.z ^ 0x80808080u, v[k][3] = z.w ^ 0x80808080u;
@@ -765,9 +787,9 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
         }
         uint32_t vs[W * 2];                         // the features' scales, float16 pairs
 #pragma unroll
-        for (int k = 0; k < W / 2; ++k) {
-          const uint4 z = lds128(sc + 32 + r * (W * 8) + k * 16);
-          vs[4 * k] = z.x, vs[4 * k + 1] = z.y, vs[4 * k + 2] = z.z, vs[4 * k + 3] = z.w;
+        for (int k = 0; k < W; ++k) {
+          const uint2 z = lds64(sc + 32 + r * (W * 8) + k * 8);
+          vs[2 * k] = z.x, vs[2 * k + 1] = z.y;
         }
         // -128 * 2^-24 * the block's weights: what the codes' bias adds to every feature
         float bias[NT][4];
@@ -838,15 +860,13 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
         } else {
 #pragma unroll
           for (int jj = 0; jj < MT; ++jj) {
-            const int d = r * (G::DP / 8) + 2 * jj;
-            if (d < D) {
-              if (t * 8 + 2 * c < heads)
-                *reinterpret_cast<uint32_t*>(o + (2 * c) * a.o_hs + d) =
-                    pack<T>(st.acc[t][jj][0] * i0, st.acc[t][jj][2] * i0);
-              if (t * 8 + 2 * c + 1 < heads)
-                *reinterpret_cast<uint32_t*>(o + (2 * c + 1) * a.o_hs + d) =
-                    pack<T>(st.acc[t][jj][1] * i1, st.acc[t][jj][3] * i1);
-            }
+            const int d = r * (D / 8) + 2 * jj;
+            if (t * 8 + 2 * c < heads)
+              *reinterpret_cast<uint32_t*>(o + (2 * c) * a.o_hs + d) =
+                  pack<T>(st.acc[t][jj][0] * i0, st.acc[t][jj][2] * i0);
+            if (t * 8 + 2 * c + 1 < heads)
+              *reinterpret_cast<uint32_t*>(o + (2 * c + 1) * a.o_hs + d) =
+                  pack<T>(st.acc[t][jj][1] * i1, st.acc[t][jj][3] * i1);
           }
         }
         if (a.lse && r == 0)
@@ -870,8 +890,8 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
           for (int jj = 0; jj < MT; ++jj)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              const int d = I8 ? r * (G::DP / 8) + 2 * jj + k : jj * 16 + 8 * k + r;
-              if (!I8 || d < D) p[h * G::OS + d] = st.acc[t][jj][2 * k + i] * (I8 ? 1.f / kCode : 1.f);
+              const int d = I8 ? r * (D / 8) + 2 * jj + k : jj * 16 + 8 * k + r;
+              p[h * G::OS + d] = st.acc[t][jj][2 * k + i] * (I8 ? 1.f / kCode : 1.f);
             }
           if (r == 0) {
             p[NH * G::OS + h] = st.m[t][i];
@@ -1075,7 +1095,7 @@ struct Room {
     const int64_t nh = 8 * head_tiles(p);
     part = 0;
     first = part + 4 * kSms * 2 * (nh * p->head_dim + 2 * nh);
-    flags = first + 4 * kSms * std::max(kWarps8Heads, kWarps16Heads) * (nh * (p->head_dim + 4) + 2 * nh);
+    flags = first + 4 * kSms * kMostWarps * (nh * (p->head_dim + 4) + 2 * nh);
     bytes = flags + kSms * 2 * nh * (int64_t)sizeof(uint64_t);
   }
 };
