@@ -211,6 +211,7 @@ class PagedEngine(KVBoost):
         if any(not ids for ids in all_ids):
             raise ValueError("empty prompt")
         B, bs, dev = len(prompts), self._block_size, self.device
+        most = max(1, int(max_new_tokens))   # a first token comes with the prompt, as in generate
         prefixes: List[List[int]] = []     # each prompt's blocks of reused chunks
         forked: List[int] = []             # references to hand back
         reserved: List[int] = []
@@ -224,11 +225,12 @@ class PagedEngine(KVBoost):
                     k, v = self._chunk_kv([c])
                     blocks = self.chunk_mapper.load_chunk(
                         c.chunk_id, [(k[l][None], v[l][None]) for l in range(k.shape[0])])
+                    # a reference of this call's own, whether or not the chunk was in the pool
+                    forked.extend(blocks if shared else self.allocator.fork(blocks))
                     table.extend(blocks)
-                    if shared:
-                        forked.extend(blocks)
                 reuse = min(cached_len, len(ids) - 1)   # a fully cached prompt's last token runs again
-                if reuse < len(table) * bs:       # the new tokens begin inside a chunk's last block
+                table = table[:-(-reuse // bs)]
+                if reuse % bs:                    # the new tokens begin inside a chunk's block
                     own = self.allocator.allocate(1)
                     reserved.extend(own)
                     for pool in self.allocator.pools:
@@ -241,7 +243,7 @@ class PagedEngine(KVBoost):
                 first_logits.append(logits)
                 kv_new.append([(k[0, :, reuse:], v[0, :, reuse:]) for k, v in layers])
             lens = [len(ids) for ids in all_ids]
-            want = [-(-(n + max_new_tokens) // bs) for n in lens]
+            want = [-(-(n + most) // bs) for n in lens]
             free = self.allocator.allocate(sum(w - len(t) for w, t in zip(want, prefixes)))
             reserved.extend(free)
             i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
@@ -260,7 +262,7 @@ class PagedEngine(KVBoost):
             del kv_new
             logits = torch.stack(first_logits)
             V = logits.shape[-1]
-            history = torch.zeros(B, max(lens) + max_new_tokens, dtype=torch.int32, device=dev)
+            history = torch.zeros(B, max(lens) + most, dtype=torch.int32, device=dev)
             for b, ids in enumerate(all_ids):
                 history[b, :lens[b]] = i32(ids)
             prompt_lens, total_lens = i32(lens), i32(lens)
@@ -289,7 +291,8 @@ class PagedEngine(KVBoost):
                 while True:
                     if allowed_tokens is not None:
                         kw["allowed_mask"] = self._token_masks(
-                            [allowed_tokens(b, list(generated[b])) for b in range(B)], V)
+                            [None if done[b] else allowed_tokens(b, list(generated[b]))
+                             for b in range(B)], V)
                     x = process_logits(logits.contiguous(), **kw)
                     # a row without a finite best (all masked, NaN) cannot be sampled from
                     lost = ~torch.isfinite(x.amax(-1))
@@ -297,16 +300,17 @@ class PagedEngine(KVBoost):
                     history[rows, total_lens.long()] = nxt.to(torch.int32)
                     total_lens += 1
                     picked, lost = torch.stack([nxt, lost.long()]).tolist()
-                    if any(lost):
-                        raise ValueError(f"no token is left for prompt {lost.index(1)}: its logits "
-                                         "are all masked or not finite")
                     for b, t in enumerate(picked):
-                        if not done[b]:
-                            generated[b].append(int(t))
-                            done[b] = eos is not None and int(t) == eos
+                        if done[b]:
+                            continue
+                        if lost[b]:
+                            raise ValueError(f"no token is left for prompt {b}: its logits are all "
+                                             "masked or not finite")
+                        generated[b].append(int(t))
+                        done[b] = eos is not None and int(t) == eos
                     t_first = t_first or time.perf_counter()
                     n_out = int(max(len(g) for g in generated))
-                    if all(done) or n_out >= max_new_tokens:
+                    if all(done) or n_out >= most:
                         break
                     step = extend_block_tables(tables, seq_lens, ones, free_blocks, num_free,
                                                self.allocator.num_blocks, B, seq_lens_out=seq_lens,

@@ -161,3 +161,48 @@ def test_a_prompt_without_a_token_left_is_refused():
     assert eng.allocator.free_blocks == 64
     twice = eng.generate_paged([p[0], p[0]], max_new_tokens=6)
     assert twice[0].generated_ids == twice[1].generated_ids
+
+
+def test_the_end_id_stops_a_prompt_and_keeps_the_others_going():
+    """A prompt that met the end id takes no more tokens and is asked for none; zero new tokens
+    means one, as in ``generate``."""
+    from types import SimpleNamespace
+
+    from kvboost_b200.paged_engine import PagedEngine
+    m = _model()
+    p = _prompts([20, 33, 50], 0)
+    eng = PagedEngine(m, num_blocks=64, recompute_strategy="none")
+    free = [r.generated_ids for r in eng.generate_paged(p, max_new_tokens=8)]
+    eos = free[1][2]
+    eng.tokenizer = SimpleNamespace(eos_token_id=eos, pad_token_id=None,
+                                    decode=lambda ids, skip_special_tokens: " ".join(map(str, ids)))
+    asked = []
+
+    def allowed(i, out):
+        asked.append((i, len(out)))
+        assert eos not in out
+        return None
+
+    got = eng.generate_paged(p, max_new_tokens=8, allowed_tokens=allowed)
+    for ids, r in zip(free, got):
+        n = ids.index(eos) + 1 if eos in ids else 8
+        assert r.generated_ids == ids[:n]
+    assert max(n for i, n in asked if i == 1) == free[1].index(eos)
+    assert eng.generate_paged(p, max_new_tokens=0)[2].generated_ids == free[2][:1]
+    assert eng.allocator.free_blocks == 64 - eng.chunk_mapper.blocks_used_by_chunks()
+
+
+@pytest.mark.parametrize("n", [33, 48, 49, 97, 128, 129, 144, 145])
+def test_reuse_that_ends_at_and_around_block_borders(n):
+    """The prompt's chunks cached or not, its last token runs again: the same tokens, within the
+    pool's blocks (the status word stays clear)."""
+    from kvboost_b200.paged_engine import PagedEngine
+    m = _model()
+    p = _prompts([n], 0, seed=n)
+    eng = PagedEngine(m, num_blocks=2 * -(-(n + 17) // 16) + 1, recompute_strategy="none")
+    eng.warm(p[0])
+    for _ in range(2):
+        r = eng.generate_paged(p, max_new_tokens=17)[0]
+        keys, values, cached, _ = eng._assemble(p[0])
+        assert r.cached_tokens == cached
+        _check_greedy(m, p[0], min(cached, n - 1), keys, values, r.generated_ids)
