@@ -251,19 +251,24 @@ __device__ __forceinline__ void from_f32(float* p, float x) { *p = x; }
 __device__ __forceinline__ void from_f32(__half* p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void from_f32(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-// Eight consecutive values as they are stored, and as float32.
-template <typename T>
+// A thread's eight values of a turn as they are stored, and as float32: STEP apart from p, left
+// of them before the slice's end.  STEP 1, in rows on 16 bytes, moves 16 bytes at a time; STEP 32
+// lets a warp's lanes lie side by side, value by value.
+template <typename T, int STEP>
 struct Eight {
   static constexpr int N = sizeof(T) / 2;
   uint4 raw[N];
-  __device__ __forceinline__ void load(const T* p, bool wide, int left) {
-    if (wide && left >= 8) {
+  __device__ __forceinline__ void load(const T* p, int left) {
+    if (STEP == 1 && left >= 8) {
 #pragma unroll
       for (int i = 0; i < N; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
     } else {
       T h[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) from_f32(h + k, k < left ? to_f32(p[k]) : 0.f);
+      for (int k = 0; k < 8; ++k) {
+        from_f32(h + k, 0.f);
+        if (k * STEP < left) h[k] = __ldcs(p + k * STEP);
+      }
       memcpy(raw, h, sizeof(raw));
     }
   }
@@ -273,11 +278,11 @@ struct Eight {
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = to_f32(h[k]);
   }
-  static __device__ __forceinline__ void store(T* p, const float (&x)[8], bool wide, int left) {
+  static __device__ __forceinline__ void store(T* p, const float (&x)[8], int left) {
     T h[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) from_f32(h + k, x[k]);
-    if (wide && left >= 8) {
+    if (STEP == 1 && left >= 8) {
       uint4 v[N];
       memcpy(v, h, sizeof(v));
 #pragma unroll
@@ -285,7 +290,7 @@ struct Eight {
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (k < left) p[k] = h[k];
+        if (k * STEP < left) p[k * STEP] = h[k];
     }
   }
 };
@@ -304,9 +309,9 @@ constexpr int kCounts16 = 16383;          // the longest history that a 16-bit n
 // stream it took 124 us for 192 rows of 151936, waiting for instructions; with 32-bit notes
 // of shorter slices, all of a thread's logits in registers, 68 us; so 41 us.  The quotients by
 // the repetition penalty and the temperature are products with their reciprocals: one more
-// rounding of float32 each.  A row whose pointers or tail do not sit on 16 bytes goes value by
-// value.
-template <typename TI, typename TO, typename NT>
+// rounding of float32 each.  Rows that do not all sit on 16 bytes (odd vocabularies) take
+// STEP 32.
+template <typename TI, typename TO, typename NT, int STEP>
 __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) {
   constexpr int PER = 4 / sizeof(NT), BITS = 8 * sizeof(NT);   // notes a word, bits a note
   constexpr uint32_t kBias = 1u << (BITS - 1), kAll = BITS == 32 ? ~0u : 0xffffu;
@@ -319,15 +324,12 @@ __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) 
   const TI* in = static_cast<const TI*>(a.logits) + b * a.logits_stride;
   TO* out = static_cast<TO*>(a.out) + b * a.out_stride;
   const uint8_t* mask = a.mask ? reinterpret_cast<const uint8_t*>(a.mask + b * a.mask_stride) : nullptr;
-  const bool wide_in = (reinterpret_cast<uintptr_t>(in + v0) & 15) == 0;
-  const bool wide_out = (reinterpret_cast<uintptr_t>(out + v0) & 15) == 0;
-  int v = v0 + tid * 8;
-  Eight<TI> next;
+  // the thread's first token of a turn, and the first of the eight whose mask byte it loads
+  const int first = STEP == 1 ? tid * 8 : (tid & ~31) * 8 + (tid & 31), byte = tid * 8;
+  Eight<TI, STEP> next;
   uint32_t next_open = 0xff;
-  if (v < v1) {
-    next.load(in + v, wide_in, v1 - v);
-    if (mask) next_open = mask[v >> 3];
-  }
+  next.load(in + v0 + first, v1 - v0 - first);
+  if (mask && v0 + byte < v1) next_open = mask[(v0 + byte) >> 3];
   const int32_t* bias_ids = a.bias_ids ? a.bias_ids + (int64_t)b * a.num_bias : nullptr;
   const float* bias_values = a.bias_values + (int64_t)b * a.num_bias;
   const int total = a.token_ids ? min(max(a.total_lens[b], 0), a.history_len) : 0;
@@ -396,20 +398,37 @@ __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) 
   const float pres = a.presence ? a.presence[b] : 0.f;
   const float inv = a.temperature ? 1.f / fmaxf(a.temperature[b], 1e-5f) : 1.f;
 #pragma unroll 1
-  for (; v < v1; v += 2048) {
+  for (int at0 = v0; at0 < v1; at0 += 2048) {
+    const int v = at0 + first;
     float x[8];
     next.values(x);
-    const uint32_t open = next_open;
-    if (v + 2048 < v1) {
-      next.load(in + v + 2048, wide_in, v1 - v - 2048);
-      if (mask) next_open = mask[(v + 2048) >> 3];
+    uint32_t open = next_open;
+    if (STEP == 32 && mask) {               // token v + 32 k's bit is bit lane % 8 of lane 4 k + lane / 8
+      uint32_t mine = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        mine |= ((__shfl_sync(~0u, next_open, 4 * k + (tid & 31) / 8) >> (tid & 7)) & 1) << k;
+      open = mine;
+    }
+    if (at0 + 2048 < v1) {
+      next.load(in + v + 2048, v1 - v - 2048);
+      if (mask && at0 + 2048 + byte < v1) next_open = mask[(at0 + 2048 + byte) >> 3];
     }
     if (noted) {
       uint32_t n[8 / PER];
+      if (STEP == 1) {
 #pragma unroll
-      for (int i = 0; i < 2 / PER; ++i) {
-        const uint4 q = reinterpret_cast<const uint4*>(note)[(v - v0) / 4 / PER + i];
-        n[4 * i] = q.x, n[4 * i + 1] = q.y, n[4 * i + 2] = q.z, n[4 * i + 3] = q.w;
+        for (int i = 0; i < 2 / PER; ++i) {
+          const uint4 q = reinterpret_cast<const uint4*>(note)[(v - v0) / 4 / PER + i];
+          n[4 * i] = q.x, n[4 * i + 1] = q.y, n[4 * i + 2] = q.z, n[4 * i + 3] = q.w;
+        }
+      } else {
+        const NT* one = reinterpret_cast<const NT*>(note) + (v - v0);
+#pragma unroll
+        for (int i = 0; i < 8 / PER; ++i) n[i] = one[i * PER * 32];
+        if (PER == 2)
+#pragma unroll
+          for (int i = 0; i < 8 / PER; ++i) n[i] |= (uint32_t)one[(i * PER + 1) * 32] << 16;
       }
       uint32_t any = 0;
 #pragma unroll
@@ -432,8 +451,8 @@ __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) 
           const int len = all ? list_len : a.num_bias;
 #pragma unroll 1
           for (int e = 0; e < len; ++e) {
-            const uint32_t at = (uint32_t)((all ? list_ids[e] : bias_ids[e]) - v);
-            if (at < 8) {
+            const uint32_t off = (uint32_t)((all ? list_ids[e] : bias_ids[e]) - v), at = off / STEP;
+            if (off % STEP == 0 && at < 8) {
               const float w = all ? list_values[e] : bias_values[e];
 #pragma unroll
               for (int k = 0; k < 8; ++k) x[k] += at == k ? w : 0.f;
@@ -444,7 +463,7 @@ __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) 
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = (open >> k) & 1 ? x[k] * inv : __uint_as_float(0xff800000u);
-    Eight<TO>::store(out + v, x, wide_out, v1 - v);
+    Eight<TO, STEP>::store(out + v, x, v1 - v);
   }
 }
 
@@ -455,10 +474,14 @@ void launch_logits(LogitsArgs a, int batch, cudaStream_t s) {
   for (a.iters = 4; a.iters > 1; a.iters /= 2)
     if ((int64_t)batch * ((a.vocab + a.iters * 2048 - 1) / (a.iters * 2048)) >= 4 * 148) break;
   const dim3 grid((a.vocab + a.iters * 2048 - 1) / (a.iters * 2048), batch);
-  if (a.history_len <= kCounts16)
-    kvb_logits_kernel<TI, TO, uint16_t><<<grid, 256, a.iters * 4096, s>>>(a);
-  else
-    kvb_logits_kernel<TI, TO, uint32_t><<<grid, 256, a.iters * 8192, s>>>(a);
+  const bool wide = aligned(a.logits, 16) && aligned(a.out, 16) &&
+                    (batch == 1 || (a.logits_stride * sizeof(TI) % 16 == 0 && a.out_stride * sizeof(TO) % 16 == 0));
+  const bool few = a.history_len <= kCounts16;
+  const int smem = a.iters * (few ? 4096 : 8192);
+  if (wide && few) kvb_logits_kernel<TI, TO, uint16_t, 1><<<grid, 256, smem, s>>>(a);
+  else if (wide) kvb_logits_kernel<TI, TO, uint32_t, 1><<<grid, 256, smem, s>>>(a);
+  else if (few) kvb_logits_kernel<TI, TO, uint16_t, 32><<<grid, 256, smem, s>>>(a);
+  else kvb_logits_kernel<TI, TO, uint32_t, 32><<<grid, 256, smem, s>>>(a);
 }
 
 }  // namespace kvb_step
