@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "kvb_attn.h"
 
@@ -70,7 +71,8 @@ __device__ __forceinline__ uint2 scan_sat(uint2 x, int lane) {
 // of each block that a token begins.
 // Latency is all there is: two dependent reads, a scan and the stores.  One cluster of up to
 // eight CTAs shares the tokens; every CTA scans for itself, and since the new lengths may go
-// over the old ones, no CTA writes before all have read.
+// over the old ones, no CTA writes before all have read.  8 rows of a token each: 4.1 us; 256 rows
+// of 43220 tokens 8.4 us, 38.7 with one CTA.
 __global__ void __launch_bounds__(1024) kvb_extend_tables_kernel(const TablesArgs a) {
   extern __shared__ int32_t sm[];
   int32_t* cu = sm;                        // [batch + 1] place of the row's tokens
@@ -251,30 +253,58 @@ __device__ __forceinline__ void from_f32(float* p, float x) { *p = x; }
 __device__ __forceinline__ void from_f32(__half* p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void from_f32(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-// A thread's eight values of a turn as they are stored, and as float32: STEP apart from p, left
-// of them before the slice's end.  STEP 1, in rows on 16 bytes, moves 16 bytes at a time; STEP 32
-// lets a warp's lanes lie side by side, value by value.
-template <typename T, int STEP>
+// A thread's eight values of a turn as they are stored, and as float32: G side by side, then the
+// next G 32 G further on; an access moves G values (G 1 needs no alignment).  left: from the first
+// value to the slice's end.  Whole 32-byte sectors a thread, or 16 bytes side by side over the
+// warp, are what the stores need: two 16-byte stores of float32, 32 bytes apart over the warp,
+// took 19.4 us for 150 rows of 100000 where these take 12.5.
+template <int G>
+__device__ __forceinline__ constexpr int place(int k) { return k / G * 32 * G + k % G; }
+
+struct alignas(32) Wide { uint32_t x[8]; };
+
+template <typename R>
+__device__ __forceinline__ R stream_in(const R* p) { return __ldcs(p); }
+template <typename R>
+__device__ __forceinline__ void stream_out(R* p, R v) { __stcs(p, v); }
+__device__ __forceinline__ Wide stream_in(const Wide* p) {
+  Wide v;
+  asm volatile("ld.global.L2::evict_first.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v.x[0]), "=r"(v.x[1]), "=r"(v.x[2]), "=r"(v.x[3]), "=r"(v.x[4]), "=r"(v.x[5]), "=r"(v.x[6]), "=r"(v.x[7])
+               : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void stream_out(Wide* p, Wide v) {
+  asm volatile("st.global.L2::evict_first.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v.x[0]), "r"(v.x[1]),
+               "r"(v.x[2]), "r"(v.x[3]), "r"(v.x[4]), "r"(v.x[5]), "r"(v.x[6]), "r"(v.x[7]) : "memory");
+}
+
+template <typename T, int G>
 struct Eight {
-  static constexpr int N = sizeof(T) / 2;
-  uint4 raw[N];
+  static constexpr int B = G * sizeof(T);
+  using Run = typename std::conditional<B == 32, Wide, typename std::conditional<B == 16, uint4,
+              typename std::conditional<B == 8, uint2, T>::type>::type>::type;
+  Run run[8 / G];
   __device__ __forceinline__ void load(const T* p, int left) {
-    if (STEP == 1 && left >= 8) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-    } else {
-      T h[8];
+    for (int i = 0; i < 8 / G; ++i) {
+      const T* q = p + place<G>(i * G);
+      if (place<G>(i * G + G - 1) < left) {
+        run[i] = stream_in(reinterpret_cast<const Run*>(q));
+      } else {
+        T h[G];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        from_f32(h + k, 0.f);
-        if (k * STEP < left) h[k] = __ldcs(p + k * STEP);
+        for (int k = 0; k < G; ++k) {
+          from_f32(h + k, 0.f);
+          if (place<G>(i * G + k) < left) h[k] = q[k];
+        }
+        memcpy(&run[i], h, sizeof(Run));
       }
-      memcpy(raw, h, sizeof(raw));
     }
   }
   __device__ __forceinline__ void values(float (&x)[8]) const {
     T h[8];
-    memcpy(h, raw, sizeof(raw));
+    memcpy(h, run, sizeof(run));
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = to_f32(h[k]);
   }
@@ -282,15 +312,18 @@ struct Eight {
     T h[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) from_f32(h + k, x[k]);
-    if (STEP == 1 && left >= 8) {
-      uint4 v[N];
-      memcpy(v, h, sizeof(v));
 #pragma unroll
-      for (int i = 0; i < N; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, v[i]);
-    } else {
+    for (int i = 0; i < 8 / G; ++i) {
+      T* q = p + place<G>(i * G);
+      if (place<G>(i * G + G - 1) < left) {
+        Run v;
+        memcpy(&v, h + i * G, sizeof(v));
+        stream_out(reinterpret_cast<Run*>(q), v);
+      } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k * STEP < left) p[k * STEP] = h[k];
+        for (int k = 0; k < G; ++k)
+          if (place<G>(i * G + k) < left) q[k] = h[i * G + k];
+      }
     }
   }
 };
@@ -301,17 +334,21 @@ constexpr int kCounts16 = 16383;          // the longest history that a 16-bit n
 // A CTA takes one slice of a row.  It notes the history's tokens that fall into the slice in
 // shared memory (per token a seen bit, a count and a bias bit, in 16 bits, or 32 for long
 // histories; integer adds: any order gives the same) and the slice's bias entries in their
-// order, then streams the slice, 2048 tokens a turn, 8 a thread, 16 bytes at a time, the next
-// turn's logits on their way.  Byte work for large batches: the logits once, the result once;
-// the history is read by every slice's CTA (from L2), so slices are long there, and short
-// (2048) where few rows have to spread over the GPU.  The stream's own work has to stay small
-// beside 6 bytes a token: with the penalties' divisions and the bias list in the unrolled
-// stream it took 124 us for 192 rows of 151936, waiting for instructions; with 32-bit notes
-// of shorter slices, all of a thread's logits in registers, 68 us; so 41 us.  The quotients by
-// the repetition penalty and the temperature are products with their reciprocals: one more
-// rounding of float32 each.  Rows that do not all sit on 16 bytes (odd vocabularies) take
-// STEP 32.
-template <typename TI, typename TO, typename NT, int STEP>
+// order, then streams the slice, 2048 tokens a turn, 8 a thread, the next turn's logits on their
+// way.  Byte work for large batches: the logits once, the result once; the history is read by
+// every slice's CTA (from L2), so slices are long there, and short (2048) where few rows have to
+// spread over the GPU.  The stream's own work has to stay small beside 6 bytes a token: with the
+// penalties' divisions and the bias list in the unrolled stream it took 124 us for 192 rows of
+// 151936, waiting for instructions; with 32-bit notes of shorter slices, all of a thread's logits
+// in registers, 68 us; so 37.4 us (4.8 TB/s; 28 us and 6.3 TB/s with the mask alone), what the
+// notes cost being the two barriers with the wait for the history before the first turn, and the
+// branches of noted tokens.  A list of the noted tokens, worked on behind the stream, took
+// longer (45 us).  The quotients by the repetition penalty and the temperature are products with
+// their reciprocals: one more rounding of float32 each.
+//
+// G 8: rows on 8 values.  G 4: rows on 4 without notes (12.5 us for 150 rows of 100000, 13.5 with
+// G 8).  G 1: other rows, odd vocabularies (150 of 100001: 25.4 us with notes, 18.8 for 100000).
+template <typename TI, typename TO, typename NT, int G>
 __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) {
   constexpr int PER = 4 / sizeof(NT), BITS = 8 * sizeof(NT);   // notes a word, bits a note
   constexpr uint32_t kBias = 1u << (BITS - 1), kAll = BITS == 32 ? ~0u : 0xffffu;
@@ -325,24 +362,28 @@ __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) 
   TO* out = static_cast<TO*>(a.out) + b * a.out_stride;
   const uint8_t* mask = a.mask ? reinterpret_cast<const uint8_t*>(a.mask + b * a.mask_stride) : nullptr;
   // the thread's first token of a turn, and the first of the eight whose mask byte it loads
-  const int first = STEP == 1 ? tid * 8 : (tid & ~31) * 8 + (tid & 31), byte = tid * 8;
-  Eight<TI, STEP> next;
+  const int first = (tid & ~31) * 8 + (tid & 31) * G, byte = tid * 8;
+  Eight<TI, G> next;
   uint32_t next_open = 0xff;
   next.load(in + v0 + first, v1 - v0 - first);
   if (mask && v0 + byte < v1) next_open = mask[(v0 + byte) >> 3];
+  const float r = a.repetition ? a.repetition[b] : 1.f;
+  const float freq = a.frequency ? a.frequency[b] : 0.f;
+  const float pres = a.presence ? a.presence[b] : 0.f;
+  const float heat = a.temperature ? fmaxf(a.temperature[b], 1e-5f) : 1.f;
   const int32_t* bias_ids = a.bias_ids ? a.bias_ids + (int64_t)b * a.num_bias : nullptr;
   const float* bias_values = a.bias_values + (int64_t)b * a.num_bias;
-  const int total = a.token_ids ? min(max(a.total_lens[b], 0), a.history_len) : 0;
-  const bool noted = total > 0 || bias_ids;
+  const bool noted = G != 4 && (a.token_ids || bias_ids);
   if (noted) {
-    // the first 2048 of the history and 64 of the bias list are on their way while the notes
-    // are cleared
-    const int prompt = a.prompt_lens ? min(max(a.prompt_lens[b], 0), total) : 0;
+    // The first 2048 of the history (before its length is known) and 64 of the bias list are
+    // on their way while the notes are cleared.
     const int32_t* ids = a.token_ids + b * a.history_stride;
+    const int room = a.token_ids ? a.history_len : 0;
+    int total = a.token_ids ? a.total_lens[b] : 0, prompt = a.token_ids && a.prompt_lens ? a.prompt_lens[b] : 0;
     int id[8], bias_id[2] = {-1, -1};
     float bias_value[2] = {0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) id[k] = tid + k * 256 < total ? ids[tid + k * 256] : -1;
+    for (int k = 0; k < 8; ++k) id[k] = tid + k * 256 < room ? ids[tid + k * 256] : -1;
     if (bias_ids && tid < 32)
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -352,11 +393,13 @@ __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) 
         }
     for (int i = tid; i < a.iters * 512 / PER; i += 256) reinterpret_cast<uint4*>(note)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
+    total = min(max(total, 0), room);
+    prompt = min(prompt, total);
     for (int i = tid; i < total; i += 8 * 256) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const uint32_t at = (uint32_t)id[k] - (uint32_t)v0, shift = (at % PER) * BITS;
-        if (id[k] >= 0 && at < (uint32_t)(v1 - v0)) {
+        if (i + k * 256 < total && id[k] >= 0 && at < (uint32_t)(v1 - v0)) {
           if (i + k * 256 < prompt) atomicOr(&note[at / PER], 1u << shift);
           else atomicAdd(&note[at / PER], 2u << shift);
         }
@@ -393,22 +436,22 @@ __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) 
     }
     __syncthreads();
   }
-  const float r = a.repetition ? a.repetition[b] : 1.f, ir = 1.f / r;
-  const float freq = a.frequency ? a.frequency[b] : 0.f;
-  const float pres = a.presence ? a.presence[b] : 0.f;
-  const float inv = a.temperature ? 1.f / fmaxf(a.temperature[b], 1e-5f) : 1.f;
+  const float ir = 1.f / r, inv = 1.f / heat;
 #pragma unroll 1
   for (int at0 = v0; at0 < v1; at0 += 2048) {
     const int v = at0 + first;
     float x[8];
     next.values(x);
-    uint32_t open = next_open;
-    if (STEP == 32 && mask) {               // token v + 32 k's bit is bit lane % 8 of lane 4 k + lane / 8
-      uint32_t mine = 0;
+    uint32_t open = 0xff;
+    if (G == 8) {
+      open = next_open;
+    } else if (mask) {                      // from the lanes that hold the bytes
+      open = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        mine |= ((__shfl_sync(~0u, next_open, 4 * k + (tid & 31) / 8) >> (tid & 7)) & 1) << k;
-      open = mine;
+      for (int i = 0; i < 8 / G; ++i) {
+        const int bit = place<G>(i * G) + (tid & 31) * G;
+        open |= ((__shfl_sync(~0u, next_open, bit / 8) >> (bit % 8)) & ((1u << G) - 1)) << (i * G);
+      }
     }
     if (at0 + 2048 < v1) {
       next.load(in + v + 2048, v1 - v - 2048);
@@ -416,19 +459,15 @@ __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) 
     }
     if (noted) {
       uint32_t n[8 / PER];
-      if (STEP == 1) {
-#pragma unroll
-        for (int i = 0; i < 2 / PER; ++i) {
-          const uint4 q = reinterpret_cast<const uint4*>(note)[(v - v0) / 4 / PER + i];
-          n[4 * i] = q.x, n[4 * i + 1] = q.y, n[4 * i + 2] = q.z, n[4 * i + 3] = q.w;
-        }
+      const NT* one = reinterpret_cast<const NT*>(note) + (v - v0);
+      if (G == 8) {
+        memcpy(n, __builtin_assume_aligned(one, 16), sizeof(n));
       } else {
-        const NT* one = reinterpret_cast<const NT*>(note) + (v - v0);
 #pragma unroll
-        for (int i = 0; i < 8 / PER; ++i) n[i] = one[i * PER * 32];
-        if (PER == 2)
-#pragma unroll
-          for (int i = 0; i < 8 / PER; ++i) n[i] |= (uint32_t)one[(i * PER + 1) * 32] << 16;
+        for (int i = 0; i < 8 / PER; ++i) {
+          n[i] = one[place<G>(i * PER)];
+          if (PER == 2) n[i] |= (uint32_t)one[place<G>(i * PER + 1)] << 16;
+        }
       }
       uint32_t any = 0;
 #pragma unroll
@@ -451,8 +490,9 @@ __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) 
           const int len = all ? list_len : a.num_bias;
 #pragma unroll 1
           for (int e = 0; e < len; ++e) {
-            const uint32_t off = (uint32_t)((all ? list_ids[e] : bias_ids[e]) - v), at = off / STEP;
-            if (off % STEP == 0 && at < 8) {
+            const uint32_t off = (uint32_t)((all ? list_ids[e] : bias_ids[e]) - v);
+            const uint32_t at = off / (32 * G) * G + off % (32 * G);
+            if (off < 256 && off % (32 * G) < G) {
               const float w = all ? list_values[e] : bias_values[e];
 #pragma unroll
               for (int k = 0; k < 8; ++k) x[k] += at == k ? w : 0.f;
@@ -463,25 +503,29 @@ __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) 
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = (open >> k) & 1 ? x[k] * inv : __uint_as_float(0xff800000u);
-    Eight<TO, STEP>::store(out + v, x, v1 - v);
+    Eight<TO, G>::store(out + v, x, v1 - v);
   }
 }
 
 template <typename TI, typename TO>
 void launch_logits(LogitsArgs a, int batch, cudaStream_t s) {
-  // Slices of up to 8192 tokens, as long as every SM gets four CTAs (192 x 151936: 41.2 us with
-  // 8192, 44.0 with 16384, 47.0 with 4096; one row: 3.9 us with 2048, 19 CTAs of 8192 5.4).
-  for (a.iters = 4; a.iters > 1; a.iters /= 2)
-    if ((int64_t)batch * ((a.vocab + a.iters * 2048 - 1) / (a.iters * 2048)) >= 4 * 148) break;
+  // Slices of up to 8192 tokens, as long as every SM gets two CTAs (192 x 151936: 34.7 us with
+  // 8192, 38.9 with 16384, 38.7 with 4096; 16 x 128000: 5.1 us with 4096, 6.5 with 2048, 5.8 with
+  // 8192), 4096 without notes (192 x 151936: 28.3 us, 29.7 with 8192).
+  for (a.iters = a.token_ids || a.bias_ids ? 4 : 2; a.iters > 1; a.iters /= 2)
+    if ((int64_t)batch * ((a.vocab + a.iters * 2048 - 1) / (a.iters * 2048)) >= 2 * 148) break;
   const dim3 grid((a.vocab + a.iters * 2048 - 1) / (a.iters * 2048), batch);
-  const bool wide = aligned(a.logits, 16) && aligned(a.out, 16) &&
-                    (batch == 1 || (a.logits_stride * sizeof(TI) % 16 == 0 && a.out_stride * sizeof(TO) % 16 == 0));
+  const auto on = [&](int n) {            // every row on n values
+    return aligned(a.logits, n * sizeof(TI)) && aligned(a.out, n * sizeof(TO)) &&
+           (batch == 1 || (a.logits_stride % n == 0 && a.out_stride % n == 0));
+  };
   const bool few = a.history_len <= kCounts16;
   const int smem = a.iters * (few ? 4096 : 8192);
-  if (wide && few) kvb_logits_kernel<TI, TO, uint16_t, 1><<<grid, 256, smem, s>>>(a);
-  else if (wide) kvb_logits_kernel<TI, TO, uint32_t, 1><<<grid, 256, smem, s>>>(a);
-  else if (few) kvb_logits_kernel<TI, TO, uint16_t, 32><<<grid, 256, smem, s>>>(a);
-  else kvb_logits_kernel<TI, TO, uint32_t, 32><<<grid, 256, smem, s>>>(a);
+  if (!a.token_ids && !a.bias_ids && on(4)) kvb_logits_kernel<TI, TO, uint16_t, 4><<<grid, 256, 0, s>>>(a);
+  else if (few && on(8)) kvb_logits_kernel<TI, TO, uint16_t, 8><<<grid, 256, smem, s>>>(a);
+  else if (few) kvb_logits_kernel<TI, TO, uint16_t, 1><<<grid, 256, smem, s>>>(a);
+  else if (on(8)) kvb_logits_kernel<TI, TO, uint32_t, 8><<<grid, 256, smem, s>>>(a);
+  else kvb_logits_kernel<TI, TO, uint32_t, 1><<<grid, 256, smem, s>>>(a);
 }
 
 }  // namespace kvb_step
