@@ -510,7 +510,11 @@ def _check_logits(got, want, c, dtype):
         n = c["bias_values"].shape[1]
     if c.get("temperature") is not None:
         mag = mag / np.maximum(c["temperature"].numpy(), 1e-5)[:, None]
-    bound = (6 + n) * U * mag + torch.finfo(dtype).eps / 2 * np.abs(np.where(fin, want, 0)) + 1e-38
+    # below the smallest normal number values are spaced eps * smallest_normal (float16: 2^-24
+    # below 2^-14), so the last rounding is off by up to half of that however small the value is:
+    # float16(-2.7018e-5) is 1.74e-8 off, more than 2^-11 of it (1.32e-8), less than 2^-25
+    info = torch.finfo(dtype)
+    bound = (6 + n) * U * mag + info.eps / 2 * (np.abs(np.where(fin, want, 0)) + info.smallest_normal) + 1e-38
     assert (np.abs(np.where(fin, got, 0) - np.where(fin, want, 0)) <= bound).all()
 
 
@@ -539,6 +543,44 @@ def test_process_logits(dtype, B, V, L, N):
     assert process_logits(**d, out=d["logits"]) is d["logits"]
     _check_logits(d["logits"], want, c, dtype)
     assert (wide[:, :3] == 7).all() and (wide[:, 3 + V:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B,V,pad", [(1, 5, 0), (5, 4100, 0), (5, 4096, 4), (3, 8191, 1), (150, 10004, 0),
+                                     (150, 10000, 8), (40, 33000, 2)])
+def test_process_logits_without_history(dtype, B, V, pad):
+    """Mask and temperature alone, rows on 8, 4 or single values, a new result and in place."""
+    from kvboost_b200.logits import process_logits
+    c = _logits_case(B, V, 0, 0, dtype, V + pad)
+    want = _oracle_logits(c)
+    d = {k: t.cuda() for k, t in c.items()}
+    wide = torch.full((B, V + pad), 7.0, dtype=dtype, device=DEV)
+    wide[:, :V] = d["logits"]
+    d["logits"] = wide[:, :V]
+    _check_logits(process_logits(**d), want, c, torch.float32)
+    for drop in ("allowed_mask", "temperature"):
+        c2 = {k: t for k, t in c.items() if k != drop}
+        _check_logits(process_logits(**{k: d[k] for k in c2}), _oracle_logits(c2), c2, torch.float32)
+    process_logits(**d, out=d["logits"])
+    _check_logits(d["logits"], want, c, dtype)
+    assert (wide[:, V:] == 7).all()
+
+
+@pytest.mark.parametrize("V", [4104, 4100, 4101])
+def test_process_logits_same_for_every_alignment(V):
+    """Rows on 8, 4 or single values, counted in 16 and in 32 bits: the
+    same bits as the same rows one by one on their own."""
+    from kvboost_b200.logits import process_logits
+    c = _logits_case(6, V, 700, 9, torch.bfloat16, V)
+    d = {k: t.cuda() for k, t in c.items()}
+    got = process_logits(**d)
+    one = torch.cat([process_logits(**{k: t[b:b + 1].clone() for k, t in d.items()}) for b in range(6)])
+    assert torch.equal(got, one)
+    long = torch.full((6, 17000), -1, dtype=torch.int32, device=DEV)
+    long[:, :700] = d["token_ids"]
+    # the lengths stay, so the longer buffer changes the counters' width alone
+    lens = {k: d[k].clamp(max=700) for k in ("total_lens", "prompt_lens")}
+    assert torch.equal(got, process_logits(**{**d, "token_ids": long, **lens}))
 
 
 def test_process_logits_captured():
