@@ -19,7 +19,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .paged_decode import _check_int32, _launch
+from .paged_decode import _allocator, _check_int32, _launch
 
 _LOGIT_DTYPES = {torch.bfloat16: _lib.KVB_DTYPE_BF16, torch.float16: _lib.KVB_DTYPE_FP16,
                  torch.float32: _lib.KVB_DTYPE_FP32}
@@ -70,7 +70,7 @@ def process_logits(logits: torch.Tensor, token_ids: Optional[torch.Tensor] = Non
     if V < 1 or (logits.stride(1) != 1 and V > 1):
         raise RuntimeError("logits must have contiguous, non-empty rows")
     if out is None:
-        out = logits.new_empty(B, V, dtype=torch.float32)
+        out = _allocator(dev)((B, V), (V, 1), torch.float32)
     elif out.shape != logits.shape or out.device != dev or (out.stride(1) != 1 and V > 1) \
             or out.dtype not in (torch.float32, logits.dtype):
         raise RuntimeError("out must be float32 or the logits' dtype, of their shape and device, "

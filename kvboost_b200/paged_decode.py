@@ -29,14 +29,24 @@ BLOCK_SIZE = 16
 
 # A decode step calls these operators once per layer, so the host's cost per call is kept
 # to a few checks: the stream handle comes from torch's C binding (2 us less than building a
-# Stream object), the device is switched only where it differs.
+# Stream object), results from its allocation of a strided tensor on the current device
+# (0.8 us, ``new_empty`` 1.3 to 1.5), the device is switched only where it differs.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_empty_strided = torch._C._dynamo.guards._empty_strided_cuda
+
+
+def _allocator(device):
+    """``f(shape, strides, dtype)``: a new tensor on the device."""
+    if _current_device() == device.index:
+        return _empty_strided
+    return lambda shape, strides, dtype: torch.empty_strided(shape, strides, dtype=dtype, device=device)
 
 
 def _launch(fn, params, device, what: str) -> None:
     """One library call on the device's current stream."""
     idx = device.index
-    if torch.cuda.current_device() == idx:
+    if _current_device() == idx:
         rc = fn(params, _raw_stream(idx))
     else:
         with torch.cuda.device(device):
@@ -122,8 +132,9 @@ def extend_block_tables(block_tables: torch.Tensor, seq_lens: torch.Tensor,
     if T < 0:
         raise RuntimeError("max_new_tokens must be >= 0")
     # the int32 results share one allocation: slots first (16-byte aligned)
-    slots, cu, lens_out, free_out = seq_lens.new_empty(T + 2 * B + 2).split_with_sizes((T, B + 1, B, 1))
-    positions = seq_lens.new_empty(T, dtype=torch.int64)
+    new = _allocator(dev)
+    slots, cu, lens_out, free_out = new((T + 2 * B + 2,), (1,), torch.int32).split_with_sizes((T, B + 1, B, 1))
+    positions = new((T,), (1,), torch.int64)
     if seq_lens_out is None:
         seq_lens_out = lens_out
     else:
@@ -252,15 +263,16 @@ def paged_decode_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_tables:
         softmax_scale = 1.0 / math.sqrt(D)
     if max_seq_len is not None and not 0 <= max_seq_len < 1 << 31:
         raise RuntimeError(f"max_seq_len must be in [0, 2^31), got {max_seq_len}")
+    new = _allocator(dev)
     if out is None:
-        out = q.new_empty(B, Hq, 1, D)
         ob, oh = Hq * D, D
+        out = new((B, Hq, 1, D), (ob, D, D, 1), dtype)
     else:
         ob, oh = out.stride()[:2] if out.dim() == 4 else (1, 1)
         if out.shape != q.shape or out.dtype != dtype or out.device != dev or out.stride(3) != 1 \
                 or ob % 8 or oh % 8 or out.data_ptr() % 16:
             raise RuntimeError("out must match q in shape, dtype and device, with 16-byte aligned heads")
-    lse = q.new_empty(B, Hq, 1, dtype=torch.float32) if return_lse else None
+    lse = new((B, Hq, 1), (Hq, 1, 1), torch.float32) if return_lse else None
     if B == 0:
         return out, lse
     qb, qh, _, _ = q.stride()
@@ -277,7 +289,7 @@ def paged_decode_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_tables:
     if need > 0:
         # partial results of this call: torch's caching allocator orders their reuse on the
         # current stream, so calls on concurrent streams never share them
-        ws = q.new_empty(need, dtype=torch.uint8)
+        ws = new((need,), (1,), torch.uint8)
         p = _lib.pack_paged_decode(*fields, ws.data_ptr(), need)
     _launch(lib.kvb_paged_decode_fwd, p, dev, "kvb_paged_decode_fwd")
     return out, lse
