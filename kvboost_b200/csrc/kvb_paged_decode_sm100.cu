@@ -82,6 +82,10 @@ constexpr int kItemCost = 1;
 // all: one request of 32768 tokens, 1 KV head: 20.3 us on 148 CTAs, 13.7 on 64).
 constexpr int kMinUnits = 16;
 constexpr int kSpan = 64;
+// Most blocks of an item that a share's end does not cut (nor one longer than a share): 2368 items
+// of 64 tokens, D 128, took 24.8 us cut and joined, 18.3 whole (int8 27.2, 18.0), of 256 63.9 and
+// 53.8 (48.3, 42.6), of 512 104.9 and 99.8 (67.5, but 69.3 whole).
+constexpr int uncut_of(bool i8) { return i8 ? 16 : 32; }
 constexpr int kSplitRows = 8192;           // most rows of a split launch (prefix sums in shared memory)
 
 struct Args {
@@ -223,6 +227,7 @@ __device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity, int32_t
 template <int D, bool I8, int NT>
 struct Geo {
   static constexpr int WARPS = warps_of(D, I8, NT);
+  static constexpr int UNCUT = uncut_of(I8);
   static constexpr int THREADS = WARPS * 32;
   static constexpr int NH = 8 * NT;                          // query heads per item
   static constexpr int HALVES = I8 ? 1 : (D + 63) / 64;      // TMA boxes per block
@@ -333,6 +338,12 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   int left;                     // what is left of this warp's share
   int u = 0, total = 0;         // split launch: the unit's place among all rows' units
   int ctas = 1;                 // split launch: CTAs that get units
+  int uncut = 0;                // split launch: items of up to so many blocks stay whole
+  // What is left of a share at an item's first block: an item that the share's end would cut
+  // belongs to the warp that has the larger part.
+  const auto whole = [&](int left, int nb) {
+    return left > 0 && left < nb && nb <= uncut ? (2 * left >= nb ? nb : 0) : left;
+  };
   if constexpr (SPLIT) {
     // A row weighs its blocks and kItemCost for each of its items; the weights laid end to end
     // are shared out, so u and left count places, of which an item's first nb are its blocks.
@@ -361,6 +372,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
         const Shares sh(total, ctas * kWarps);
         u = sh.first(me);
         left = sh.first(me + 1) - u;
+        uncut = min(G::UNCUT, sh.q);
       }
     };
     if (a.batch <= 32) {                            // every warp for itself, a row a lane
@@ -432,7 +444,12 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
       j = rel / weight;
       blk = rel - j * weight;
       nb = weight - kItemCost;
-      if (blk >= nb) {                              // between two items: on to the next
+      if (blk > 0 && 2 * blk < nb && nb <= uncut) { // the item is this warp's from its start
+        u -= blk;
+        left += blk;
+        blk = 0;
+      }
+      if (blk >= nb || (blk > 0 && nb <= uncut)) {  // between two items, or the one before's: on to the next
         const int skip = weight - blk;
         blk = 0;
         u += skip;
@@ -442,6 +459,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
           do { nb = (row_len(a, ++b) + 15) >> 4; } while (nb == 0);
         }
       }
+      if (blk == 0) left = whole(left, nb);
     }
   } else {
     b = blockIdx.x / a.items;
@@ -503,6 +521,10 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
       if (++pj == a.items) {
         pj = 0;
         do { pnb = (row_len(a, ++pb) + 15) >> 4; } while (pnb == 0);
+      }
+      if constexpr (SPLIT) {
+        to_issue = whole(to_issue, pnb);
+        if (to_issue == 0) return;
       }
       pkv = a.tiles == 1 ? pj : pj / a.tiles;
       // the item's query heads will be wanted NS blocks from now
@@ -569,6 +591,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
   bool alive = true, fetched = false;
   while (left > 0 && alive) {
     // one item, or the part of it in this warp's range
+    if (SPLIT && blk == 0 && (left = whole(left, nb)) == 0) break;
     const int kvh = a.tiles == 1 ? j : j / a.tiles;
     const int h0 = kvh * a.group + (j - kvh * a.tiles) * NH;
     const int heads = min(NH, (kvh + 1) * a.group - h0);

@@ -421,6 +421,23 @@ def test_paged_decode_batch_sizes(pool_kind, B, longest):
     _check_attention(o, lse, q, pool, tables, ln, 0.125, ks, vs)
 
 
+@pytest.mark.parametrize("pool_kind", ["same", "int8"])
+@pytest.mark.parametrize("B,H,group,D,longest", [(300, 8, 1, 64, 300), (200, 16, 2, 128, 160), (90, 20, 9, 64, 700)])
+def test_paged_decode_many_short_items(pool_kind, B, H, group, D, longest):
+    """More items than warps: a share's end leaves an item that is short enough whole, with one
+    warp or the next, and cuts the others; idle rows, one-token rows and one long row among them."""
+    g = torch.Generator().manual_seed(B + D)
+    ln = torch.randint(1, longest + 1, (B,), generator=g)
+    ln[::17] = 1
+    ln[::23] = 0
+    ln[B // 2] = 6000
+    ln = ln.tolist()
+    pool, tables, ks, vs = _pool(g, ln, H, D, torch.float16, pool_kind == "int8")
+    q = torch.randn(B, H * group, 1, D, generator=g).to(torch.float16)
+    o, lse = _attend(q, pool, tables, ln, ks, vs)
+    _check_attention(o, lse, q, pool, tables, ln, D ** -0.5, ks, vs)
+
+
 @pytest.mark.parametrize("ln", [[50, 20], [5000, 3000, 9]])
 def test_paged_decode_over_its_own_query(ln):
     """out=q: the output takes the query's place."""
