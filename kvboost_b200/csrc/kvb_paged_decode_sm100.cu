@@ -82,9 +82,13 @@ constexpr int kItemCost = 1;
 // all: one request of 32768 tokens, 1 KV head: 20.3 us on 148 CTAs, 13.7 on 64).
 constexpr int kMinUnits = 16;
 constexpr int kSpan = 64;
-// Most blocks of an item that a share's end does not cut (nor one longer than a share): 2368 items
-// of 64 tokens, D 128, took 24.8 us cut and joined, 18.3 whole (int8 27.2, 18.0), of 256 63.9 and
-// 53.8 (48.3, 42.6), of 512 104.9 and 99.8 (67.5, but 69.3 whole).
+// Most blocks of an item that a share's end does not cut, one warp taking all of it: kShort, more
+// where the shares are long enough for the uneven ends not to show (kShort 2 up to four shares,
+// uncut_of up to two).  D 128, cut and joined / whole: 640 items of 64 tokens 10.3 us / 7.3, of 256
+// 21.6 / 17.3 (8 heads 26.4 / 17.6); 2368 of 64 24.8 / 18.3 (int8 27.2 / 18.0), of 256 63.9 /
+// 53.8 (48.3 / 42.6), of 512 104.9 / 99.8 (67.5 / 69.3).  With shares of less than two blocks
+// the cut is better: 128 items of 256 tokens 12.8 / 15.7.
+constexpr int kShort = 8;
 constexpr int uncut_of(bool i8) { return i8 ? 16 : 32; }
 constexpr int kSplitRows = 8192;           // most rows of a split launch (prefix sums in shared memory)
 
@@ -372,7 +376,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
         const Shares sh(total, ctas * kWarps);
         u = sh.first(me);
         left = sh.first(me + 1) - u;
-        uncut = min(G::UNCUT, sh.q);
+        uncut = max(max(kShort, min(2 * kShort, 4 * sh.q)), min(G::UNCUT, 2 * sh.q));
       }
     };
     if (a.batch <= 32) {                            // every warp for itself, a row a lane
@@ -1096,9 +1100,9 @@ int64_t items(const KvbPagedDecodeParams* p) {
 // keeps its CTA for long, and very many items are as many starts.  What the host knows is the
 // table's width (or the caller's bound).  Measured, us per call (CTA per item / split), KV
 // heads x requests = items, D 128, 16 bits: 2 items of 256 tokens 5.1 / 7.7, of 1024 9.2 / 8.0,
-// of 2048 15.0 / 8.9; 32 of 1024 9.8 / 10.7; 128 of 2048 25.1 / 31.3; 512 of 64 13.7 / 15.3, of
-// 2048 85.7 / 95.9; 2048 of 64 54.5 / 26.4, of 256 73.0 / 62.7, of 1024 164 / 188.  int8: 256 of
-// 1024 25.0 / 26.8; 512 of 256 27.1 / 22.8, of 1024 45.6 / 41.0.
+// of 2048 15.0 / 8.9; 32 of 1024 9.7 / 12.4; 128 of 2048 25.0 / 31.5; 256 of 64 7.0 / 6.7, of 256
+// 12.9 / 15.9; 512 of 64 13.0 / 7.4, of 256 24.8 / 18.8, of 512 35.1 / 34.5, of 1024 51.8 / 54.2,
+// of 2048 84.9 / 93.5.  int8: 256 of 1024 24.9 / 26.6; 512 of 256 27.1 / 22.8, of 1024 45.6 / 41.5.
 bool split(const KvbPagedDecodeParams* p) {
   if (p->batch > kSplitRows) return false;
   // 32-bit places: wider than any pool
@@ -1107,7 +1111,7 @@ bool split(const KvbPagedDecodeParams* p) {
                             ? std::min<int64_t>(p->max_blocks_per_seq, ((int64_t)p->max_seq_len + 15) / 16)
                             : p->max_blocks_per_seq;
   const int64_t n = items(p);
-  if (n > (p->pool_format == KVB_POOL_INT8_KIVI ? 2 : 4) * kSms) return true;
+  if (n > (p->pool_format == KVB_POOL_INT8_KIVI || width <= 32 ? 2 : 4) * kSms) return true;
   return width > (n < 64 ? 64 : 128);
 }
 
