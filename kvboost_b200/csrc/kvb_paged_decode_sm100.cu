@@ -13,7 +13,8 @@
 // the lengths on the device, so ragged batches balance to a block without the host
 // knowing a length.  A warp walks its units alone: lane 0 brings each block's K and V
 // by TMA into the warp's ring of stages, several blocks ahead, through the block table;
-// no CTA-wide step sits in the loop.  Items that a warp holds whole it writes itself;
+// no CTA-wide step sits in the loop.  Items that a warp holds whole it writes itself
+// (short ones are left whole with one warp or the next, not cut);
 // the pieces at its range's ends are joined in shared memory at the CTA's end, and what
 // still spans CTAs goes to the workspace, where the CTA that finds all of an item's pieces
 // joins them.  Short tables take one CTA per item instead, whose warps split the item (split()
