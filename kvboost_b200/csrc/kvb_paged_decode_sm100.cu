@@ -26,15 +26,14 @@
 // P is carried in two 16-bit halves (p = hi + lo), so the weights keep 16 bits and the
 // result's error is that of its final rounding; the second MMA is free here.
 // KIVI int8 pools: a code is exact in float16 (as a subnormal, biased by 128; the bias leaves
-// through the accumulators' start), so Q (scaled by a power of two per row) and P are float16
-// and the scales act in float32 on S (K, per token) and on each block's product (V, per
-// channel): the dequantised values are never rounded.  Under bfloat16, whose output rounds by
-// 2^-8, P is one float16 number (2^-11) there.
+// through the accumulators' start), so Q (scaled by a power of two per row) and P's halves are
+// float16 and the scales act in float32 on S (K, per token) and on each block's product (V, per
+// channel): the dequantised values are never rounded.
 //
 // Measured (B200, us per call in a CUDA graph, of the measured 6.48 TB/s copy): 64 requests of
 // 700 .. 16381 tokens, 32/8 heads, D 128, bfloat16: 206 (6.3 TB/s, 97 %); 8 x 4096, 16/2 heads:
-// 14.4 (start, joins); int8 4 x 32768, 64/8 heads: 56.5 (5.1 TB/s, 78 %: the same compute-free, so
-// start and end of the one wave); 24 requests of 1 .. 2051 tokens, 32 heads of D 96, float16: 23.3
+// 14.4 (start, joins); int8 4 x 32768, 64/8 heads: 60.6 (4.7 TB/s, 73 %; 56.6 with the weights'
+// high halves alone, which under bfloat16 left 2.5 % of the outputs a step off); 24 requests of 1 .. 2051 tokens, 32 heads of D 96, float16: 23.3
 // (3.8 TB/s).
 
 #include <cuda_bf16.h>
@@ -311,8 +310,6 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     kvb_paged_decode_kernel(const __grid_constant__ CUtensorMap map, const Args a) {
   using G = Geo<D, I8, NT>;
   using E = typename std::conditional<I8, __half, T>::type;   // MMA operand type
-  // int8 pools under bfloat16: float16 weights (2^-11) are well below the output's own 2^-8
-  constexpr bool LOW = !(I8 && std::is_same<T, __nv_bfloat16>::value);
   constexpr int MT = D / 16, KS = D / 16, NS = G::NS, NH = G::NH;
   constexpr int kWarps = G::WARPS, kThreads = G::THREADS;
   extern __shared__ uint8_t smem_raw[];
@@ -764,7 +761,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
           const uint32_t hi = pack<E>(p[2 * h], p[2 * h + 1]);
           const float2 back = unpack<E>(hi);
           ph[t][h] = transpose8(hi);
-          if (LOW) pl[t][h] = transpose8(pack<E>(p[2 * h] - back.x, p[2 * h + 1] - back.y));
+          pl[t][h] = transpose8(pack<E>(p[2 * h] - back.x, p[2 * h + 1] - back.y));
         }
       }
       // O^T += V^T P^T
@@ -826,7 +823,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
         for (int t = 0; t < NT; ++t) {
           bias[t][0] = bias[t][1] = bias[t][2] = bias[t][3] = 0.f;
           mma<E>(bias[t], minus, ph[t][0], ph[t][1]);
-          if (LOW) mma<E>(bias[t], minus, pl[t][0], pl[t][1]);
+          mma<E>(bias[t], minus, pl[t][0], pl[t][1]);
         }
 #pragma unroll
         for (int w = 0; w < W; ++w) {
@@ -842,7 +839,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
             for (int t = 0; t < NT; ++t) {
               float o[4];
               mma_from(o, f, ph[t][0], ph[t][1], bias[t]);
-              if (LOW) mma<E>(o, f, pl[t][0], pl[t][1]);
+              mma<E>(o, f, pl[t][0], pl[t][1]);
               st.acc[t][jj][0] += z.x * o[0];
               st.acc[t][jj][1] += z.x * o[1];
               st.acc[t][jj][2] += z.y * o[2];
