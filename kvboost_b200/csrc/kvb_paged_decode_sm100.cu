@@ -22,7 +22,7 @@
 //
 // Arithmetic (per block, tokens on the MMA's rows, query heads on its columns):
 //   S^T = K Q^T; online softmax down the rows against a maximum that is raised only when
-//   a score passes it by 2^8 (one vote instead of shuffles); O^T += V^T P^T.
+//   a score passes it by 2^8 (float16: 2^4; one vote instead of shuffles); O^T += V^T P^T.
 // P is carried in two 16-bit halves (p = hi + lo), so the weights keep 16 bits and the
 // result's error is that of its final rounding; the second MMA is free here.
 // KIVI int8 pools: a code is exact in float16 (as a subnormal, biased by 128; the bias leaves
@@ -61,9 +61,13 @@ int fail(int code, const std::string& msg) { return kvb_detail_fail(code, msg); 
 
 constexpr int kSms = 148;
 constexpr uint64_t kWaitNs = 2000000000ull;
-// Log2 units that a score may pass the running maximum by before it is raised.  (0, raising at
-// every new maximum: int8 4 x 32768 tokens 56.9 us instead of 56.4.)
-constexpr float kRaise = 8.f;
+// Weights are exp2(x - m) with m kept kLift below the running maximum (log2 units), and m is raised
+// when a score passes m by kTop.  In bfloat16, with float32's exponents, that is a maximum raised
+// when it is passed by 2^8.  A float16 half has nothing below 2^-25, so there the weights lie as high
+// as 2^15 and the maximum's own at 2^11 or above: what is lost lies below 2^-36 of the largest (2^-25
+// without the lift: 2000 tokens of weight 2^-26 and V 60000 beside some of weight 1 were all lost).
+template <typename E> constexpr float kLift = std::is_same<E, __half>::value ? 11.f : 0.f;
+template <typename E> constexpr float kTop = std::is_same<E, __half>::value ? 15.f : 8.f;
 // Warps per CTA, as registers allow.  Items of up to 8 heads: 64 requests of 700 .. 16381 tokens in
 // bfloat16 took 211 us with 8 warps of three stages, 209 with 10, 206 with 12 of two; int8 4 x
 // 32768 tokens, 64/8 heads: 65.0 with 8, 63.4 with 10, 57.0 with 12, 60.6 with 14, 60.5 with 16
@@ -293,8 +297,15 @@ __device__ __forceinline__ float warp_max(float x) {
   return __int_as_float(top < 0 ? top ^ 0x7fffffff : top);
 }
 
-// Writes a joined head: lane i features 4 i .. 4 i + 3; top in log2 units.
-template <typename T, int D>
+// ln of the weights' sum: the lift leaves both exactly before the logarithm
+template <typename E>
+__device__ __forceinline__ float lse_of(float m, float sum) {
+  constexpr float unlift = 1.f / (1 << (int)kLift<E>);
+  return ((m == -INFINITY ? 0.f : m + kLift<E>) + log2f(sum * unlift)) * 0.6931471805599453f;
+}
+
+// Writes a joined head: lane i features 4 i .. 4 i + 3; top, kLift below the maximum, in log2 units.
+template <typename T, typename E, int D>
 __device__ __forceinline__ void write_head(const Args& a, int b, int head, int lane, const float4& o, float top,
                                            float sum) {
   const float inv = 1.f / sum;
@@ -302,7 +313,7 @@ __device__ __forceinline__ void write_head(const Args& a, int b, int head, int l
     *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + b * a.o_bs + (int64_t)head * a.o_hs + 4 * lane) =
         make_uint2(pack<T>(o.x * inv, o.y * inv), pack<T>(o.z * inv, o.w * inv));
   if (lane == 0 && a.lse)
-    a.lse[b * a.lse_bs + head] = ((top == -INFINITY ? 0.f : top) + log2f(sum)) * 0.6931471805599453f;
+    a.lse[b * a.lse_bs + head] = lse_of<E>(top, sum);
 }
 
 template <typename T, int D, bool I8, int NT, bool SPLIT>
@@ -723,7 +734,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
           v *= I8 ? qx[t][i & 1] * (i < 2 ? k0 : k1) : qx[t][i & 1];
           if (r + (i < 2 ? 0 : 8) >= valid) v = -INFINITY;
           x[t][i] = v;
-          raise |= v > st.m[t][i & 1] + kRaise;
+          raise |= v > st.m[t][i & 1] + kTop<E>;
         }
       if (__any_sync(~0u, raise)) {
 #pragma unroll
@@ -734,7 +745,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-            top = fmaxf(top, st.m[t][i]);
+            top = fmaxf(top - kLift<E>, st.m[t][i]);
             const float f = top == -INFINITY ? 1.f : ex2(st.m[t][i] - top);
             st.m[t][i] = top;
             st.l[t][i] *= f;
@@ -898,8 +909,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
             if (t * 8 + 2 * c + i < heads)
-              a.lse[b * a.lse_bs + h0 + t * 8 + 2 * c + i] =
-                  (st.m[t][i] + log2f(st.l[t][i])) * 0.6931471805599453f;
+              a.lse[b * a.lse_bs + h0 + t * 8 + 2 * c + i] = lse_of<E>(st.m[t][i], st.l[t][i]);
       }
     } else {
       // a piece: in the workspace, or at the end of the warp's range over its stages (every load
@@ -1015,7 +1025,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
         if (lane == pending) wait_for = make_int4(ib, ij | h << 24, c0, c1);
         ++pending;
       } else {
-        write_head<T, D>(a, ib, h0 + h, lane, o, top, sum);
+        write_head<T, E, D>(a, ib, h0 + h, lane, o, top, sum);
       }
     }
   }
@@ -1077,7 +1087,7 @@ __global__ void __launch_bounds__(Geo<D, I8, NT>::THREADS, 1)
     sum = __shfl_sync(~0u, sum, 0);
     for (int k = c0 + lane; k <= c1; k += 32) a.flags[(2 * k + (k == c0 ? 1 : 0)) * NH + h] = 0;
     const int kvh = a.tiles == 1 ? ij : ij / a.tiles;
-    write_head<T, D>(a, ib, kvh * a.group + (ij - kvh * a.tiles) * NH + h, lane, o, top, sum);
+    write_head<T, E, D>(a, ib, kvh * a.group + (ij - kvh * a.tiles) * NH + h, lane, o, top, sum);
   }
 }
 

@@ -67,3 +67,45 @@ def test_int8_weights_keep_their_bits(dtype, D, group):
     bound = np.maximum(_half_step(want, dtype), _half_step(got, dtype)) + off
     bad = np.abs(got - want) > bound
     assert not bad.any(), (bad.mean(), np.argwhere(bad)[:4], (np.abs(got - want) / bound).max())
+
+
+@pytest.mark.parametrize("dtype,int8", [(torch.float16, False), (torch.bfloat16, False), (torch.float16, True),
+                                        (torch.bfloat16, True)])
+@pytest.mark.parametrize("B,n,every", [(64, 2000, 160), (256, 8000, 1000)])
+def test_small_weights_are_kept(dtype, int8, B, n, every):
+    """Tokens of weight 2^-25.05, each below half of float16's smallest step, with large V beside a few
+    tokens of weight 1 and V 0: the result is their sum alone.  Scores as above (|x| 25.05: 2^-16 of
+    a, the exponential and subtraction included); in float16 halves 2^-36 of the largest weight may
+    be lost per token."""
+    from kvboost_b200.paged_decode import paged_decode_attention
+    D, nb = 64, n // 16
+    tail = torch.arange(n) % every != 0
+    pool = torch.zeros(nb, 2, 1, 16, D)
+    k = torch.where(tail, -127.0 if int8 else -25.046875, 0.0).view(nb, 16)
+    v = torch.where(tail, 127.0 if int8 else 60000.0, 0.0).view(nb, 16)
+    pool[:, 0, 0, :, 5] = k
+    pool[:, 1, 0] = v[..., None]
+    ks = vs = None
+    if int8:
+        pool = pool.to(torch.int8)
+        ks = torch.full((nb, 1, 16), 25.05 / 127).to(torch.float16)
+        vs = torch.full((nb, 1, D), 400.0).to(torch.float16)
+    else:
+        pool = pool.to(dtype)
+    q = torch.zeros(B, 1, 1, D)
+    q[..., 5] = 1.0
+    q = q.to(dtype)
+    tables = torch.arange(nb, dtype=torch.int32).repeat(B, 1)
+    c = lambda t: None if t is None else t.cuda()  # noqa: E731
+    f = lambda t: None if t is None else t.float().numpy()  # noqa: E731
+    o, lse = paged_decode_attention(q.cuda(), pool.cuda(), tables.cuda(),
+                                    torch.full((B,), n, dtype=torch.int32, device=DEV), c(ks), c(vs),
+                                    softmax_scale=math.log(2.0))
+    want, wl, a, _, vmax, _, _ = ostep.decode_attention(
+        f(q[:1, :, 0]), pool.numpy() if int8 else f(pool), tables[:1].numpy(), [n], math.log(2.0), f(ks), f(vs))
+    got = o[:, :, 0].double().cpu().numpy()
+    off = (2.0 ** -16 + 2 * n * 2.0 ** -24) * a + ((48 * 2.0 ** -24 if int8 else 0) + n * 2.0 ** -36) * vmax[..., None]
+    bound = np.maximum(_half_step(want, dtype), _half_step(got, dtype)) + off
+    assert (np.abs(got - want) <= bound).all(), (got.min(), got.max(), want.min(), want.max())
+    gl = lse[:, :, 0].double().cpu().numpy()
+    assert np.abs(gl - wl).max() <= 2.0 ** -18 + 2 * n * 2.0 ** -24
