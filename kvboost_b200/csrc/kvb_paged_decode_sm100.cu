@@ -218,12 +218,13 @@ __device__ __forceinline__ uint32_t codes_to_half(uint32_t biased, uint32_t sele
   return __byte_perm(biased, 0u, select);
 }
 
-// Waits for a phase; false after 2 s (the status word says so).
+// A warp's wait for a phase; false after 2 s (the status word says so).  The lanes vote at each look, so
+// all of them get one verdict: what follows is warp-wide.
 __device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity, int32_t* status) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (__all_sync(~0u, mbar_try_wait(bar, parity))) return true;
   const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, parity)) {
-    if (globaltimer_ns() - t0 > kWaitNs) {
+  while (!__all_sync(~0u, mbar_try_wait(bar, parity))) {
+    if (__any_sync(~0u, globaltimer_ns() - t0 > kWaitNs)) {
       if (status) atomicOr(status, KVB_STATUS_LOAD_WAIT);
       return false;
     }
