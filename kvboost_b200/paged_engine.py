@@ -189,8 +189,9 @@ class PagedEngine(KVBoost):
                        ) -> List[GenerationResult]:
         """Decode several prompts together, their K/V in the block pool.
 
-        Each prompt reuses its cached chunks as ``generate`` does (seams repaired, chunk
-        blocks shared through the mapper; a chunk's part-filled last block is copied) and
+        Each prompt reuses its cached chunks as ``generate`` does (seams repaired, the blocks
+        that a chunk fills shared through the mapper; blocks with tokens of two chunks, where
+        ``chunk_size`` is no multiple of 16, and a part-filled last block are written anew) and
         prefills its new tokens; then every step runs one token of every prompt: block
         tables and slots from the lengths (``extend_block_tables``), K/V into the pool and
         attention over it in every layer, and the logits' processing
@@ -218,24 +219,29 @@ class PagedEngine(KVBoost):
         try:
             first_logits, kv_new, cached, reused = [], [], [], []
             for ids in all_ids:
-                keys, values, cached_len, _, chunks = self._assemble_run(ids)
-                table: List[int] = []
-                for c in chunks:
+                keys, values, cached_len, bounds, chunks = self._assemble_run(ids)
+                reuse = min(cached_len, len(ids) - 1)   # a fully cached prompt's last token runs again
+                table = [-1] * -(-reuse // bs)
+                for c, (start, end) in zip(chunks, bounds):
+                    # a chunk that begins on a block's border shares the blocks it fills
+                    whole = range(start // bs, min(end, reuse) // bs) if start % bs == 0 else ()
+                    if not whole:
+                        continue
                     shared = c.chunk_id in self.chunk_mapper._chunk_blocks
                     k, v = self._chunk_kv([c])
                     blocks = self.chunk_mapper.load_chunk(
                         c.chunk_id, [(k[l][None], v[l][None]) for l in range(k.shape[0])])
                     # a reference of this call's own, whether or not the chunk was in the pool
                     forked.extend(blocks if shared else self.allocator.fork(blocks))
-                    table.extend(blocks)
-                reuse = min(cached_len, len(ids) - 1)   # a fully cached prompt's last token runs again
-                table = table[:-(-reuse // bs)]
-                if reuse % bs:                    # the new tokens begin inside a chunk's block
-                    own = self.allocator.allocate(1)
-                    reserved.extend(own)
-                    for pool in self.allocator.pools:
-                        pool[own[0]].copy_(pool[table[-1]])
-                    table[-1] = own[0]
+                    for i in whole:
+                        table[i] = blocks[i - start // bs]
+                own = [i for i, block in enumerate(table) if block < 0]
+                if own:     # blocks that hold parts of two chunks, or that the new tokens begin in
+                    blocks = self.allocator.allocate(len(own))
+                    reserved.extend(blocks)
+                    self._write_blocks(blocks, own, keys[:, :, :reuse], values[:, :, :reuse])
+                    for i, block in zip(own, blocks):
+                        table[i] = block
                 prefixes.append(table)
                 cached.append(cached_len)
                 reused.append(reuse)
@@ -336,6 +342,16 @@ class PagedEngine(KVBoost):
         for ids in all_ids:
             self._store_prompt_chunks(ids)
         return results
+
+    def _write_blocks(self, blocks: List[int], places: List[int], keys: torch.Tensor,
+                      values: torch.Tensor) -> None:
+        """The 16-token pieces ``places`` of ``[L, H, P, D]`` K/V into ``blocks`` of every layer;
+        slots past P repeat the last token."""
+        bs = self._block_size
+        at = torch.tensor(places, device=keys.device)[:, None] * bs + torch.arange(bs, device=keys.device)
+        at = at.flatten().clamp(max=keys.shape[2] - 1)
+        for layer in range(keys.shape[0]):
+            self.allocator.write_chunk(layer, blocks, keys[layer][:, at], values[layer][:, at])
 
     def _prefill_suffix(self, ids: TokenIds, keys, values, reuse: int):
         """The prompt's tokens from ``reuse`` on over its reused prefix: the last logits
