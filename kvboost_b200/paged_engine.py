@@ -42,7 +42,7 @@ from typing import Callable, Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
-from .engine import GenerationMode, GenerationResult, KVBoost, TokenIds
+from .engine import GenerationMode, GenerationResult, KVBoost, RecomputeStrategy, TokenIds
 from .flash_attn_ext import install_paged_attention, uninstall_paged_attention
 from .logits import process_logits
 from .paged import BLOCK_SIZE, DeviceBlockAllocator, DeviceChunkMapper, block_table_tensor
@@ -189,10 +189,12 @@ class PagedEngine(KVBoost):
                        ) -> List[GenerationResult]:
         """Decode several prompts together, their K/V in the block pool.
 
-        Each prompt reuses its cached chunks as ``generate`` does (seams repaired, the blocks
-        that a chunk fills shared through the mapper; blocks with tokens of two chunks, where
-        ``chunk_size`` is no multiple of 16, and a part-filled last block are written anew) and
-        prefills its new tokens; then every step runs one token of every prompt: block
+        Each prompt reuses its cached chunks, seams repaired by the engine's strategy for the
+        prefill and for every step (as in ``KVBoost.generate``; this engine's ``generate``
+        decodes over the chunks as cached).  The blocks that a chunk fills are shared through
+        the mapper; those that the repair changed, those with tokens of two chunks (where
+        ``chunk_size`` is no multiple of 16) and a part-filled last block are written anew.
+        Then it prefills its new tokens, and every step runs one token of every prompt: block
         tables and slots from the lengths (``extend_block_tables``), K/V into the pool and
         attention over it in every layer, and the logits' processing
         (``process_logits``): ``repetition_penalty`` over prompt and output,
@@ -222,13 +224,23 @@ class PagedEngine(KVBoost):
                 keys, values, cached_len, bounds, chunks = self._assemble_run(ids)
                 reuse = min(cached_len, len(ids) - 1)   # a fully cached prompt's last token runs again
                 table = [-1] * -(-reuse // bs)
+                repaired = len(chunks) > 1 and self.recompute_strategy != RecomputeStrategy.NONE
                 for c, (start, end) in zip(chunks, bounds):
-                    # a chunk that begins on a block's border shares the blocks it fills
+                    # a chunk that begins on a block's border shares the blocks it fills, but for
+                    # those whose K/V the seam repair changed
                     whole = range(start // bs, min(end, reuse) // bs) if start % bs == 0 else ()
                     if not whole:
                         continue
-                    shared = c.chunk_id in self.chunk_mapper._chunk_blocks
                     k, v = self._chunk_kv([c])
+                    if repaired:
+                        n = len(whole) * bs
+                        same = ((keys[:, :, start:start + n] == k[:, :, :n]) &
+                                (values[:, :, start:start + n] == v[:, :, :n]))
+                        same = same.unflatten(2, (len(whole), bs)).all(-1).all(-1).all(1).all(0)
+                        whole = [i for i, ok in zip(whole, same.tolist()) if ok]
+                        if not whole:
+                            continue
+                    shared = c.chunk_id in self.chunk_mapper._chunk_blocks
                     blocks = self.chunk_mapper.load_chunk(
                         c.chunk_id, [(k[l][None], v[l][None]) for l in range(k.shape[0])])
                     # a reference of this call's own, whether or not the chunk was in the pool
@@ -236,7 +248,7 @@ class PagedEngine(KVBoost):
                     for i in whole:
                         table[i] = blocks[i - start // bs]
                 own = [i for i, block in enumerate(table) if block < 0]
-                if own:     # blocks that hold parts of two chunks, or that the new tokens begin in
+                if own:     # changed blocks, blocks with parts of two chunks, the one that new tokens begin in
                     blocks = self.allocator.allocate(len(own))
                     reserved.extend(blocks)
                     self._write_blocks(blocks, own, keys[:, :, :reuse], values[:, :, :reuse])
