@@ -119,3 +119,84 @@ def test_repaired_seams_reach_the_decode_steps(monkeypatch, strategy, chunk_size
             own = [15, 23] if again else [15]
             same = [a == b for a, b in zip(tables[0][:24], tables[2][:24])]
             assert same[:7] + same[8:] == [i not in own for i in range(24) if i != 7]
+
+
+def test_steps_append_in_order(monkeypatch):
+    """After the last step the pool holds the prefill's K/V and, behind them, what the steps appended,
+    and every step attended to its own token and all before it."""
+    from kvboost_b200 import paged_decode, paged_engine
+    from kvboost_b200.paged_engine import PagedEngine
+    prompts = _prompts([100, 31, 16, 1, 77], 64)
+    new = 20
+    eng = PagedEngine(_model(), num_blocks=64, chunk_size=32, min_chunk_tokens=8)
+    eng.warm(prompts[0][:64])
+    append, attend, uninstall = (paged_decode.append_paged_kv, paged_decode.paged_decode_attention,
+                                 paged_engine.uninstall_paged_attention)
+    added, seen, last, state_of = [], [], [], []
+
+    def record_append(k, v, pool, slots):
+        added.append((k.clone(), v.clone()))
+        append(k, v, pool, slots)
+
+    def record_attend(q, pool, tables, lens, *a, **kw):
+        seen.append(lens.tolist())
+        state_of[:] = [tables.tolist(), lens.tolist()]
+        return attend(q, pool, tables, lens, *a, **kw)
+
+    def record_last(model):
+        for table, n in zip(*state_of):
+            last.append([eng.allocator.read_kv(layer, table[:-(-n // 16)], n) for layer in range(2)])
+        return uninstall(model)
+
+    monkeypatch.setattr(paged_decode, "append_paged_kv", record_append)
+    monkeypatch.setattr(paged_decode, "paged_decode_attention", record_attend)
+    monkeypatch.setattr(paged_engine, "uninstall_paged_attention", record_last)
+    _, _, prefill, _ = _pool_and_prefill(eng, prompts, monkeypatch, max_new_tokens=new)
+    assert len(added) == len(seen) == 2 * (new - 1)
+    assert seen[::2] == seen[1::2] == [[len(p) + i + 1 for p in prompts] for i in range(new - 1)]
+    for b, p in enumerate(prompts):
+        for layer in range(2):
+            for kv in range(2):
+                steps = [added[2 * i + layer][kv][b] for i in range(new - 1)]
+                want = torch.cat([prefill[b][layer][kv], torch.stack(steps, 1)], 1)
+                assert torch.equal(last[b][layer][kv], want)
+
+
+# Logits of magnitude up to 4 in bfloat16: two of them compared, each in two evaluations, rounded by at
+# most 4 * 2^-8 = 0.016 apiece, and as much again from the activations below.
+CLOSE = 0.12
+
+
+def _behind(model, ids, reuse, keys, values, tokens):
+    """How far each token lies behind the best of a dense forward over the reused K/V, the prompt's
+    other tokens and the tokens before it."""
+    from kvboost_b200.engine import KVBoost
+    cache = KVBoost._cache_from(keys[:, :, :reuse].contiguous(), values[:, :, :reuse].contiguous())
+    x = torch.tensor([ids[reuse:] + tokens[:-1]], device="cuda")
+    pos = torch.arange(reuse, reuse + x.shape[1], device="cuda")[None]
+    with torch.no_grad():
+        logits = model(input_ids=x, position_ids=pos, past_key_values=cache, use_cache=True).logits[0]
+    logits = logits[-len(tokens):].float()
+    return logits.amax(-1) - logits[torch.arange(len(tokens)), torch.tensor(tokens)]
+
+
+def test_greedy_tokens_follow_the_repaired_context():
+    """Short prompts, where each block carries weight: the tokens are the best over the repaired K/V, and
+    with one block of the reference zeroed they are not (the comparison can tell)."""
+    from kvboost_b200.paged_engine import PagedEngine
+    m = _model()
+    prompts = _prompts([36, 40, 33], 32, seed=5)
+    eng = PagedEngine(m, num_blocks=64, chunk_size=16, min_chunk_tokens=8, recompute_overlap=4)
+    eng.warm(prompts[0][:32])
+    want = [eng._assemble(p) for p in prompts]
+    got = eng.generate_paged(prompts, max_new_tokens=12)
+    for block in (0, 1):
+        far = 0.0
+        for p, r, (keys, values, n, _) in zip(prompts, got, want):
+            assert n == r.cached_tokens == 32
+            assert (_behind(m, p, 32, keys, values, r.generated_ids) <= CLOSE).all()
+            keys, values = keys.clone(), values.clone()
+            keys[:, :, 16 * block:16 * block + 16] = 0
+            values[:, :, 16 * block:16 * block + 16] = 0
+            far = max(far, float(_behind(m, p, 32, keys, values, r.generated_ids).max()))
+        assert far > 2 * CLOSE
