@@ -120,13 +120,22 @@ class PagedEngine(KVBoost):
                       t0: float, hit_ratio: float) -> GenerationResult:
         from transformers import DynamicCache
         table: List[int] = []
-        in_pool = 0
+        in_pool = shared_blocks = 0
         if keys is not None and cached_len > 0:
-            for c in chunks:      # the chunks as cached (before any seam repair)
-                k, v = self._chunk_kv([c])
-                table.extend(self.chunk_mapper.load_chunk(
-                    c.chunk_id, [(k[l][None], v[l][None]) for l in range(k.shape[0])]))
             in_pool = cached_len
+            if any(c.length % self._block_size for c in chunks[:-1]):
+                # chunks that begin inside a block cannot lend their blocks: the sequence's own
+                n = -(-cached_len // self._block_size)
+                table = self.allocator.allocate(n)
+                kv = [self._chunk_kv([c]) for c in chunks]
+                self._write_blocks(table, list(range(n)), torch.cat([k for k, _ in kv], 2),
+                                   torch.cat([v for _, v in kv], 2))
+            else:
+                shared_blocks = -(-cached_len // self._block_size)
+                for c in chunks:      # the chunks as cached (before any seam repair)
+                    k, v = self._chunk_kv([c])
+                    table.extend(self.chunk_mapper.load_chunk(
+                        c.chunk_id, [(k[l][None], v[l][None]) for l in range(k.shape[0])]))
         live = token_ids[cached_len:]
         if live:
             cache = self._cache_from(keys, values) if keys is not None else DynamicCache()
@@ -166,9 +175,8 @@ class PagedEngine(KVBoost):
         table = state["block_table"]
         t1 = time.perf_counter()
         # the sequence's own blocks (past the reused prefix's) return to the free list
-        cached_blocks = (cached_len + self._block_size - 1) // self._block_size
-        if table[cached_blocks:]:
-            self.allocator.free(table[cached_blocks:])
+        if table[shared_blocks:]:
+            self.allocator.free(table[shared_blocks:])
         self.last_block_table = table
         return GenerationResult(
             mode=mode_name, prompt=prompt if isinstance(prompt, str) else "",

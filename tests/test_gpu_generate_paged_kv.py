@@ -200,3 +200,23 @@ def test_greedy_tokens_follow_the_repaired_context():
             values[:, :, 16 * block:16 * block + 16] = 0
             far = max(far, float(_behind(m, p, 32, keys, values, r.generated_ids).max()))
         assert far > 2 * CLOSE
+
+
+@pytest.mark.parametrize("chunk_size", [40, 24, 32])
+def test_generate_with_chunks_that_end_inside_a_block(chunk_size):
+    """The one-prompt loop, two and more chunks reused: greedy tokens follow the assembled K/V, and no
+    cached chunk's block is freed while the mapper holds it."""
+    from kvboost_b200.paged_engine import PagedEngine
+    m = _model()
+    prompts = _prompts([84, 90, 85], 80, seed=11)
+    eng = PagedEngine(m, num_blocks=64, chunk_size=chunk_size, min_chunk_tokens=chunk_size, recompute_strategy="none")
+    eng.warm(prompts[0][:80])
+    n = 80 // chunk_size * chunk_size
+    for p in prompts:
+        keys, values, cached, _ = eng._assemble(p)
+        tokens = eng.generate(p, max_new_tokens=12).generated_ids
+        assert cached == n
+        assert (_behind(m, p, n, keys, values, tokens) <= CLOSE).all()
+        held = [b for blocks in eng.chunk_mapper._chunk_blocks.values() for b in blocks]
+        assert not set(held) & set(eng.allocator._free)
+        assert eng.allocator.used_blocks == len(held)
