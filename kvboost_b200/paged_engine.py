@@ -45,6 +45,7 @@ import torch
 from .engine import GenerationMode, GenerationResult, KVBoost, RecomputeStrategy, TokenIds
 from .flash_attn_ext import install_paged_attention, uninstall_paged_attention
 from .logits import process_logits
+from .ops import read_status, status_word
 from .paged import BLOCK_SIZE, DeviceBlockAllocator, DeviceChunkMapper, block_table_tensor
 from .paged_decode import append_paged_kv, extend_block_tables
 
@@ -210,7 +211,8 @@ class PagedEngine(KVBoost):
         token id, and ``allowed_tokens(i, output ids)``, the ids prompt i may continue with
         (None: any).  A prompt that has met the end id keeps its place in the steps until
         all have ended.  The blocks of the longest outputs are reserved before the first
-        step and returned at the end; the prompts' new chunks are then stored.
+        step and returned at the end; the prompts' new chunks are then stored.  A step that the
+        device refused a part of (``ops.read_status``) raises.
         """
         if self.allocator.dtype != next(self.model.parameters()).dtype:
             raise RuntimeError("generate_paged needs a pool in the model's dtype")
@@ -221,6 +223,9 @@ class PagedEngine(KVBoost):
         all_ids = [self._encode(p) for p in prompts]
         if any(not ids for ids in all_ids):
             raise ValueError("empty prompt")
+        # the device's status word is read with every step's tokens; what others left in it waits
+        status = status_word(self.device)
+        before = read_status(self.device)
         B, bs, dev = len(prompts), self._block_size, self.device
         most = max(1, int(max_new_tokens))   # a first token comes with the prompt, as in generate
         prefixes: List[List[int]] = []     # each prompt's blocks of reused chunks
@@ -325,7 +330,11 @@ class PagedEngine(KVBoost):
                     nxt = self._sample(x.masked_fill_(lost[:, None], 0.0), 1.0, do_sample)
                     history[rows, total_lens.long()] = nxt.to(torch.int32)
                     total_lens += 1
-                    picked, lost = torch.stack([nxt, lost.long()]).tolist()
+                    picked, lost, refused = torch.stack(
+                        [nxt, lost.long(), status.long().expand(B)]).tolist()
+                    if refused[0]:
+                        raise RuntimeError(f"the device refused part of a step (status {refused[0]:#x}, "
+                                           "KVB_STATUS_*): no tokens are returned")
                     for b, t in enumerate(picked):
                         if done[b]:
                             continue
@@ -349,6 +358,8 @@ class PagedEngine(KVBoost):
                 uninstall_paged_attention(self.model)
             t1 = time.perf_counter()
         finally:
+            if before:
+                status.bitwise_or_(before)
             self.allocator.free(reserved)
             self.allocator.free(forked)
         results = [GenerationResult(

@@ -220,3 +220,28 @@ def test_generate_with_chunks_that_end_inside_a_block(chunk_size):
         held = [b for blocks in eng.chunk_mapper._chunk_blocks.values() for b in blocks]
         assert not set(held) & set(eng.allocator._free)
         assert eng.allocator.used_blocks == len(held)
+
+
+def test_a_refused_step_raises(monkeypatch):
+    """A block id outside the pool, which the kernels skip and report: no tokens, the pool whole, the bit
+    left for ``read_status``; bits that others left do not stop a call and are there after it."""
+    from kvboost_b200 import ops, paged_engine
+    from kvboost_b200.paged_engine import PagedEngine
+    eng = PagedEngine(_model(), num_blocks=64, chunk_size=32, min_chunk_tokens=8)
+    prompts = _prompts([50, 20], 0)
+    dev = torch.device("cuda")
+    ops.status_word(dev).fill_(64)
+    assert len(eng.generate_paged(prompts, max_new_tokens=4)[0].generated_ids) == 4
+    assert ops.read_status(dev) == 64
+    tables = paged_engine.block_table_tensor
+
+    def spoiled(lists, device):
+        t = tables(lists, device)
+        t[0, 0] = 1 << 20               # a block of the reused chunk
+        return t
+
+    monkeypatch.setattr(paged_engine, "block_table_tensor", spoiled)
+    with pytest.raises(RuntimeError, match="status 0x10"):
+        eng.generate_paged([p[:-1] + [7] for p in prompts], max_new_tokens=4)
+    assert ops.read_status(dev) == 16
+    assert eng.allocator.used_blocks == eng.chunk_mapper.blocks_used_by_chunks()
