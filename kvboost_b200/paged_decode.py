@@ -27,13 +27,29 @@ from .ops import _DTYPES, _check_tensor, _status_words, status_word
 
 BLOCK_SIZE = 16
 
+def _stream_of(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def _new_strided(shape, strides, dtype) -> torch.Tensor:
+    return torch.empty_strided(shape, strides, dtype=dtype, device="cuda")
+
+
+def _binding(name: str, public):
+    """A function of torch's C binding, or ``public`` on a torch without it."""
+    f = torch._C
+    for part in name.split("."):
+        f = getattr(f, part, None)
+    return f or public
+
+
 # A decode step calls these operators once per layer, so the host's cost per call is kept
 # to a few checks: the stream handle comes from torch's C binding (2 us less than building a
 # Stream object), results from its allocation of a strided tensor on the current device
 # (0.8 us, ``new_empty`` 1.3 to 1.5), the device is switched only where it differs.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
-_empty_strided = torch._C._dynamo.guards._empty_strided_cuda
+_raw_stream = _binding("_cuda_getCurrentRawStream", _stream_of)
+_current_device = _binding("_cuda_getDevice", torch.cuda.current_device)
+_empty_strided = _binding("_dynamo.guards._empty_strided_cuda", _new_strided)
 
 
 def _allocator(device):

@@ -1,0 +1,59 @@
+"""GPU: the batched step's operators where host code and device meet: torch without private bindings, calls
+from several threads, captured calls whose inputs change, results that overlap."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import step as ostep
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(autouse=True)
+def _gpu():
+    if not torch.cuda.is_available() or torch.cuda.get_device_capability()[0] != 10:
+        pytest.skip("needs an sm_100 (B200) device")
+    from kvboost_b200 import ops
+    ops.read_status(torch.device("cuda"))
+    yield
+    assert ops.read_status(torch.device("cuda")) == 0
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _step(g, n=700):
+    """One call of each operator; the results."""
+    from kvboost_b200.logits import process_logits
+    from kvboost_b200.paged_decode import append_paged_kv, extend_block_tables, paged_decode_attention
+    tables = torch.zeros(2, 200, dtype=torch.int32, device=DEV)
+    s = extend_block_tables(tables, _i32([0, 0]), _i32([n, 5]), torch.arange(300, dtype=torch.int32, device=DEV), _i32([300]),
+                            300, n + 5)
+    pool = torch.zeros(300, 2, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    kv = torch.randn(2, n + 5, 2, 64, generator=g).to(DEV, torch.bfloat16)
+    append_paged_kv(kv[0], kv[1], pool, s.slots)
+    q = torch.randn(2, 8, 1, 64, generator=g).to(DEV, torch.bfloat16)
+    o, lse = paged_decode_attention(q, pool, tables, s.seq_lens)
+    x = process_logits(torch.randn(2, 1001, generator=g).to(DEV), temperature=torch.full((2,), 0.7, device=DEV))
+    return [*s, tables, pool, o, lse, x]
+
+
+def test_torch_without_private_bindings(monkeypatch):
+    """The public functions in their place give the same results, on another stream too."""
+    from kvboost_b200 import paged_decode as pd
+    want = _step(torch.Generator().manual_seed(1))
+    monkeypatch.setattr(pd, "_raw_stream", pd._stream_of)
+    monkeypatch.setattr(pd, "_current_device", torch.cuda.current_device)
+    monkeypatch.setattr(pd, "_empty_strided", pd._new_strided)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = _step(torch.Generator().manual_seed(1))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
