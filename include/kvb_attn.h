@@ -620,7 +620,7 @@ int kvb_paged_decode_fwd(const KvbPagedDecodeParams* params, void* stream);
  * in the history or the bias list are ignored; total_lens is clamped to [0,
  * history_len], prompt_lens to [0, total].  A row whose mask leaves nothing is all -inf.
  * Output: float32, or the logits' dtype rounded once at the end; o may be the
- * logits themselves (same dtype and stride).  No counterpart in the reference,
+ * logits themselves (same dtype and stride), and overlaps none of their rows otherwise.  No counterpart in the reference,
  * which samples from softmax(logits / max(temperature, 1e-5)).
  */
 enum { KVB_DTYPE_FP32 = 2 }; /* logits only */

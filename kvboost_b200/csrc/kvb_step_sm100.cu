@@ -507,6 +507,20 @@ __global__ void __launch_bounds__(256, 6) kvb_logits_kernel(const LogitsArgs a) 
   }
 }
 
+// Whether a row of n bytes, `step` bytes from one to the next, of one buffer shares bytes with one of
+// the other.  (Rows of two buffers may lie side by side in one wider buffer.)
+bool rows_meet(const void* p, int64_t n, int64_t step, const void* q, int64_t m, int64_t other, int rows) {
+  const int64_t x = (int64_t)reinterpret_cast<uintptr_t>(p), y = (int64_t)reinterpret_cast<uintptr_t>(q);
+  if (x + (rows - 1) * step + n <= y || y + (rows - 1) * other + m <= x) return false;
+  for (int i = 0, j = 0; i < rows && j < rows;) {
+    const int64_t a = x + i * step, b = y + j * other;
+    if (a + n <= b) ++i;
+    else if (b + m <= a) ++j;
+    else return true;
+  }
+  return false;
+}
+
 template <typename TI, typename TO>
 void launch_logits(LogitsArgs a, int batch, cudaStream_t s) {
   // Slices of up to 8192 tokens, as long as every SM gets two CTAs (192 x 151936: 34.7 us with
@@ -643,6 +657,10 @@ extern "C" int kvb_process_logits(const KvbLogitsParams* p, void* stream) {
     return fail(KVB_ERR_INVALID, "row strides must be >= vocab");
   if (p->logits == p->out && (p->dtype != p->out_dtype || p->logits_stride != p->out_stride))
     return fail(KVB_ERR_INVALID, "processing in place needs the logits' dtype and stride");
+  if (p->logits != p->out &&
+      kvb_step::rows_meet(p->logits, p->vocab * (int64_t)el_in, p->logits_stride * (int64_t)el_in, p->out,
+                          p->vocab * (int64_t)el_out, p->out_stride * (int64_t)el_out, p->batch))
+    return fail(KVB_ERR_INVALID, "out must be the logits themselves or not overlap them");
   if (p->token_ids && (!p->total_lens || p->history_stride < p->history_len))
     return fail(KVB_ERR_INVALID, "token_ids needs total_lens and history_stride >= history_len");
   if (!p->token_ids && (p->repetition_penalty || p->frequency_penalty || p->presence_penalty))

@@ -58,7 +58,8 @@ def process_logits(logits: torch.Tensor, token_ids: Optional[torch.Tensor] = Non
     given twice adds twice.  ``allowed_mask``: int32 ``[B, >= ceil(V / 32)]``, bit ``v % 32`` of
     word ``v // 32`` set where token v is allowed; a row that allows nothing is all -inf.
     Every part is optional.  Ids outside the vocabulary are ignored.  ``out``: float32 or
-    the logits' dtype; ``out=logits`` works in place.
+    the logits' dtype; ``out=logits`` works in place, an ``out`` that overlaps them otherwise is
+    refused.
     """
     if not isinstance(logits, torch.Tensor):
         raise TypeError("logits must be a torch.Tensor")

@@ -57,3 +57,22 @@ def test_torch_without_private_bindings(monkeypatch):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                             (torch.float32, torch.float32)])
+def test_logits_beside_their_result_in_one_buffer(dtype, out_dtype):
+    """Rows of the logits and of the result in turn in one buffer do not overlap; rows that do are
+    refused."""
+    from kvboost_b200.logits import process_logits
+    B, V = 5, 1004
+    wide = torch.zeros(B, 3 * V * 4, dtype=torch.uint8, device=DEV)
+    x = wide[:, :V * dtype.itemsize].view(dtype)
+    o = wide[:, V * 8:V * 8 + V * out_dtype.itemsize].view(out_dtype)
+    x.copy_(torch.randn(B, V, device=DEV))
+    want = x.float() * 2
+    t = torch.full((B,), 0.5, device=DEV)
+    assert process_logits(x, temperature=t, out=o) is o
+    assert torch.equal(o.float(), want)
+    with pytest.raises(Exception, match="overlap"):
+        process_logits(x, temperature=t, out=wide[:, 8:8 + V * out_dtype.itemsize].view(out_dtype))
