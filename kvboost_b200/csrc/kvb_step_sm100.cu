@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <string>
 #include <type_traits>
@@ -576,8 +577,17 @@ extern "C" int kvb_extend_block_tables(const KvbExtendTablesParams* p, void* str
     return fail(KVB_ERR_INVALID, "slots and positions must be 16-byte aligned");
   const int smem = (3 * p->batch + 1) * 4;
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kvb_step::kvb_extend_tables_kernel,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // the largest batch's limit, once per device: a limit of each call's own could shrink between
+    // another thread's setting and its launch
+    static std::atomic<uint64_t> ready{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e == cudaSuccess && (dev > 63 || !(ready.load(std::memory_order_acquire) & bit))) {
+      e = cudaFuncSetAttribute(kvb_step::kvb_extend_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (3 * KVB_MAX_STEP_ROWS + 1) * 4);
+      if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_release);
+    }
     if (e != cudaSuccess)
       return fail(KVB_ERR_CUDA, std::string("kvb_extend_block_tables: ") + cudaGetErrorString(e));
   }

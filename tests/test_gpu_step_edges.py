@@ -76,3 +76,53 @@ def test_logits_beside_their_result_in_one_buffer(dtype, out_dtype):
     assert torch.equal(o.float(), want)
     with pytest.raises(Exception, match="overlap"):
         process_logits(x, temperature=t, out=wide[:, 8:8 + V * out_dtype.itemsize].view(out_dtype))
+
+
+def _tables_args(B, seed):
+    rng = np.random.default_rng(seed)
+    lens, new = rng.integers(0, 34, B), rng.integers(0, 4, B)
+    tables = np.full((B, 4), -7)
+    ids = rng.permutation(B * 4 + 10)
+    have = -(-lens // 16)
+    at = 0
+    for b in range(B):
+        tables[b, :have[b]] = ids[at:at + have[b]]
+        at += have[b]
+    return tables, lens, new, ids[at:], len(ids) - at, B * 4 + 10, int(new.sum())
+
+
+def test_tables_of_large_and_small_batches_from_two_threads():
+    """Host threads that build the tables of batches of different size at once get their own results."""
+    import threading
+
+    from kvboost_b200 import _lib
+    lib = _lib.load()
+    work = []
+    for B in (8192, 3500):
+        tables, lens, new, free, nfree, nblk, total = _tables_args(B, B)
+        want = ostep.extend_tables(tables, lens, new, free, nfree, nblk, total)
+        ins = [_i32(x) for x in (tables, lens, new, free, [nfree])]
+        outs = [torch.zeros(n, dtype=t, device=DEV) for n, t in
+                ((total, torch.int32), (total, torch.int64), (B + 1, torch.int32), (B, torch.int32), (1, torch.int32),
+                 (1, torch.int32))]
+        p = _lib.pack_extend_tables(B, 4, 16, nblk, total, len(free), 4, *[t.data_ptr() for t in ins + outs])
+        work.append((p, torch.cuda.Stream(), ins, outs, want))
+    torch.cuda.synchronize()
+    refused = []
+
+    def run(p, stream):
+        for _ in range(20000):
+            if lib.kvb_extend_block_tables(p, stream.cuda_stream):
+                refused.append(lib.kvb_last_error())
+
+    threads = [threading.Thread(target=run, args=w[:2]) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not refused, (len(refused), refused[0])
+    for _, _, ins, outs, want in work:
+        for got, w in zip((ins[0], *outs[:4]), want):
+            assert np.array_equal(got.cpu().numpy(), w)
+        assert outs[4].item() == want[5] and outs[5].item() == 0
