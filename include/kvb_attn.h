@@ -651,6 +651,12 @@ typedef struct KvbLogitsParams {
 
 int kvb_process_logits(const KvbLogitsParams* params, void* stream);
 
+/*
+ * A new status word, zeroed, on the current device; freed with cudaFree.  It may be
+ * called while the calling thread captures a graph and becomes no part of it.
+ */
+int kvb_new_status(int32_t** status);
+
 /* Human-readable reason for the last non-zero return on this host thread. */
 const char* kvb_last_error(void);
 

@@ -275,6 +275,8 @@ def load() -> ctypes.CDLL:
         lib.kvb_paged_decode_workspace_bytes.restype = ctypes.c_int64
         lib.kvb_process_logits.argtypes = [_vp, _vp]   # packed bytes or a pointer
         lib.kvb_process_logits.restype = ctypes.c_int
+        lib.kvb_new_status.argtypes = [ctypes.POINTER(_vp)]
+        lib.kvb_new_status.restype = ctypes.c_int
         lib.kvb_last_error.argtypes = []
         lib.kvb_last_error.restype = ctypes.c_char_p
         lib.kvb_abi_version.argtypes = []

@@ -709,3 +709,24 @@ extern "C" int kvb_process_logits(const KvbLogitsParams* p, void* stream) {
   else kvb_step::launch_logits<bf16, bf16>(a, p->batch, s);
   return kvb_step::launched("kvb_process_logits");
 }
+
+extern "C" int kvb_new_status(int32_t** status) {
+  if (!status) return fail(KVB_ERR_INVALID, "status must be non-null");
+  *status = nullptr;
+  // a thread that captures may neither allocate nor wait for other streams unless it says so
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return fail(KVB_ERR_CUDA, std::string("kvb_new_status: ") + cudaGetErrorString(e));
+  int32_t* word = nullptr;
+  cudaStream_t s = nullptr;
+  e = cudaMalloc(&word, sizeof(*word));
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof(*word), s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (s) cudaStreamDestroy(s);
+  if (e != cudaSuccess && word) cudaFree(word);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return fail(KVB_ERR_CUDA, std::string("kvb_new_status: ") + cudaGetErrorString(e));
+  *status = word;
+  return KVB_OK;
+}

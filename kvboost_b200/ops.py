@@ -17,6 +17,7 @@ Layouts
 
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional, Tuple
 
@@ -28,6 +29,14 @@ _DTYPES = {torch.bfloat16: _lib.KVB_DTYPE_BF16, torch.float16: _lib.KVB_DTYPE_FP
 _status_words = {}
 
 
+class _StatusMemory:
+    """One int32 of device memory, which lives as long as the process."""
+
+    def __init__(self, address: int) -> None:
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False),
+                                         "version": 2}
+
+
 def status_word(device: torch.device) -> torch.Tensor:
     """Per-device int32 word the kernels OR error codes into (bounded waits)."""
     idx = torch.device(device).index
@@ -35,7 +44,13 @@ def status_word(device: torch.device) -> torch.Tensor:
         idx = torch.cuda.current_device()
     w = _status_words.get(idx)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=f"cuda:{idx}")
+        # made and zeroed by the library, beside torch's allocator and streams: a first call inside
+        # a graph's capture would otherwise record the zeroing, and every replay would wipe what
+        # other calls reported
+        with torch.cuda.device(idx), torch.inference_mode(False):   # cleared outside of it too
+            at = ctypes.c_void_p()
+            _lib.check(_lib.load().kvb_new_status(ctypes.byref(at)), "kvb_new_status")
+            w = torch.as_tensor(_StatusMemory(at.value), device=f"cuda:{idx}")
         _status_words[idx] = w
     return w
 

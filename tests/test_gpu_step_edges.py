@@ -126,3 +126,32 @@ def test_tables_of_large_and_small_batches_from_two_threads():
         for got, w in zip((ins[0], *outs[:4]), want):
             assert np.array_equal(got.cpu().numpy(), w)
         assert outs[4].item() == want[5] and outs[5].item() == 0
+
+
+def test_first_call_on_a_device_inside_a_capture():
+    """The status word that it makes is zero before the first replay, and replays add to it."""
+    from kvboost_b200 import ops
+    from kvboost_b200.paged_decode import extend_block_tables
+    dev = torch.device(DEV)
+    args = (torch.zeros(2, 4, dtype=torch.int32, device=DEV), _i32([0, 0]), _i32([1, 99]), _i32([5, 6]), _i32([2]), 10, 100)
+    extend_block_tables(*args)
+    assert ops.read_status(dev) == ostep.BAD_LENGTH
+    words = dict(ops._status_words)
+    ops._status_words.clear()
+    try:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            s = extend_block_tables(*args)
+        assert ops.read_status(dev, reset=False) == 0
+        ops.status_word(dev).fill_(ostep.BAD_BLOCK)
+        graph.replay()
+        assert ops.read_status(dev) == ostep.BAD_BLOCK | ostep.BAD_LENGTH
+        assert s.slots[:2].tolist() == [6 * 16, -1]
+        ops._status_words.clear()
+        with torch.inference_mode():
+            extend_block_tables(*args)
+        assert ops.read_status(dev) == ostep.BAD_LENGTH and ops.read_status(dev) == 0
+    finally:
+        ops._status_words.clear()
+        ops._status_words.update(words)
