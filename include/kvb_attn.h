@@ -571,7 +571,8 @@ int kvb_append_paged_kv(const KvbAppendPagedParams* params, void* stream);
  * kvb_paged_decode_workspace_bytes(params) bytes (-1: invalid params), 16-byte
  * aligned, whatever it holds; calls that may overlap on the GPU must not share
  * one, and one of a call that set KVB_STATUS_LOAD_WAIT must not be used again.  max_seq_len (0: unknown) is a hint that only chooses the launch shape;
- * any value gives right results (their last bits may differ).
+ * any value gives right results (their last bits may differ).  o may be q (same strides); its heads
+ * do not overlap one another.
  */
 typedef struct KvbPagedDecodeParams {
   int32_t dtype;

@@ -1168,6 +1168,13 @@ int check(const KvbPagedDecodeParams* p) {
   if (p->q_batch_stride % 8 || p->q_head_stride % 8 || p->o_batch_stride % 8 ||
       p->o_head_stride % 8)
     return fail(KVB_ERR_INVALID, "strides must be multiples of 8 elements");
+  // heads of one request inside its row, or requests of one head inside the head's
+  const auto apart = [&](int64_t in, int64_t n_in, int64_t out, int64_t n_out) {
+    return (n_in == 1 || in >= p->head_dim) && (n_out == 1 || out >= (n_in > 1 ? (n_in - 1) * in : 0) + p->head_dim);
+  };
+  if (!apart(p->o_head_stride, p->num_q_heads, p->o_batch_stride, p->batch) &&
+      !apart(p->o_batch_stride, p->batch, p->o_head_stride, p->num_q_heads))
+    return fail(KVB_ERR_INVALID, "heads of o must not overlap");
   return KVB_OK;
 }
 

@@ -241,7 +241,8 @@ def paged_decode_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_tables:
     ``block_tables``: int32 ``[B, max_blocks]``; ``seq_lens``: int32 ``[B]`` device tensor, the
     tokens row b attends to (its own included, once appended).  ``Hq % Hkv == 0``.
     Returns ``(o [B, Hq, 1, D] in q's dtype, lse float32 [B, Hq, 1] or None)``; a row of
-    length 0 gives zeros and -inf.  ``max_seq_len``, a host-known bound of the lengths,
+    length 0 gives zeros and -inf.  ``out``: q's shape and dtype, in heads that do not overlap
+    (``out=q`` works in place).  ``max_seq_len``, a host-known bound of the lengths,
     only tunes the launch.
     """
     _check_tensor("q", q, 4)

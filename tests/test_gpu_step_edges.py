@@ -155,3 +155,26 @@ def test_first_call_on_a_device_inside_a_capture():
     finally:
         ops._status_words.clear()
         ops._status_words.update(words)
+
+
+@pytest.mark.parametrize("lens", [[3000, 5, 64], [40, 0, 333]])
+def test_attention_into_the_query_and_into_other_layouts(lens):
+    """``out=q``, a result with the heads outermost, both launch shapes; a broadcast one is refused."""
+    from kvboost_b200.paged_decode import paged_decode_attention
+    g = torch.Generator().manual_seed(2)
+    nblk = [-(-n // 16) for n in lens]
+    tables = torch.zeros(3, max(nblk), dtype=torch.int32)
+    ids = torch.randperm(sum(nblk), generator=g).to(torch.int32)
+    for b in range(3):
+        tables[b, :nblk[b]] = ids[sum(nblk[:b]):sum(nblk[:b + 1])]
+    pool = torch.randn(sum(nblk), 2, 2, 16, 64, generator=g).to(DEV, torch.bfloat16)
+    q = torch.randn(3, 8, 1, 64, generator=g).to(DEV, torch.bfloat16)
+    args = (pool, tables.to(DEV), _i32(lens))
+    want, _ = paged_decode_attention(q, *args)
+    own = q.clone()
+    assert paged_decode_attention(own, *args, out=own)[0] is own
+    assert torch.equal(own, want)
+    turned = torch.empty(8, 3, 1, 64, dtype=q.dtype, device=DEV).transpose(0, 1)
+    assert torch.equal(paged_decode_attention(q, *args, out=turned)[0], want)
+    with pytest.raises(Exception, match="overlap"):
+        paged_decode_attention(q, *args, out=torch.empty(1, 8, 1, 64, dtype=q.dtype, device=DEV).expand(3, -1, -1, -1))

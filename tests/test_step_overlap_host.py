@@ -29,3 +29,24 @@ def test_logits_refuse_an_overlapping_result(lib, batch, out_dtype, stride, off,
     p = _lib.KvbLogitsParams(0, out_dtype, batch, 1000, 0, 0, 1 << 20, (1 << 20) + off, stride, out_stride)
     assert lib.kvb_process_logits(ctypes.byref(p), None) == _lib.KVB_ERR_INVALID
     assert "overlap" in lib.kvb_last_error().decode()
+
+
+@pytest.mark.parametrize("batch,batch_stride,head_stride", [
+    (2, 0, 128), (2, 1024, 0), (2, 1016, 128), (3, 128, 256), (1, 0, 64), (2, 1024, 120)])
+def test_decode_refuses_a_result_whose_heads_overlap(lib, batch, batch_stride, head_stride):
+    """8 heads of 128: a broadcast result, rows closer than their heads, heads closer than their width."""
+    at = 1 << 20
+    p = _lib.KvbPagedDecodeParams(0, 128, batch, 8, 2, 16, 1, 0.1, at, at, at, 1024, 128, batch_stride, head_stride, 8,
+                                  at, None, None, 10, 4, 4, at, at, 0, 0, at, None, 0)
+    assert lib.kvb_paged_decode_fwd(ctypes.byref(p), None) == _lib.KVB_ERR_INVALID
+    assert "overlap" in lib.kvb_last_error().decode()
+    assert lib.kvb_paged_decode_workspace_bytes(ctypes.byref(p)) == -1
+
+
+@pytest.mark.parametrize("batch,heads,batch_stride,head_stride", [
+    (2, 8, 1024, 128), (1, 8, 0, 128), (3, 1, 128, 0), (3, 8, 128, 384), (2, 8, 4096, 512), (0, 8, 0, 0)])
+def test_decode_takes_results_whose_heads_do_not(lib, batch, heads, batch_stride, head_stride):
+    at = 1 << 20
+    p = _lib.KvbPagedDecodeParams(0, 128, batch, heads, 1, 16, 1, 0.1, at, at, at, 1024, 128, batch_stride, head_stride, 8,
+                                  at, None, None, 10, 4, 4, at, at, 0, 0, at, None, 0)
+    assert lib.kvb_paged_decode_workspace_bytes(ctypes.byref(p)) == 0
