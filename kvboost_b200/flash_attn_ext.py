@@ -309,6 +309,8 @@ def _make_paged_attn_fn(layer_idx: int, state: dict):
         if state.get("slots") is not None:
             if query.size(2) != 1 or key.size(2) != 1:
                 raise NotImplementedError("a batched paged step takes one token per request")
+            if kwargs.get("sliding_window") is not None or kwargs.get("softcap") is not None:
+                raise NotImplementedError("kvboost_b200: sliding-window / softcapped attention")
             pool = allocator.pools[layer_idx]
             append_paged_kv(key[:, :, 0], value[:, :, 0], pool, state["slots"])
             out, _ = paged_decode_attention(query, pool, state["block_tables"], state["seq_lens"],

@@ -1,5 +1,5 @@
-"""The paged paths import on a torch whose C binding lacks the private names that the batched step's
-operators use to save host time (CPU)."""
+"""Host side of the paged paths (CPU): they import on a torch whose C binding lacks the private names that
+the batched step's operators use to save host time, and the step refuses attention it does not have."""
 
 import subprocess
 import sys
@@ -34,3 +34,15 @@ for name in sys.argv[1:]:
 """
     names = NAMES if missing == "all" else [missing]
     subprocess.run([sys.executable, "-c", code, *names], check=True, cwd=_build.ROOT, timeout=300)
+
+
+@pytest.mark.parametrize("kw", [{"sliding_window": 128}, {"softcap": 30.0}])
+def test_a_batched_step_refuses_attention_it_does_not_have(kw):
+    """As the other attention paths do, and before anything is written to the pool."""
+    import torch
+
+    from kvboost_b200.flash_attn_ext import _make_paged_attn_fn
+    fn = _make_paged_attn_fn(0, {"allocator": None, "slots": torch.zeros(1, dtype=torch.int32)})
+    x = torch.zeros(1, 2, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(NotImplementedError, match="sliding-window"):
+        fn(None, x, x, x, **kw)
