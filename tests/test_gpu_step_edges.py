@@ -178,3 +178,108 @@ def test_attention_into_the_query_and_into_other_layouts(lens):
     assert torch.equal(paged_decode_attention(q, *args, out=turned)[0], want)
     with pytest.raises(Exception, match="overlap"):
         paged_decode_attention(q, *args, out=torch.empty(1, 8, 1, 64, dtype=q.dtype, device=DEV).expand(3, -1, -1, -1))
+
+
+def _scene(g, B, H, group, D, dtype, int8, width, most):
+    """Fixed buffers of a captured call and a function that fills them anew."""
+    nb = B * width if B * width < 4000 else 4000
+    pool = torch.zeros(nb, 2, H, 16, D, dtype=torch.int8 if int8 else dtype, device=DEV)
+    ks = torch.zeros(nb, H, 16, dtype=torch.float16, device=DEV) if int8 else None
+    vs = torch.zeros(nb, H, D, dtype=torch.float16, device=DEV) if int8 else None
+    q = torch.zeros(B, H * group, 1, D, dtype=dtype, device=DEV)
+    tables = torch.zeros(B, width, dtype=torch.int32, device=DEV)
+    lens = torch.zeros(B, dtype=torch.int32, device=DEV)
+
+    def fill(i):
+        n = torch.randint(0, most + 1, (B,), generator=g)
+        n[i % B] = most if i % 3 else 1           # a long row that moves, and replays without one
+        n[(i + 1) % B] = 0
+        lens.copy_(n.to(torch.int32))
+        tables.copy_(torch.stack([torch.randperm(nb, generator=g)[:width] for _ in range(B)]).to(torch.int32))
+        q.copy_(torch.randn(q.shape, generator=g))
+        if int8:
+            pool.copy_(torch.randint(-127, 128, pool.shape, generator=g))
+            ks.copy_((0.5 + torch.rand(ks.shape, generator=g)) / 64)
+            vs.copy_((0.5 + torch.rand(vs.shape, generator=g)) / 64)
+        else:
+            pool.copy_(torch.randn(pool.shape, generator=g))
+
+    return (q, pool, tables, lens, ks, vs), fill
+
+
+def _expect(o, lse, args):
+    from test_gpu_step_ops import _check_attention
+    q, pool, tables, lens, ks, vs = (None if t is None else t.cpu() for t in args)
+    _check_attention(o, lse, q, pool, tables, lens.tolist(), 1 / math.sqrt(q.shape[-1]), ks, vs)
+
+
+@pytest.mark.parametrize("B,H,group,D,dtype,int8", [
+    (2, 1, 4, 64, torch.bfloat16, False), (3, 2, 12, 96, torch.float16, False), (3, 2, 8, 128, torch.bfloat16, True),
+    (40, 1, 2, 64, torch.float16, True), (300, 1, 1, 64, torch.bfloat16, False)])
+def test_split_launch_replayed_with_other_inputs(B, H, group, D, dtype, int8):
+    """A captured call whose items span CTAs, its queries, lengths, tables and pool new at every replay and
+    its results wiped before: each replay's results are its own."""
+    from kvboost_b200.paged_decode import paged_decode_attention
+    g = torch.Generator().manual_seed(B + D)
+    args, fill = _scene(g, B, H, group, D, dtype, int8, 200, 3200 if B < 100 else 600)
+    fill(0)
+    paged_decode_attention(*args[:4], k_scale=args[4], v_scale=args[5])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, lse = paged_decode_attention(*args[:4], k_scale=args[4], v_scale=args[5])
+    for i in range(6):
+        fill(i)
+        o.fill_(float("nan"))
+        lse.fill_(float("nan"))
+        graph.replay()
+        _expect(o, lse, args)
+
+
+def test_two_split_graphs_on_two_streams_with_other_inputs():
+    """As above, both graphs in flight at once."""
+    from kvboost_b200.paged_decode import paged_decode_attention
+    g = torch.Generator().manual_seed(5)
+    sides = []
+    for H, D in ((2, 128), (1, 64)):
+        args, fill = _scene(g, 2, H, 8, D, torch.bfloat16, False, 200, 3200)
+        fill(0)
+        paged_decode_attention(*args[:4])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o, lse = paged_decode_attention(*args[:4])
+        sides.append((graph, torch.cuda.Stream(), o, lse, args, fill))
+    for i in range(8):
+        for _, _, o, lse, _, fill in sides:
+            fill(i)
+            o.fill_(float("nan"))
+            lse.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for graph, stream, *_ in sides:
+            with torch.cuda.stream(stream):
+                for _ in range(3):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for _, _, o, lse, args, _ in sides:
+            _expect(o, lse, args)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 96, 128])
+@pytest.mark.parametrize("H,group", [(1, 9), (2, 12), (1, 16), (1, 17)])
+@pytest.mark.parametrize("lens", [[300, 0, 17, 1000], [2500, 0, 17, 33]])
+def test_groups_above_eight(lens, H, group, D, dtype, int8):
+    """16 query heads an item, every width and type, a CTA an item (tables of up to 64 blocks) and split."""
+    from test_gpu_step_ops import _check_attention, _pool
+
+    from kvboost_b200.paged_decode import paged_decode_attention
+    g = torch.Generator().manual_seed(D + group)
+    pool, tables, ks, vs = _pool(g, lens, H, D, dtype, int8)
+    if max(lens) <= 1000:
+        tables = tables[:, :64].contiguous()
+    q = torch.randn(len(lens), H * group, 1, D, generator=g).to(dtype)
+    c = lambda t: None if t is None else t.cuda()  # noqa: E731
+    o, lse = paged_decode_attention(c(q), c(pool), c(tables), _i32(lens), k_scale=c(ks), v_scale=c(vs))
+    _check_attention(o, lse, q, pool, tables, lens, 1 / math.sqrt(D), ks, vs)
