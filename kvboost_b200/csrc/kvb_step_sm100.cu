@@ -627,6 +627,14 @@ extern "C" int kvb_append_paged_kv(const KvbAppendPagedParams* p, void* stream) 
   if (p->k_token_stride % 8 || p->k_head_stride % 8 || p->v_token_stride % 8 ||
       p->v_head_stride % 8)
     return fail(KVB_ERR_INVALID, "strides must be multiples of 8 elements");
+  const int64_t pool_bytes = (int64_t)p->num_blocks * 2 * p->num_kv_heads * 16 * p->head_dim * 2;
+  const auto in_pool = [&](const void* src, int64_t token_stride, int64_t head_stride) {
+    const int64_t from = (int64_t)reinterpret_cast<uintptr_t>(src), pool = (int64_t)reinterpret_cast<uintptr_t>(p->kv_pool);
+    const int64_t last = (p->num_tokens - 1) * token_stride + (p->num_kv_heads - 1) * head_stride + p->head_dim;
+    return from < pool + pool_bytes && pool < from + last * 2;
+  };
+  if (in_pool(p->k_new, p->k_token_stride, p->k_head_stride) || in_pool(p->v_new, p->v_token_stride, p->v_head_stride))
+    return fail(KVB_ERR_INVALID, "k_new and v_new must not overlap kv_pool");
   const int vecs = p->head_dim / 8;
   const int64_t pieces = (int64_t)p->num_tokens * p->num_kv_heads * vecs;
   if (pieces >= (1ll << 31) - 1024 * 256)

@@ -190,7 +190,8 @@ def append_paged_kv(k_new: torch.Tensor, v_new: torch.Tensor, kv_pool: torch.Ten
     read in place through its transpose) in the pool's dtype; ``kv_pool``: one layer's
     ``[num_blocks, 2, Hkv, 16, D]`` (``DeviceBlockAllocator.pools[layer]``); ``slots``: int32
     ``[T]`` from ``extend_block_tables``, all different, -1 where a token is not stored.
-    Slots outside the pool are skipped and set ``KVB_STATUS_BAD_BLOCK``.
+    Slots outside the pool are skipped and set ``KVB_STATUS_BAD_BLOCK``.  Sources inside the pool
+    itself are refused.
     """
     _check_tensor("k_new", k_new, 3)
     _check_tensor("v_new", v_new, 3)

@@ -50,3 +50,13 @@ def test_decode_takes_results_whose_heads_do_not(lib, batch, heads, batch_stride
     p = _lib.KvbPagedDecodeParams(0, 128, batch, heads, 1, 16, 1, 0.1, at, at, at, 1024, 128, batch_stride, head_stride, 8,
                                   at, None, None, 10, 4, 4, at, at, 0, 0, at, None, 0)
     assert lib.kvb_paged_decode_workspace_bytes(ctypes.byref(p)) == 0
+
+
+@pytest.mark.parametrize("field,at", [("k_new", 0), ("v_new", 0), ("k_new", -16), ("v_new", 10 * 2 * 2 * 16 * 128 * 2 - 16)])
+def test_append_refuses_sources_inside_the_pool(lib, field, at):
+    """A pool of 10 blocks, 2 heads of 128; 3 tokens whose vectors lie in it, or reach into it."""
+    pool = 1 << 24
+    p = _lib.KvbAppendPagedParams(128, 2, 3, 10, 4096, 4096, 256, 128, 256, 128, pool, 4096, 4096)
+    setattr(p, field, pool + at)
+    assert lib.kvb_append_paged_kv(ctypes.byref(p), None) == _lib.KVB_ERR_INVALID
+    assert "overlap" in lib.kvb_last_error().decode()
