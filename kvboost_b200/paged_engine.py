@@ -37,6 +37,7 @@ logits on the device (``paged_decode``, ``logits``).
 
 from __future__ import annotations
 
+import threading
 import time
 from typing import Callable, Dict, List, Optional, Sequence, Tuple, Union
 
@@ -77,6 +78,7 @@ class PagedEngine(KVBoost):
                                               device=self.device, dtype=dt)
         self.chunk_mapper = DeviceChunkMapper(self.allocator)
         self._num_layers, self._block_size = L, block_size
+        self._stepping = threading.Lock()    # held while the model's attention is a batched step's
         store_evict = self.store.on_evict
 
         def on_evict(chunk):      # chunk blocks leave the pool with the chunk (:124-126)
@@ -90,6 +92,8 @@ class PagedEngine(KVBoost):
                  temperature: float = 1.0, do_sample: bool = False,
                  cacheable_prefix_len: Optional[int] = None) -> GenerationResult:
         mode = GenerationMode(mode)
+        if self._stepping.locked():
+            raise RuntimeError("generate_paged is running on this engine")
         if mode == GenerationMode.BASELINE:
             return super().generate(prompt, max_new_tokens, mode, temperature, do_sample)
         self._sync()
@@ -212,8 +216,22 @@ class PagedEngine(KVBoost):
         (None: any).  A prompt that has met the end id keeps its place in the steps until
         all have ended.  The blocks of the longest outputs are reserved before the first
         step and returned at the end; the prompts' new chunks are then stored.  A step that the
-        device refused a part of (``ops.read_status``) raises.
+        device refused a part of (``ops.read_status``) raises, and so does a call while another
+        runs on the engine (from ``allowed_tokens``, or from another thread): its steps would
+        go through the other's tables.
         """
+        if not self._stepping.acquire(blocking=False):
+            raise RuntimeError("generate_paged is running on this engine")
+        try:
+            return self._generate_paged(prompts, max_new_tokens, temperature, do_sample,
+                                        repetition_penalty, frequency_penalty, presence_penalty,
+                                        logit_bias, allowed_tokens)
+        finally:
+            self._stepping.release()
+
+    def _generate_paged(self, prompts, max_new_tokens, temperature, do_sample, repetition_penalty,
+                        frequency_penalty, presence_penalty, logit_bias,
+                        allowed_tokens) -> List[GenerationResult]:
         if self.allocator.dtype != next(self.model.parameters()).dtype:
             raise RuntimeError("generate_paged needs a pool in the model's dtype")
         if not prompts:

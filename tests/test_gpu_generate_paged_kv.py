@@ -78,13 +78,14 @@ def _equal(pool, prefill, prompts):
             assert k.shape[1] == len(p) and torch.equal(k, kk) and torch.equal(v, vv)
 
 
-@pytest.mark.parametrize("chunk_size", [40, 24, 16, 33, 128])
-def test_the_pool_holds_what_the_prefill_saw(monkeypatch, chunk_size):
+@pytest.mark.parametrize("chunk_size,bits", [(40, 16), (24, 16), (16, 16), (33, 16), (128, 16), (128, 8), (32, 8)])
+def test_the_pool_holds_what_the_prefill_saw(monkeypatch, chunk_size, bits):
     """Chunks that fill their blocks and chunks that do not, two or more of them reused, one prompt
     without reuse and one fully cached."""
     from kvboost_b200.paged_engine import PagedEngine
     prompts = _prompts([300, 256, 5, 281, 80], 256)
-    eng = PagedEngine(_model(), num_blocks=256, chunk_size=chunk_size, min_chunk_tokens=8, recompute_strategy="none")
+    eng = PagedEngine(_model(), num_blocks=256, chunk_size=chunk_size, min_chunk_tokens=8, recompute_strategy="none",
+                      kv_cache_bits=bits)
     eng.warm(prompts[0][:256])
     for _ in range(2):                       # the second time the prompts' own chunks are cached too
         got, pool, prefill, _ = _pool_and_prefill(eng, prompts, monkeypatch, max_new_tokens=3)
@@ -245,3 +246,36 @@ def test_a_refused_step_raises(monkeypatch):
         eng.generate_paged([p[:-1] + [7] for p in prompts], max_new_tokens=4)
     assert ops.read_status(dev) == 16
     assert eng.allocator.used_blocks == eng.chunk_mapper.blocks_used_by_chunks()
+
+
+def test_one_call_at_a_time():
+    """Calls from ``allowed_tokens`` and from another thread are refused, and the outer one's tokens are
+    those of a call on its own."""
+    import threading
+
+    from kvboost_b200.paged_engine import PagedEngine
+    eng = PagedEngine(_model(), num_blocks=64, chunk_size=32, min_chunk_tokens=8)
+    prompts = _prompts([50], 0)
+    eng.warm(prompts[0])                      # every call reuses the same chunks
+    want = eng.generate_paged(prompts, max_new_tokens=6)[0].generated_ids
+    refused = []
+
+    def attempt(call):
+        try:
+            call()
+        except RuntimeError as e:
+            refused.append("running" in str(e))
+
+    def allowed(i, out):
+        calls = [lambda: eng.generate_paged(prompts, 3), lambda: eng.generate(prompts[0], 3),
+                 lambda: eng.generate([5], 2, mode="baseline")]
+        for call in calls:
+            attempt(call)
+        t = threading.Thread(target=attempt, args=(calls[0],))
+        t.start()
+        t.join()
+        return None
+
+    got = eng.generate_paged(prompts, max_new_tokens=6, allowed_tokens=allowed)[0].generated_ids
+    assert got == want and refused == [True] * 24
+    assert eng.generate_paged(prompts, max_new_tokens=6)[0].generated_ids == want
