@@ -31,10 +31,10 @@
 // channel): the dequantised values are never rounded.
 //
 // Measured (B200, us per call in a CUDA graph, of the measured 6.48 TB/s copy): 64 requests of
-// 700 .. 16381 tokens, 32/8 heads, D 128, bfloat16: 206 (6.3 TB/s, 97 %); 8 x 4096, 16/2 heads:
-// 14.4 (start, joins); int8 4 x 32768, 64/8 heads: 60.6 (4.7 TB/s, 73 %; 56.6 with the weights'
-// high halves alone, which under bfloat16 left 2.5 % of the outputs a step off); 24 requests of 1 .. 2051 tokens, 32 heads of D 96, float16: 23.3
-// (3.8 TB/s).
+// 700 .. 16381 tokens, 32/8 heads, D 128, bfloat16: 203 to 207 (6.3 to 6.4 TB/s, 97 to 99 %); 8 x 4096,
+// 16/2 heads: 14.6 (start, joins); int8 4 x 32768, 64/8 heads: 60.3 (4.8 TB/s, 74 %; 56.5 with the
+// weights' high halves alone, which under bfloat16 left 2.5 % of the outputs a step off); 24 requests
+// of 1 .. 2051 tokens, 32 heads of D 96, float16: 23.1 (3.9 TB/s).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -66,14 +66,15 @@ constexpr uint64_t kWaitNs = 2000000000ull;
 // when it is passed by 2^8.  A float16 half has nothing below 2^-25, so there the weights lie as high
 // as 2^15 and the maximum's own at 2^11 or above: what is lost lies below 2^-36 of the largest (2^-25
 // without the lift: 2000 tokens of weight 2^-26 and V 60000 beside some of weight 1 were all lost).
+// Raising at every new maximum instead: int8 4 x 32768 tokens 61.2 us, 60.3 so.
 template <typename E> constexpr float kLift = std::is_same<E, __half>::value ? 11.f : 0.f;
 template <typename E> constexpr float kTop = std::is_same<E, __half>::value ? 15.f : 8.f;
 // Warps per CTA, as registers allow.  Items of up to 8 heads: 64 requests of 700 .. 16381 tokens in
 // bfloat16 took 211 us with 8 warps of three stages, 209 with 10, 206 with 12 of two; int8 4 x
-// 32768 tokens, 64/8 heads: 65.0 with 8, 63.4 with 10, 57.0 with 12, 60.6 with 14, 60.5 with 16
-// (which spill).  D 64 needs fewer registers: 16 warps instead of 12 took 32 x 16384 tokens, 8 KV
-// heads, from 6.28 to 6.43 TB/s, 64 x 16384 in int8 from 4.36 to 4.96.  Items of 16 heads hold twice
-// the accumulators: 8 warps (10: 5.81 TB/s instead of 5.89), 12 for int8 of D 64 (3.68, with 8 2.94).
+// 32768 tokens, 64/8 heads: 68.3 with 10, 60.3 with 12, 66.4 with 14, 65.9 with 16 (which spill).
+// D 64 needs fewer registers: 16 warps instead of 12 took 32 x 16384 tokens, 8 KV
+// heads, from 6.28 to 6.43 TB/s, 64 x 16384 in int8 from 4.32 to 4.61.  Items of 16 heads hold twice
+// the accumulators: 8 warps (10: 5.81 TB/s instead of 5.89), 12 for int8 of D 64 (3.12, with 8 2.65).
 constexpr int warps_of(int D, bool i8, int tiles8) {
   return tiles8 == 1 ? (D == 64 ? 16 : 12) : (D == 64 && i8 ? 12 : 8);
 }
@@ -89,8 +90,8 @@ constexpr int kSpan = 64;
 // Most blocks of an item that a share's end does not cut, one warp taking all of it: kShort, more
 // where the shares are long enough for the uneven ends not to show (kShort 2 up to four shares,
 // uncut_of up to two).  D 128, cut and joined / whole: 640 items of 64 tokens 10.3 us / 7.3, of 256
-// 21.6 / 17.3 (8 heads 26.4 / 17.6); 2368 of 64 24.8 / 18.3 (int8 27.2 / 18.0), of 256 63.9 /
-// 53.8 (48.3 / 42.6), of 512 104.9 / 99.8 (67.5 / 69.3).  With shares of less than two blocks
+// 21.6 / 17.3 (8 heads 26.4 / 17.6); 2368 of 64 24.8 / 18.3 (int8 27.5 / 18.6), of 256 63.9 /
+// 53.8 (50.5 / 45.7), of 512 104.9 / 99.8 (71.1 / 74.2).  With shares of less than two blocks
 // the cut is better: 128 items of 256 tokens 12.8 / 15.7.
 constexpr int kShort = 8;
 constexpr int uncut_of(bool i8) { return i8 ? 16 : 32; }
@@ -1111,7 +1112,7 @@ int64_t items(const KvbPagedDecodeParams* p) {
 // heads x requests = items, D 128, 16 bits: 2 items of 256 tokens 5.1 / 7.7, of 1024 9.2 / 8.0,
 // of 2048 15.0 / 8.9; 32 of 1024 9.7 / 12.4; 128 of 2048 25.0 / 31.5; 256 of 64 7.0 / 6.7, of 256
 // 12.9 / 15.9; 512 of 64 13.0 / 7.4, of 256 24.8 / 18.8, of 512 35.1 / 34.5, of 1024 51.8 / 54.2,
-// of 2048 84.9 / 93.5.  int8: 256 of 1024 24.9 / 26.6; 512 of 256 27.1 / 22.8, of 1024 45.6 / 41.5.
+// of 2048 84.9 / 93.5.  int8: 256 of 1024 25.7 / 27.9; 512 of 256 24.5 / 24.5, of 1024 41.9 / 41.8.
 bool split(const KvbPagedDecodeParams* p) {
   if (p->batch > kSplitRows) return false;
   // 32-bit places: wider than any pool

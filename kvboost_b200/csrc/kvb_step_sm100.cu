@@ -341,11 +341,12 @@ constexpr int kCounts16 = 16383;          // the longest history that a 16-bit n
 // spread over the GPU.  The stream's own work has to stay small beside 6 bytes a token: with the
 // penalties' divisions and the bias list in the unrolled stream it took 124 us for 192 rows of
 // 151936, waiting for instructions; with 32-bit notes of shorter slices, all of a thread's logits
-// in registers, 68 us; so 37.4 us (4.8 TB/s; 28 us and 6.3 TB/s with the mask alone), what the
+// in registers, 68 us; so 37.9 us (4.7 TB/s; 28.4 us and 6.3 TB/s with the mask alone), what the
 // notes cost being the two barriers with the wait for the history before the first turn, and the
 // branches of noted tokens.  A list of the noted tokens, worked on behind the stream, took
 // longer (45 us).  The quotients by the repetition penalty and the temperature are products with
-// their reciprocals: one more rounding of float32 each.
+// their reciprocals: one more rounding of float32 each (3.5e-8 from the 64-bit result instead of
+// 2.5e-8 in the 2-norm); with divisions an eager call takes 47.3 us instead of 38.9.
 //
 // G 8: rows on 8 values.  G 4: rows on 4 without notes (12.5 us for 150 rows of 100000, 13.5 with
 // G 8).  G 1: other rows, odd vocabularies (150 of 100001: 25.4 us with notes, 18.8 for 100000).
@@ -524,9 +525,9 @@ bool rows_meet(const void* p, int64_t n, int64_t step, const void* q, int64_t m,
 
 template <typename TI, typename TO>
 void launch_logits(LogitsArgs a, int batch, cudaStream_t s) {
-  // Slices of up to 8192 tokens, as long as every SM gets two CTAs (192 x 151936: 34.7 us with
-  // 8192, 38.9 with 16384, 38.7 with 4096; 16 x 128000: 5.1 us with 4096, 6.5 with 2048, 5.8 with
-  // 8192), 4096 without notes (192 x 151936: 28.3 us, 29.7 with 8192).
+  // Slices of up to 8192 tokens, as long as every SM gets two CTAs (192 x 151936: 37.9 us with
+  // 8192, 41.5 with 16384, 43.8 with 4096; 16 x 128000: 6.0 us with 4096, 7.0 with 2048, 7.8 with
+  // 8192), 4096 without notes (192 x 151936: 28.3 us, 27.6 with 2048, 29.5 with 8192).
   for (a.iters = a.token_ids || a.bias_ids ? 4 : 2; a.iters > 1; a.iters /= 2)
     if ((int64_t)batch * ((a.vocab + a.iters * 2048 - 1) / (a.iters * 2048)) >= 2 * 148) break;
   const dim3 grid((a.vocab + a.iters * 2048 - 1) / (a.iters * 2048), batch);

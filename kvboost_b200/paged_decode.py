@@ -238,7 +238,8 @@ def paged_decode_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_tables:
 
     q: ``[B, Hq, 1, D]``; ``kv_pool``: one layer's ``[num_blocks, 2, Hkv, 16, D]`` in q's
     dtype, or int8 with its float16 scales ``k_scale [num_blocks, Hkv, 16]`` and ``v_scale
-    [num_blocks, Hkv, D]`` (``DeviceBlockAllocator.k_scale16`` / ``v_scale16``);
+    [num_blocks, Hkv, D]`` (``DeviceBlockAllocator.k_scale16`` / ``v_scale16``; such a pool holds
+    whole KIVI chunks and takes no single tokens, so the rows attend to reused chunks alone);
     ``block_tables``: int32 ``[B, max_blocks]``; ``seq_lens``: int32 ``[B]`` device tensor, the
     tokens row b attends to (its own included, once appended).  ``Hq % Hkv == 0``.
     Returns ``(o [B, Hq, 1, D] in q's dtype, lse float32 [B, Hq, 1] or None)``; a row of
