@@ -216,7 +216,8 @@ class PagedEngine(KVBoost):
         (None: any).  A prompt that has met the end id keeps its place in the steps until
         all have ended.  The blocks of the longest outputs are reserved before the first
         step and returned at the end; the prompts' new chunks are then stored.  A step that the
-        device refused a part of (``ops.read_status``) raises, and so does a call while another
+        device refused a part of (``ops.read_status``; the word is the device's, so a report of
+        other work on it counts) raises, and so does a call while another
         runs on the engine (from ``allowed_tokens``, or from another thread): its steps would
         go through the other's tables.
         """
